@@ -35,6 +35,7 @@ extern "C" {
 #define W4J_GGML_F32 0
 #define W4J_GGML_F16 1
 #define W4J_GGML_Q8_0 8
+#define W4J_GGML_BF16 30 /* operands of the paged cache and of the 8-bit integer products only */
 
 /* W4J/model/ModelDimensions.java:6-17, same field order. */
 typedef struct w4j_dims {
@@ -316,6 +317,77 @@ int w4j_test_withhold_logits_copies(int n_launches);
 int w4j_op_logits_argmax_noalloc(int device, const float *x, int M, int d, const void *E, int V,
                                  const float *ln_g, const float *ln_b, int32_t *out_token, double *out_logprob,
                                  void *stream);
+
+/* ---------------------------------------------------------------------------
+ * A paged key/value cache for hosts that drive their own loop (no counterpart in the reference, whose
+ * kvCache map copies and concatenates, W4J/nn/MultiHeadAttention.java:140-164).  Rows (sequences) hold
+ * pages of page_tokens tokens; a page may be held by many rows, so beams of a stream and re-decodes of a
+ * window keep their common prompt once.  All memory is the caller's, on `device`:
+ *
+ *   pool    [2 n_layer][n_pages][n_kv_head][page_tokens][head_dim], F16 or BF16, 16-byte aligned; plane 2 l
+ *           holds the keys of layer l, plane 2 l + 1 its values
+ *   ref     [n_pages] rows that hold each page (0: free)
+ *   table   [n_rows][table_width] page of each run of page_tokens tokens; entries behind a row's length
+ *           are neither read nor written
+ *   len     [n_rows] tokens of each row
+ *   status  [1] what calls could not do, W4J_PAGES_* bits, added up until the caller clears it
+ *   work    w4j_op_pages_workspace() bytes of scratch that this cache's calls share
+ *
+ * A new cache is ref, len and status set to zero.  A last page that is not full belongs to one row alone:
+ * every call here keeps that so, and a caller that builds tables of its own has to.
+ *
+ * The calls are asynchronous on `stream` and change the cache in stream order; calls on one cache that
+ * may run at the same time (several streams without an event between them) are the caller's to order, and
+ * so are replays of graphs that hold them.  The integer arguments (rows, start, dst, src) are device arrays
+ * that must stay as they are until the call has run.  Each call is all or nothing: where a row is out of
+ * range or named twice, a length does not fit or the free pages do not suffice, it changes nothing but
+ * `status`.  New pages are the lowest free ones in the order of the call's rows; pages that a call lets go
+ * of are free for the next call.  page_tokens is a multiple of 8 up to 1024, head_dim 64 or 128.
+ * ------------------------------------------------------------------------- */
+#define W4J_PAGES_BAD_ROW 1   /* a row out of range, or named twice by one call */
+#define W4J_PAGES_FULL 2      /* too few free pages */
+#define W4J_PAGES_TOO_LONG 4  /* a row would outgrow its table */
+#define W4J_PAGES_BAD_START 8 /* start does not begin at 0, does not ascend or does not fit the row lengths */
+#define W4J_PAGES_BAD_PAGE 16 /* a table entry out of range, or one whose page nobody holds */
+
+typedef struct w4j_pages {
+    int32_t device;
+    int32_t type;                /* of the pool: W4J_GGML_F16 or W4J_GGML_BF16 */
+    int32_t n_layer, n_kv_head, head_dim, page_tokens, n_pages, n_rows, table_width;
+    void *pool;
+    int32_t *ref, *table, *len, *status;
+    void *work;
+    size_t work_bytes;
+} w4j_pages;
+
+/* Bytes of scratch (16-byte aligned) that a cache of these sizes needs; 0 where the sizes are refused. */
+size_t w4j_op_pages_workspace(const w4j_pages *cache);
+
+/* Row rows[i] grows by start[i + 1] - start[i] tokens (start: n + 1 ascending numbers from 0), whose keys
+ * and values w4j_op_pages_write brings layer by layer. */
+int w4j_op_pages_extend(const w4j_pages *cache, const int32_t *rows, const int32_t *start, int n, void *stream);
+
+/* Keys and values of the last start[i + 1] - start[i] tokens of row rows[i], as tokens start[i] ..
+ * start[i + 1] - 1 of k and v (n_tokens = start[n] tokens of [n_kv_head][head_dim], k_stride and v_stride
+ * elements apart, multiples of 8, both 16-byte aligned: the K and V parts of a fused projection can stay in
+ * place).  After w4j_op_pages_extend of the same rows and start.  A token whose row or page is out of range
+ * is left out and raises its status bit. */
+int w4j_op_pages_write(const w4j_pages *cache, int layer, const int32_t *rows, const int32_t *start, int n,
+                       const void *k, int64_t k_stride, const void *v, int64_t v_stride, int n_tokens, void *stream);
+
+/* Row dst[i] becomes what row src[i] was before the call, for all i at once (a beam reorder, or new
+ * beams off one row); src[i] = -1 empties dst[i].  Full pages are shared.  A last page that is not full stays
+ * with one holder (the source row if it goes on, else the lowest i that takes it over) and is copied, as far
+ * as it is filled, to a new page for every other. */
+int w4j_op_pages_fork(const w4j_pages *cache, const int32_t *dst, const int32_t *src, int n, void *stream);
+
+/* The rows become empty; pages that nobody else holds become free. */
+int w4j_op_pages_free(const w4j_pages *cache, const int32_t *rows, int n, void *stream);
+
+/* Moves the held pages to the front of the pool: with n of them held, the i-th lowest free page below n
+ * takes over the i-th lowest held page from n on, in the tables of all rows too.  n_live (device, may be
+ * NULL) gets n: pages n .. n_pages - 1 are free afterwards and may be cut off. */
+int w4j_op_pages_compact(const w4j_pages *cache, int32_t *n_live, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,110 @@
+"""Refusals of the op-level operators: every argument check that needs no device (dummy pointers, no launch)."""
+import ctypes
+
+import pytest
+
+from whisper4j_b200 import _lib
+from whisper4j_b200._lib import GGML_BF16, GGML_F16, GGML_F32, W4J_ERR_ARG, W4J_ERR_CUDA, W4J_OK, Pages, lib
+
+P = 4096  # an aligned dummy address; refused calls never reach it
+
+
+def cache(**kw):
+    f = dict(device=0, type=GGML_F16, n_layer=2, n_kv_head=3, head_dim=64, page_tokens=16, n_pages=10, n_rows=4,
+             table_width=5, pool=P, ref=P, table=P, len=P, status=P, work=P, work_bytes=1 << 30)
+    f.update(kw)
+    return Pages(**f)
+
+
+def refused(rc, text):
+    assert rc == W4J_ERR_ARG, lib().w4j_last_error()
+    assert text in lib().w4j_last_error().decode()
+
+
+BAD_CACHES = [(dict(type=GGML_F32), "type"), (dict(head_dim=96), "head_dim"), (dict(page_tokens=0), "page_tokens"),
+              (dict(page_tokens=12), "page_tokens"), (dict(page_tokens=1032), "page_tokens"), (dict(n_layer=0), "n_layer"),
+              (dict(n_kv_head=-1), "n_kv_head"), (dict(n_pages=0), "n_pages"), (dict(n_pages=(1 << 21) + 1), "n_pages"),
+              (dict(n_rows=0), "n_rows"), (dict(table_width=0), "table_width"),
+              (dict(table_width=1 << 27), "table_width"),
+              (dict(n_pages=1 << 21, n_kv_head=128, page_tokens=16), "2^32")]
+BAD_POINTERS = [(dict(pool=None), "null"), (dict(ref=None), "null"), (dict(table=None), "null"), (dict(len=None), "null"),
+                (dict(status=None), "null"), (dict(work=None), "null"), (dict(pool=P + 8), "aligned"),
+                (dict(work=P + 4), "aligned"), (dict(work_bytes=100), "work")]
+
+
+@pytest.mark.parametrize("kw,text", BAD_CACHES)
+def test_workspace_refuses_sizes(kw, text):
+    assert lib().w4j_op_pages_workspace(ctypes.byref(cache(**kw))) == 0
+    assert text in lib().w4j_last_error().decode()
+
+
+def test_workspace_grows_with_the_cache():
+    small = lib().w4j_op_pages_workspace(ctypes.byref(cache(pool=None, work=None)))
+    assert 0 < small < lib().w4j_op_pages_workspace(ctypes.byref(cache(n_rows=8))) < 1 << 16
+    assert lib().w4j_op_pages_workspace(None) == 0
+
+
+@pytest.mark.parametrize("kw,text", BAD_CACHES + BAD_POINTERS)
+def test_every_call_refuses_a_bad_cache(kw, text):
+    c, L = ctypes.byref(cache(**kw)), lib()
+    refused(L.w4j_op_pages_extend(c, P, P, 1, None), text)
+    refused(L.w4j_op_pages_write(c, 0, P, P, 1, P, 192, P, 192, 1, None), text)
+    refused(L.w4j_op_pages_fork(c, P, P, 1, None), text)
+    refused(L.w4j_op_pages_free(c, P, 1, None), text)
+    refused(L.w4j_op_pages_compact(c, None, None), text)
+
+
+def test_row_lists():
+    c, L = ctypes.byref(cache()), lib()
+    for n in (-1, 5):
+        refused(L.w4j_op_pages_extend(c, P, P, n, None), "rows")
+        refused(L.w4j_op_pages_write(c, 0, P, P, n, P, 192, P, 192, 1, None), "rows")
+        refused(L.w4j_op_pages_fork(c, P, P, n, None), "rows")
+        refused(L.w4j_op_pages_free(c, P, n, None), "rows")
+    refused(L.w4j_op_pages_extend(c, P, None, 1, None), "null")
+    refused(L.w4j_op_pages_fork(c, None, P, 1, None), "null")
+    refused(L.w4j_op_pages_free(c, None, 1, None), "null")
+    refused(L.w4j_op_pages_extend(None, P, P, 1, None), "null")
+    # nothing to do is no error, and needs no device
+    assert L.w4j_op_pages_extend(c, None, None, 0, None) == W4J_OK
+    assert L.w4j_op_pages_fork(c, None, None, 0, None) == W4J_OK
+    assert L.w4j_op_pages_free(c, None, 0, None) == W4J_OK
+    assert L.w4j_op_pages_write(c, 0, P, P, 1, None, 0, None, 0, 0, None) == W4J_OK
+
+
+@pytest.mark.parametrize("layer,k,ks,v,vs,tokens,text", [
+    (-1, P, 192, P, 192, 1, "layer"), (2, P, 192, P, 192, 1, "layer"), (0, P, 192, P, 192, -1, "n_tokens"),
+    (0, None, 192, P, 192, 1, "null"), (0, P, 192, None, 192, 1, "null"), (0, P, 184, P, 192, 1, "strides"),
+    (0, P, 192, P, 196, 1, "strides"), (0, P, -192, P, 192, 2, "strides"), (0, P + 2, 192, P, 192, 1, "aligned"),
+    (0, P, 192, P + 8, 192, 1, "aligned")])
+def test_write_refusals(layer, k, ks, v, vs, tokens, text):
+    refused(lib().w4j_op_pages_write(ctypes.byref(cache()), layer, P, P, 1, k, ks, v, vs, tokens, None), text)
+
+
+def test_bf16_is_a_cache_type():
+    assert lib().w4j_op_pages_workspace(ctypes.byref(cache(type=GGML_BF16, head_dim=128))) > 0
+
+
+def test_a_device_that_is_not_there():
+    if _has_gpu():
+        refused(lib().w4j_op_pages_free(ctypes.byref(cache(device=99)), P, 1, None), "device 99")
+        refused(lib().w4j_op_pages_free(ctypes.byref(cache(device=-1)), P, 1, None), "device -1")
+    else:
+        assert lib().w4j_op_pages_free(ctypes.byref(cache()), P, 1, None) == W4J_ERR_CUDA
+
+
+def _has_gpu():
+    torch = pytest.importorskip("torch")
+    return torch.cuda.is_available()
+
+
+def test_python_cache_refuses_host_tensors():
+    torch = pytest.importorskip("torch")
+    from whisper4j_b200 import ops
+    i = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.PagedCache.from_tensors(torch.zeros(2, 4, 2, 16, 64, dtype=torch.float16), i, i.view(4, 1), i)
+    with pytest.raises(ValueError, match="pool"):
+        ops.PagedCache.from_tensors(torch.zeros(2, 4, 2, 16, 64), i, i.view(4, 1), i)
+    with pytest.raises(ValueError, match="positive"):
+        ops.PagedCache(1, 2, 64, 0, 16, 4, 64, device="cpu")

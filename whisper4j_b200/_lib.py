@@ -19,7 +19,9 @@ W4J_ERR_CUDA = -3
 W4J_ERR_OOM = -4
 W4J_ERR_CANCELLED = -5
 
-GGML_F32, GGML_F16, GGML_Q8_0 = 0, 1, 8
+GGML_F32, GGML_F16, GGML_Q8_0, GGML_BF16 = 0, 1, 8, 30
+
+PAGES_BAD_ROW, PAGES_FULL, PAGES_TOO_LONG, PAGES_BAD_START, PAGES_BAD_PAGE = 1, 2, 4, 8, 16
 
 
 class W4jError(RuntimeError):
@@ -68,8 +70,16 @@ class Result(ctypes.Structure):
                 ("compression", ctypes.POINTER(ctypes.c_float)), ("no_speech_prob", ctypes.POINTER(ctypes.c_float))]
 
 
+class Pages(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "device", "type", "n_layer", "n_kv_head", "head_dim", "page_tokens", "n_pages", "n_rows", "table_width")] + [
+        (n, ctypes.c_void_p) for n in ("pool", "ref", "table", "len", "status", "work")] + [
+        ("work_bytes", ctypes.c_size_t)]
+
+
 # every symbol declared in include/whisper4j_cuda.h: name -> (restype, argtypes)
 _P, _I, _F, _D, _U64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_double, ctypes.c_uint64
+_I64, _SZ = ctypes.c_int64, ctypes.c_size_t
 SIGNATURES = {
     "w4j_last_error": (ctypes.c_char_p, []),
     "w4j_version": (ctypes.c_char_p, []),
@@ -101,6 +111,12 @@ SIGNATURES = {
     "w4j_op_logits_argmax": (_I, [_P, _P, _I, _P, _I, _P, _P, _P, _P, _P]),
     "w4j_op_logits_argmax_noalloc": (_I, [_I, _P, _I, _I, _P, _I, _P, _P, _P, _P, _P]),
     "w4j_test_withhold_logits_copies": (_I, [_I]),
+    "w4j_op_pages_workspace": (_SZ, [_P]),
+    "w4j_op_pages_extend": (_I, [_P, _P, _P, _I, _P]),
+    "w4j_op_pages_write": (_I, [_P, _I, _P, _P, _I, _P, _I64, _P, _I64, _I, _P]),
+    "w4j_op_pages_fork": (_I, [_P, _P, _P, _I, _P]),
+    "w4j_op_pages_free": (_I, [_P, _P, _I, _P]),
+    "w4j_op_pages_compact": (_I, [_P, _P, _P]),
 }
 
 _lib = None

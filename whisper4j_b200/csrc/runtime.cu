@@ -23,6 +23,7 @@
 #include <vector>
 
 #include "../../include/whisper4j_cuda.h"
+#include "host_api.cuh"
 #include "k_step.cuh"
 #include "w4j_internal.cuh"
 
@@ -33,7 +34,7 @@ using namespace w4j;
 // ---------------------------------------------------------------------------
 static thread_local std::string g_err;
 
-static int set_err(int code, const char *fmt, ...) {
+int w4j::set_err(int code, const char *fmt, ...) {
     char buf[1024];
     va_list ap;
     va_start(ap, fmt);
@@ -42,25 +43,6 @@ static int set_err(int code, const char *fmt, ...) {
     g_err = buf;
     return code;
 }
-
-// A failed call leaves its error as the thread's last CUDA error (cudaGetLastError); it is consumed
-// here, so a later launch check does not report an earlier, already handled failure (a refused
-// allocation, for instance).
-#define CUDA_TRY(expr)                                                                             \
-    do {                                                                                           \
-        cudaError_t e_ = (expr);                                                                   \
-        if (e_ != cudaSuccess) {                                                                   \
-            cudaGetLastError();                                                                    \
-            return set_err(e_ == cudaErrorMemoryAllocation ? W4J_ERR_OOM : W4J_ERR_CUDA, "%s: %s (%s:%d)", \
-                           #expr, cudaGetErrorString(e_), __FILE__, __LINE__);                     \
-        }                                                                                          \
-    } while (0)
-
-#define TRY(expr)            \
-    do {                     \
-        int r_ = (expr);     \
-        if (r_ < 0) return r_; \
-    } while (0)
 
 // ---------------------------------------------------------------------------
 // context
