@@ -389,6 +389,47 @@ int w4j_op_pages_free(const w4j_pages *cache, const int32_t *rows, int n, void *
  * NULL) gets n: pages n .. n_pages - 1 are free afterwards and may be cut off. */
 int w4j_op_pages_compact(const w4j_pages *cache, int32_t *n_live, void *stream);
 
+/*
+ * Attention of one layer over a paged cache, for a batch whose groups share their first tokens (the
+ * softmax(q k^T) v of W4J/nn/MultiHeadAttention.java:77-132 for many sequences at once).
+ *
+ * Sequence i (0 <= i < n_seq) is row rows[i] of the cache; group g is sequences group_start[g] ..
+ * group_start[g + 1] - 1 (n_group + 1 ascending numbers from 0 to n_seq).  All sequences of group g hold the
+ * same first shared[g] tokens, on the same pages or on copies of them: their keys and values are read
+ * once for the whole group, through the table of its first sequence.  Query t (0 <= t < n_query) of a
+ * sequence sees the first len - n_query + t + 1 tokens of its row: the last n_query tokens are the queries'
+ * own, already written.  A query that sees no token gets zeros.  What lies behind a row's length, and what a
+ * query does not see, may be anything, NaN included.
+ *
+ *   q, out  [n_seq n_query] tokens of [n_head][head_dim] of the cache's type, q_stride and out_stride
+ *           elements apart (multiples of 8, 16-byte aligned); query head h reads key/value head h / (n_head / n_kv_head)
+ *   shared[g] may be at most max_shared, and at most len - n_query + 1 (or 0) of each of its rows.  max_shared and
+ *           max_own (an upper bound of len - shared over the rows) size the launch; only max_shared is a limit
+ *   work    w4j_op_attn_shared_workspace() bytes, 16-byte aligned, for this call alone until it has run
+ *
+ * Scores, the softmax and all sums are held in 32 bits; the softmax's weights are rounded to the cache's
+ * type before they meet the values.  A sequence whose row, group or shared length is bad, or whose table names a
+ * page that is not there, gets NaN, and the cache's status its bit.  Asynchronous on `stream`; results do
+ * not depend on the order in which blocks run.
+ */
+#define W4J_PAGES_BAD_SHARED 32 /* a shared length over max_shared, or over what a row's queries all see */
+
+typedef struct w4j_attn_shared {
+    const w4j_pages *cache;
+    int32_t layer, n_head, n_query, n_seq, n_group, max_shared, max_own;
+    float scale;
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    const int32_t *rows, *group_start, *shared;
+    void *work;
+    size_t work_bytes;
+} w4j_attn_shared;
+
+/* Bytes of scratch a call of these sizes needs (pointers and strides are not looked at); 0 where they are refused. */
+size_t w4j_op_attn_shared_workspace(const w4j_attn_shared *args);
+int w4j_op_attn_shared(const w4j_attn_shared *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -108,3 +108,40 @@ def test_python_cache_refuses_host_tensors():
         ops.PagedCache.from_tensors(torch.zeros(2, 4, 2, 16, 64), i, i.view(4, 1), i)
     with pytest.raises(ValueError, match="positive"):
         ops.PagedCache(1, 2, 64, 0, 16, 4, 64, device="cpu")
+
+
+def attn(c, **kw):
+    f = dict(cache=ctypes.pointer(c) if c is not None else None, layer=0, n_head=6, n_query=1, n_seq=2, n_group=1,
+             max_shared=20, max_own=30, scale=0.125, q=P, out=P, q_stride=384, out_stride=384, rows=P, group_start=P, shared=P,
+             work=P, work_bytes=1 << 40)
+    f.update(kw)
+    return _lib.AttnShared(**f)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(layer=2), "layer"), (dict(layer=-1), "layer"), (dict(n_head=4), "n_head"), (dict(n_head=0), "n_head"),
+    (dict(n_query=0), "n_query"), (dict(n_query=4097), "n_query"), (dict(n_seq=0), "n_seq"), (dict(n_seq=65537), "n_seq"),
+    (dict(n_group=0), "n_group"), (dict(n_seq=65536, n_query=4096), "2^24"), (dict(max_shared=-1), "max_shared"),
+    (dict(max_shared=81), "max_shared"), (dict(max_own=81), "max_own")])
+def test_attention_refuses_sizes(kw, text):
+    a = ctypes.byref(attn(cache(), **kw))
+    assert lib().w4j_op_attn_shared_workspace(a) == 0
+    assert text in lib().w4j_last_error().decode()
+    refused(lib().w4j_op_attn_shared(a, None), text)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(q=None), "null"), (dict(out=None), "null"), (dict(rows=None), "null"), (dict(group_start=None), "null"),
+    (dict(shared=None), "null"), (dict(work=None), "null"), (dict(q_stride=376), "strides"), (dict(out_stride=388), "strides"),
+    (dict(q=P + 8), "aligned"), (dict(out=P + 2), "aligned"), (dict(work=P + 8), "aligned"), (dict(work_bytes=64), "work"),
+    (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(scale=float("inf")), "scale")])
+def test_attention_refuses_arguments(kw, text):
+    refused(lib().w4j_op_attn_shared(ctypes.byref(attn(cache(), **kw)), None), text)
+
+
+def test_attention_refuses_a_bad_cache():
+    for kw, text in BAD_CACHES + BAD_POINTERS:
+        refused(lib().w4j_op_attn_shared(ctypes.byref(attn(cache(**kw))), None), text)
+    refused(lib().w4j_op_attn_shared(ctypes.byref(attn(None)), None), "null")
+    refused(lib().w4j_op_attn_shared(None, None), "null")

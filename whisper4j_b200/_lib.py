@@ -21,7 +21,7 @@ W4J_ERR_CANCELLED = -5
 
 GGML_F32, GGML_F16, GGML_Q8_0, GGML_BF16 = 0, 1, 8, 30
 
-PAGES_BAD_ROW, PAGES_FULL, PAGES_TOO_LONG, PAGES_BAD_START, PAGES_BAD_PAGE = 1, 2, 4, 8, 16
+PAGES_BAD_ROW, PAGES_FULL, PAGES_TOO_LONG, PAGES_BAD_START, PAGES_BAD_PAGE, PAGES_BAD_SHARED = 1, 2, 4, 8, 16, 32
 
 
 class W4jError(RuntimeError):
@@ -77,6 +77,13 @@ class Pages(ctypes.Structure):
         ("work_bytes", ctypes.c_size_t)]
 
 
+class AttnShared(ctypes.Structure):
+    _fields_ = [("cache", ctypes.POINTER(Pages))] + [(n, ctypes.c_int32) for n in (
+        "layer", "n_head", "n_query", "n_seq", "n_group", "max_shared", "max_own")] + [("scale", ctypes.c_float)] + [
+        (n, ctypes.c_void_p) for n in ("q", "out")] + [(n, ctypes.c_int64) for n in ("q_stride", "out_stride")] + [
+        (n, ctypes.c_void_p) for n in ("rows", "group_start", "shared", "work")] + [("work_bytes", ctypes.c_size_t)]
+
+
 # every symbol declared in include/whisper4j_cuda.h: name -> (restype, argtypes)
 _P, _I, _F, _D, _U64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_double, ctypes.c_uint64
 _I64, _SZ = ctypes.c_int64, ctypes.c_size_t
@@ -117,6 +124,8 @@ SIGNATURES = {
     "w4j_op_pages_fork": (_I, [_P, _P, _P, _I, _P]),
     "w4j_op_pages_free": (_I, [_P, _P, _I, _P]),
     "w4j_op_pages_compact": (_I, [_P, _P, _P]),
+    "w4j_op_attn_shared_workspace": (_SZ, [_P]),
+    "w4j_op_attn_shared": (_I, [_P, _P]),
 }
 
 _lib = None

@@ -1,5 +1,7 @@
-// op_api.cu — C entry points of the operators for hosts that drive their own loop: the paged cache.
+// op_api.cu — C entry points of the operators for hosts that drive their own loop: the paged cache
+// and the attention over it.
 // Every argument check that needs no device memory is made here, before any device call.
+#include "attn_shared.cuh"
 #include "host_api.cuh"
 #include "pages.cuh"
 
@@ -116,5 +118,58 @@ extern "C" int w4j_op_pages_compact(const w4j_pages *c, int32_t *n_live, void *s
     DeviceGuard g(c->device);
     TRY(g.rc());
     CUDA_TRY(launch_pages_compact(p, n_live, stream_of(stream)));
+    return W4J_OK;
+}
+
+static int attn_sizes(const w4j_attn_shared *x, const char *who, AttnSharedArgs *a) {
+    if (!x) return set_err(W4J_ERR_ARG, "%s: null argument", who);
+    TRY(pages_sizes(x->cache, who, &a->p));
+    if (x->n_head < 1 || x->n_head > 4096 || x->n_head % a->p.n_kv_head)
+        return set_err(W4J_ERR_ARG, "%s: n_head = %d must be a multiple of n_kv_head = %d in [1, 4096]", who, x->n_head,
+                       a->p.n_kv_head);
+    if (x->n_query < 1 || x->n_query > 4096) return set_err(W4J_ERR_ARG, "%s: n_query must be in [1, 4096]", who);
+    if (x->n_seq < 1 || x->n_seq > 1 << 16 || x->n_group < 1 || x->n_group > 1 << 16)
+        return set_err(W4J_ERR_ARG, "%s: n_seq and n_group must be in [1, 65536]", who);
+    if ((int64_t)x->n_seq * x->n_query * x->n_head > 1 << 24)
+        return set_err(W4J_ERR_ARG, "%s: n_seq * n_query * n_head must be at most 2^24", who);
+    if (x->layer < 0 || x->layer >= a->p.n_layer) return set_err(W4J_ERR_ARG, "%s: layer %d of %d", who, x->layer, a->p.n_layer);
+    const int most = a->p.width * a->p.page_tokens;
+    if (x->max_shared < 0 || x->max_shared > most || x->max_own < 0 || x->max_own > most)
+        return set_err(W4J_ERR_ARG, "%s: max_shared and max_own must be in [0, %d], what a row can hold", who, most);
+    a->layer = x->layer, a->n_head = x->n_head, a->rep = x->n_head / a->p.n_kv_head, a->n_query = x->n_query;
+    a->n_seq = x->n_seq, a->n_group = x->n_group, a->max_shared = x->max_shared, a->max_own = x->max_own;
+    attn_shared_plan(*a);
+    return W4J_OK;
+}
+
+extern "C" size_t w4j_op_attn_shared_workspace(const w4j_attn_shared *x) {
+    AttnSharedArgs a;
+    return attn_sizes(x, "w4j_op_attn_shared_workspace", &a) < 0 ? 0 : attn_shared_work_bytes(a);
+}
+
+extern "C" int w4j_op_attn_shared(const w4j_attn_shared *x, void *stream) {
+    const char *who = "w4j_op_attn_shared";
+    AttnSharedArgs a;
+    TRY(attn_sizes(x, who, &a));
+    TRY(pages_check(x->cache, who, &a.p));
+    if (!x->q || !x->out || !x->rows || !x->group_start || !x->shared || !x->work)
+        return set_err(W4J_ERR_ARG, "%s: null argument", who);
+    const int64_t token = (int64_t)x->n_head * a.p.head_dim;
+    if (x->q_stride < token || x->out_stride < token || x->q_stride % 8 || x->out_stride % 8)
+        return set_err(W4J_ERR_ARG, "%s: strides must be multiples of 8 of at least n_head * head_dim", who);
+    if (!aligned(x->q, 16) || !aligned(x->out, 16) || !aligned(x->work, 16))
+        return set_err(W4J_ERR_ARG, "%s: q, out and work must be 16-byte aligned", who);
+    if (!(x->scale > 0) || x->scale > 3e38f) return set_err(W4J_ERR_ARG, "%s: scale must be positive and finite", who);
+    if (x->work_bytes < attn_shared_work_bytes(a))
+        return set_err(W4J_ERR_ARG, "%s: work has %zu bytes, w4j_op_attn_shared_workspace asks for %zu", who, x->work_bytes,
+                       attn_shared_work_bytes(a));
+    a.scale_log2 = x->scale * 1.44269504f;
+    a.q = x->q, a.out = x->out, a.q_stride = x->q_stride, a.out_stride = x->out_stride;
+    a.rows = x->rows, a.group_start = x->group_start, a.shared = x->shared;
+    a.part_o = static_cast<float *>(x->work);
+    a.part_ml = a.part_o + (size_t)a.n_seq * a.n_query * a.n_head * a.slots * a.p.head_dim;
+    DeviceGuard g(x->cache->device);
+    TRY(g.rc());
+    CUDA_TRY(launch_attn_shared(a, x->cache->type == W4J_GGML_BF16, stream_of(stream)));
     return W4J_OK;
 }

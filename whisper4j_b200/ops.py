@@ -15,13 +15,14 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import GGML_BF16, GGML_F16, GGML_F32, IllegalStateError, Pages, check, lib
+from ._lib import GGML_BF16, GGML_F16, GGML_F32, AttnShared, IllegalStateError, Pages, check, lib
 
 _TYPES = {torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
 _STATUS = {_lib.PAGES_BAD_ROW: "a row is out of range or named twice", _lib.PAGES_FULL: "too few free pages",
            _lib.PAGES_TOO_LONG: "a row would outgrow its table",
            _lib.PAGES_BAD_START: "start does not ascend from 0 or does not fit the rows",
-           _lib.PAGES_BAD_PAGE: "a table entry names no held page"}
+           _lib.PAGES_BAD_PAGE: "a table entry names no held page",
+           _lib.PAGES_BAD_SHARED: "a shared length is over max_shared or over what a row's queries see"}
 
 
 def _stream(device):
@@ -124,6 +125,47 @@ class PagedCache:
         live = torch.empty(1, dtype=torch.int32, device=self.device)
         check(lib().w4j_op_pages_compact(self._ref, live.data_ptr(), _stream(self.device)))
         return live
+
+    def attend(self, layer, q, rows, group_start, shared, max_shared, max_own, scale=None, out=None):
+        """Attention of one layer: q (n_seq, n_query, n_head, head_dim) -> out of the same shape.
+
+        Sequence i is row rows[i]; its queries are the row's last n_query tokens, already written, and see their own
+        token and all before it.  Group g is sequences group_start[g] .. group_start[g + 1] - 1, whose rows hold the same
+        first shared[g] tokens: they are read once for the group.  max_shared and max_own are upper bounds, known on
+        the host, of shared and of the rows' tokens behind it.  ``scale`` defaults to head_dim ** -0.5.
+        """
+        _need(q.dim() == 4 and q.dtype == self.pool.dtype and q.device == self.device,
+              f"q must be (n_seq, n_query, n_head, head_dim) {self.pool.dtype} on {self.device}")
+        n_seq, n_query, n_head, dim = q.shape
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, "out must be like q")
+        _need(dim == self.head_dim, f"q has heads of {dim} in a cache of {self.head_dim}")
+        if q.numel() == 0:
+            return out
+        r, _ = self._rows(rows, "rows")
+        _need(rows.shape[0] == n_seq, f"rows must have shape ({n_seq},)")
+        g, n = self._rows(shared, "shared")
+        a = AttnShared(ctypes.pointer(self._c), layer, n_head, n_query, n_seq, n, max_shared, max_own,
+                       self.head_dim ** -0.5 if scale is None else scale, q.data_ptr(), out.data_ptr(),
+                       self._query_stride(q, "q"), self._query_stride(out, "out"), r,
+                       self._int32(group_start, "group_start", n + 1), g)
+        ref = ctypes.byref(a)
+        a.work_bytes = lib().w4j_op_attn_shared_workspace(ref)
+        _need(a.work_bytes, lib().w4j_last_error().decode())
+        work = torch.empty(a.work_bytes, dtype=torch.uint8, device=self.device)
+        a.work = work.data_ptr()
+        check(lib().w4j_op_attn_shared(ref, _stream(self.device)))
+        return out
+
+    @staticmethod
+    def _query_stride(t, name):
+        """Elements from one query token to the next; sequences follow one another."""
+        n_seq, n_query, n_head, dim = t.shape
+        stride = t.stride(1) if n_query > 1 else t.stride(0) if n_seq > 1 else n_head * dim
+        _need((dim == 1 or t.stride(3) == 1) and (n_head == 1 or t.stride(2) == dim) and
+              (n_seq == 1 or t.stride(0) == n_query * stride), f"{name} must have contiguous heads and evenly spaced tokens")
+        return stride
 
     def check(self):
         """Wait for the calls so far; IllegalStateError where one of them could not be done (and clear that)."""
