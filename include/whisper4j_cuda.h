@@ -430,6 +430,34 @@ typedef struct w4j_attn_shared {
 size_t w4j_op_attn_shared_workspace(const w4j_attn_shared *args);
 int w4j_op_attn_shared(const w4j_attn_shared *args, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * A Linear layer in 8-bit integers with a scale for each row of activations and each output channel (the
+ * product of W4J/nn/Linear.java:23-26 with both operands quantised; w4j_op_linear keeps the activations).
+ * ------------------------------------------------------------------------- */
+
+/*
+ * q = round(x / s), s = max |x| / 127 for each of M rows of K elements (ldx elements apart, of type
+ * x_type: F32, F16 or BF16), optionally behind a LayerNorm (ln_g and ln_b, K floats each, or both NULL).  The
+ * quotient is rounded as if exact, ties to even, and kept within +-127.  q has rows ldq bytes apart (a multiple of 16 of at least
+ * K, 16-byte aligned); columns K up to the next multiple of 16 get zeros.  A row of zeros gets scale 0, a row with
+ * an infinity or a NaN zeros and scale NaN, which a product hands on to all of the row's outputs.  The weights of
+ * a layer are quantised by the same call, a row being an output channel.
+ */
+int w4j_op_quantize_rows(int device, const void *x, int x_type, int M, int K, int64_t ldx, const float *ln_g,
+                         const float *ln_b, int8_t *q, int64_t ldq, float *scale, void *stream);
+
+/*
+ * y[m][n] = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n] (bias may be NULL), the sum exact in 32-bit
+ * integers, the rest in 32-bit floats, rounded once to y_type (F32, F16 or BF16).  x: M rows, w: N rows,
+ * ldx and ldw bytes apart (multiples of 16), 16-byte aligned, columns K up to the next multiple of 16 zero (as
+ * w4j_op_quantize_rows leaves them).  K at most 131056.  y: rows ldy elements apart, at least N.  epilogue: 0 =
+ * store, 1 = GELU (tanh form in 32 bits; w4j_op_linear looks the same function up by the f16 of its argument),
+ * 2 = residual y += ....  y may not overlap the inputs.
+ */
+int w4j_op_linear_i8(int device, const int8_t *x, int64_t ldx, const float *x_scale, int M, int K, const int8_t *w,
+                     int64_t ldw, const float *w_scale, int N, const float *bias, int epilogue, void *y, int y_type,
+                     int64_t ldy, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,220 @@
+"""The 8-bit integer Linear against its definition in 64 bits.
+
+The quantised numbers of a row without a LayerNorm are exactly defined and have to be equal.  A product's integer sum is
+exact; after it come the conversion (2^-24), two products (2^-24 each) and the bias (2^-24) in 32 bits, and the
+rounding to y's type (u = eps / 2, nothing for 32 bits), so |error| <= 4 2^-24 (|product| + |y|) + u |y|; a residual adds
+one more sum of 32 bits.  GELU has slope below 1.13, and its own arithmetic v / (1 + exp(-2 u)) an exponential of
+2 + 1.2 |2 u| units in the last place with an argument that is off by 4 2^-24 |2 u|: (8 + 8 |u|) 2^-23 relative.
+"""
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+E = 2.0 ** -24
+
+
+def quantised(x):
+    """(q, scale) of float32-valued rows, in 64 bits."""
+    x = x.double()
+    s = (x.abs().amax(1) / 127).float()
+    # a scale below 32 bits' normal range is rounded as a 32-bit division rounds
+    s = torch.from_numpy((x.abs().amax(1).float().cpu().numpy() / np.float32(127)).astype(np.float32)).to(x.device) if x.numel() else s
+    q = torch.where(s[:, None] > 0, x / s.double()[:, None], 0).round().clamp(-127, 127)
+    return q.to(torch.int8), s
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 1280), (3, 7), (5, 8), (2, 9), (4, 16), (7, 100), (33, 1000), (300, 1280), (64, 2049),
+                                 (10, 5120), (3, 8200), (2, 20001)])
+def test_quantize_is_exact(m, k, dtype):
+    from whisper4j_b200 import ops
+    g = torch.Generator("cuda").manual_seed(m + k)
+    x = (torch.randn(m, k, device="cuda", generator=g) * torch.rand(m, 1, device="cuda", generator=g) * 50).to(dtype)
+    q, s = ops.quantize_rows(x)
+    qw, sw = quantised(x.float())
+    assert q.shape == (m, (k + 15) // 16 * 16)
+    assert torch.equal(s, sw)
+    assert torch.equal(q[:, :k], qw)
+    assert not q[:, k:].any()
+
+
+def test_quantize_ties_borders_and_extremes():
+    from whisper4j_b200 import ops
+    rows = [[127.0, 0.5, 1.5, -0.5, -2.5, 126.5, 3.5 + 2 ** -20, 3.5 - 2 ** -20],
+            [3.0, 0.0, -3.0, 1.0, 2.0, 1e-30, -1e-30, 0.1],
+            [0.0] * 8, [-0.0] * 8, [1e-40] * 8, [1e-45, 0, 0, 0, 0, 0, 0, 0], [3e-38, 1e-38, -2e-38, 1e-39, 5e-39, 0, 0, 0],
+            [3.4e38, -3.4e38, 1e38, 1.0, 1e30, 2e38, 0, -1e38], [1e-31 * i for i in range(8)],
+            [1e-44, 2e-44, 3e-44, 7e-44, 1e-43, 9e-44, 0, 0]]
+    x = torch.tensor(rows, dtype=torch.float32, device="cuda")
+    rnd = torch.randn(20000, 8, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    # quotients next to halves: x = (n + 1/2) s, one step to either side
+    s = (rnd[:, :1].abs() + 0.1) * 127 / 127
+    n = torch.randint(-126, 126, (20000, 8), device="cuda", generator=torch.Generator("cuda").manual_seed(2)) + 0.5
+    near = (n * s).float()
+    near[:, 0] = (s * 127)[:, 0]
+    near[:, 3] = torch.nextafter(near[:, 3], torch.tensor(9e9, device="cuda"))
+    near[:, 4] = torch.nextafter(near[:, 4], torch.tensor(-9e9, device="cuda"))
+    for t in (x, near):
+        q, sc = ops.quantize_rows(t)
+        qw, sw = quantised(t)
+        assert torch.equal(sc, sw)
+        assert torch.equal(q[:, :8], qw)
+
+
+def test_rows_that_are_not_finite():
+    from whisper4j_b200 import ops
+    x = torch.randn(6, 40, device="cuda")
+    x[1, 3], x[2, 39], x[4, 0] = float("nan"), float("inf"), float("-inf")
+    q, s = ops.quantize_rows(x)
+    assert torch.isnan(s).tolist() == [False, True, True, False, True, False]
+    assert not q[[1, 2, 4]].any()
+    y = ops.Int8Linear.from_float(torch.randn(9, 40, device="cuda"))(x)
+    assert torch.isnan(y).all(1).tolist() == [False, True, True, False, True, False]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k", [(1, 16), (4, 1280), (33, 777), (2, 5120), (2, 9001)])
+def test_quantize_behind_a_layer_norm(m, k, dtype):
+    """The normalised row is off by 32-bit sums of depth d = 8 ceil(K / 2048) + 20 (a thread's run, the warp, the block):
+    the mean by d E mean|x|, the deviation's factor by (d + 8) E; a quantised number by half a step more."""
+    from whisper4j_b200 import ops
+    g = torch.Generator("cuda").manual_seed(k)
+    x = (torch.randn(m, k, device="cuda", generator=g) * 3 + 1).to(dtype)
+    gamma = 1 + 0.1 * torch.randn(k, device="cuda", generator=g)
+    beta = 0.1 * torch.randn(k, device="cuda", generator=g)
+    q, s = ops.quantize_rows(x, ln=(gamma, beta))
+    x = x.double()
+    mean = x.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + 1e-5)
+    y = (x - mean) * rstd * gamma.double() + beta.double()
+    d = 8 * math.ceil(k / 2048) + 20
+    off = gamma.double().abs() * rstd * d * E * x.abs().mean(1, keepdim=True) + (y - beta.double()).abs() * (d + 8) * E + y.abs() * 2 * E
+    want = y.abs().amax(1) / 127
+    assert ((s.double() - want).abs() <= off.amax(1) / 127 + 2 * E * want).all()
+    back = q[:, :k].double() * s.double()[:, None]
+    assert ((back - y).abs() <= 0.5 * s.double()[:, None] * (1 + 1e-6) + off).all()
+
+
+def product_case(m, k, n, ytype, epilogue, bias, seed=0, big=False):
+    from whisper4j_b200 import _lib
+    from whisper4j_b200._lib import check, lib
+    g = torch.Generator("cuda").manual_seed(seed + m + 3 * k + 7 * n)
+    k16, ldy = (k + 15) // 16 * 16, n + 3
+    xq = torch.zeros(m, k16 + 32, dtype=torch.int8, device="cuda")
+    wq = torch.zeros(n, k16 + 16, dtype=torch.int8, device="cuda")
+    if big:  # the largest sums there are
+        xq[:, :k], wq[:, :k] = 127, 127
+        xq[1::2, :k] = -128
+    else:
+        xq[:, :k] = torch.randint(-128, 128, (m, k), device="cuda", generator=g)
+        wq[:, :k] = torch.randint(-128, 128, (n, k), device="cuda", generator=g)
+    xq[:, k16:], wq[:, k16:] = 99, 99  # behind the padding there may be anything
+    scale = 4.0 / (74 * 74 * math.sqrt(k))
+    xs = torch.rand(m, device="cuda", generator=g) + 0.5
+    ws = (torch.rand(n, device="cuda", generator=g) + 0.5) * scale
+    b = torch.randn(n, device="cuda", generator=g) if bias else None
+    y = torch.randn(m, ldy, device="cuda", generator=g).to(ytype)
+    before = y.clone()
+    code = {torch.float32: _lib.GGML_F32, torch.float16: _lib.GGML_F16, torch.bfloat16: _lib.GGML_BF16}[ytype]
+    check(lib().w4j_op_linear_i8(0, xq.data_ptr(), k16 + 32, xs.data_ptr(), m, k, wq.data_ptr(), k16 + 16, ws.data_ptr(), n,
+                                 b.data_ptr() if bias else None, epilogue, y.data_ptr(), code, ldy,
+                                 torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(y[:, n:], before[:, n:])  # nothing behind the last channel
+    prod = (xq[:, :k].double() @ wq[:, :k].double().T) * xs.double()[:, None] * ws.double()
+    v = prod + (b.double() if bias else 0)
+    tol = 4 * E * (prod.abs() + v.abs())
+    if epilogue == 1:
+        u = math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)
+        v = v / (1 + torch.exp(-2 * u))
+        tol = 1.13 * tol + v.abs() * (8 + 8 * u.abs()) * 2 * E + 1e-36
+    elif epilogue == 2:
+        v = v + before[:, :n].double()
+        tol = tol + E * v.abs()
+    half = 0 if ytype == torch.float32 else torch.finfo(ytype).eps / 2
+    tol = tol * (1 + half) + half * v.abs() + (torch.finfo(ytype).smallest_normal * torch.finfo(ytype).eps)
+    bad = (y[:, :n].double() - v).abs() > tol
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist())
+
+
+@pytest.mark.parametrize("ytype", TYPES)
+@pytest.mark.parametrize("epilogue", [0, 1, 2])
+@pytest.mark.parametrize("m,k,n", [(1, 16, 1), (1, 1280, 3840), (2, 384, 51), (5, 100, 700), (8, 5120, 1280), (9, 1280, 129),
+                                   (16, 2048, 512), (17, 512, 1000), (40, 1280, 1280), (77, 1000, 701), (128, 5120, 1280),
+                                   (130, 384, 384), (320, 5120, 1280), (700, 1280, 640)])
+def test_product(m, k, n, epilogue, ytype):
+    product_case(m, k, n, ytype, epilogue, bias=(m + n) % 2 == 0 or epilogue == 1)
+
+
+@pytest.mark.parametrize("m,k,n", [(3000, 1280, 5120), (1500, 384, 1536), (2049, 1008, 2050), (257, 5120, 1300)])
+@pytest.mark.parametrize("epilogue,ytype", [(0, torch.float32), (1, torch.float16), (2, torch.bfloat16)])
+def test_large_products(m, k, n, epilogue, ytype):
+    product_case(m, k, n, ytype, epilogue, True)
+
+
+@pytest.mark.parametrize("m", [1, 4, 60, 300])
+def test_sums_at_the_limit_of_32_bits(m):
+    product_case(m, 131056, 130, torch.float32, 0, False, big=True)
+
+
+@pytest.mark.parametrize("xtype,ytype", [(torch.float32, torch.float32), (torch.float16, torch.bfloat16), (torch.bfloat16, torch.float16)])
+def test_layer(xtype, ytype):
+    """The whole layer against a Linear on the numbers that its integers stand for."""
+    from whisper4j_b200 import ops
+    g = torch.Generator("cuda").manual_seed(9)
+    w, b = torch.randn(700, 1000, device="cuda", generator=g) * 0.03, torch.randn(700, device="cuda", generator=g)
+    x = torch.randn(50, 1100, device="cuda", generator=g).to(xtype)[:, 60:1060]
+    layer = ops.Int8Linear.from_float(w, b)
+    wq, ws = quantised(w)
+    assert torch.equal(layer.weight[:, :1000], wq) and torch.equal(layer.scale, ws)
+    xq, xs = quantised(x.float())
+    v = (xq.double() @ wq.double().T) * xs.double()[:, None] * ws.double() + b.double()
+    half = 0 if ytype == torch.float32 else torch.finfo(ytype).eps / 2
+    y = layer(x, out_dtype=ytype)
+    assert y.dtype == ytype
+    assert ((y.double() - v).abs() <= (8 * E + half) * (v.abs() + b.double().abs())).all()
+    wide = torch.zeros(50, 1500, dtype=ytype, device="cuda")
+    layer(x, out=wide[:, 3:703])
+    assert torch.equal(wide[:, 3:703], y) and not wide[:, :3].any() and not wide[:, 703:].any()
+    again = layer(x, epilogue="residual", out=y.clone())
+    assert ((again.double() - 2 * v).abs() <= (16 * E + 3 * half) * (2 * v.abs() + b.double().abs())).all()
+    assert layer(x[:0]).shape == (0, 700)
+
+
+def test_captured_on_a_side_stream():
+    from whisper4j_b200 import ops
+    layer = ops.Int8Linear.from_float(torch.randn(640, 320, device="cuda"))
+    x = torch.zeros(70, 320, device="cuda")
+    out = torch.empty(70, 640, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer(x, out=out)
+    for i in range(5):
+        x.normal_()
+        graph.replay()
+        assert torch.equal(out, layer(x))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = layer(x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(y, out)
+
+
+def test_refusals():
+    from whisper4j_b200 import ops
+    w = torch.randn(30, 40, device="cuda")
+    layer = ops.Int8Linear.from_float(w)
+    x = torch.randn(3, 40, device="cuda")
+    for bad in (lambda: layer(x[:, :39]), lambda: layer(x.double()), lambda: layer(x.cpu()), lambda: layer(x, epilogue="relu"),
+                lambda: layer(x, epilogue="residual"), lambda: layer(x, out=torch.empty(3, 31, device="cuda")),
+                lambda: layer(x, out=torch.empty(3, 30, device="cuda"), out_dtype=torch.float16), lambda: layer(x.t()),
+                lambda: layer(x, ln=(x[0], x[0, :39])), lambda: ops.Int8Linear(w, w[:, 0]),
+                lambda: ops.Int8Linear(layer.weight, layer.scale[:5]), lambda: layer(x.T.contiguous().T)):
+        with pytest.raises(ValueError):
+            bad()

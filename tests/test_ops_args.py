@@ -145,3 +145,30 @@ def test_attention_refuses_a_bad_cache():
         refused(lib().w4j_op_attn_shared(ctypes.byref(attn(cache(**kw))), None), text)
     refused(lib().w4j_op_attn_shared(ctypes.byref(attn(None)), None), "null")
     refused(lib().w4j_op_attn_shared(None, None), "null")
+
+
+def quantize(device=0, x=P, x_type=GGML_F32, m=2, k=100, ldx=100, g=None, b=None, q=P, ldq=112, scale=P):
+    return lib().w4j_op_quantize_rows(device, x, x_type, m, k, ldx, g, b, q, ldq, scale, None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(x=None), "null"), (dict(q=None), "null"), (dict(scale=None), "null"), (dict(x_type=8), "x_type"), (dict(m=0), "shape"),
+    (dict(k=0, ldq=16), "shape"), (dict(k=-3), "shape"), (dict(ldx=99), "ldx"), (dict(ldq=96), "ldq"), (dict(ldq=104), "ldq"),
+    (dict(q=P + 8), "ldq"), (dict(x=P + 2), "aligned"), (dict(x=P + 1, x_type=GGML_F16), "aligned"), (dict(scale=P + 2), "aligned"),
+    (dict(g=P), "gamma"), (dict(b=P), "gamma")])
+def test_quantize_refusals(kw, text):
+    refused(quantize(**kw), text)
+
+
+def linear(device=0, x=P, ldx=112, xs=P, m=2, k=100, w=P, ldw=112, ws=P, n=30, bias=None, epilogue=0, y=P, y_type=GGML_F32, ldy=30):
+    return lib().w4j_op_linear_i8(device, x, ldx, xs, m, k, w, ldw, ws, n, bias, epilogue, y, y_type, ldy, None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(x=None), "null"), (dict(xs=None), "null"), (dict(w=None), "null"), (dict(ws=None), "null"), (dict(y=None), "null"),
+    (dict(y_type=8), "y_type"), (dict(m=0), "shape"), (dict(n=0, ldy=0), "shape"), (dict(k=0), "shape"), (dict(m=(1 << 24) + 1), "shape"),
+    (dict(k=131057, ldx=131072, ldw=131072), "131056"), (dict(ldx=96), "rows"), (dict(ldw=104), "rows"), (dict(x=P + 8), "aligned"),
+    (dict(w=P + 4), "aligned"), (dict(ldy=29), "ldy"), (dict(y=P + 2), "aligned"), (dict(epilogue=3), "epilogue"),
+    (dict(epilogue=-1), "epilogue")])
+def test_linear_refusals(kw, text):
+    refused(linear(**kw), text)

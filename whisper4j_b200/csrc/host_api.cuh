@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "../../include/whisper4j_cuda.h"
 
 namespace w4j {
@@ -61,6 +63,20 @@ inline cudaError_t launch_after(Kern kern, dim3 grid, dim3 block, size_t smem, c
         cfg.numAttrs = 2;
     }
     return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device, once for each device.
+template <auto Kern>
+inline cudaError_t allow_smem(size_t bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 }  // namespace w4j

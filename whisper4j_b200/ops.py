@@ -7,6 +7,8 @@ a ValueError; what only the device can see (a row named twice, no free page) rai
 ``status``, which ``PagedCache.check`` reads.
 
     PagedCache     a key/value cache of pages that rows (beams, re-decodes of a window) share
+    quantize_rows  rows to 8-bit integers, a scale for each
+    Int8Linear     a Linear layer in 8-bit integers
 """
 from __future__ import annotations
 
@@ -173,3 +175,82 @@ class PagedCache:
         if bits:
             self.status.zero_()
             raise IllegalStateError("; ".join(text for bit, text in _STATUS.items() if bits & bit))
+
+
+def _vector(t, n, device, name):
+    _need(t.dtype == torch.float32 and t.device == device and t.is_contiguous() and t.shape == (n,),
+          f"{name} must be a contiguous float32 tensor of shape ({n},) on {device}")
+    return t.data_ptr()
+
+
+def _ld(t):
+    """Elements from one row of a matrix to the next."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _matrix(t, name):
+    _need(t.dim() == 2 and t.dtype in _TYPES and t.is_cuda, f"{name} must be a float32, float16 or bfloat16 matrix on a CUDA device")
+    _need((t.shape[1] == 1 or t.stride(1) == 1) and _ld(t) >= t.shape[1], f"{name} must have contiguous rows")
+
+
+def quantize_rows(x, ln=None):
+    """x (M, K) -> (q, scale): q (M, K rounded up to 16) int8 = round(LayerNorm?(x) / scale), zeros behind K, and
+    scale (M,) = max |row| / 127.  ``ln`` is (gamma, beta)."""
+    _matrix(x, "x")
+    m, k = x.shape
+    q = torch.empty(m, (k + 15) // 16 * 16, dtype=torch.int8, device=x.device)
+    scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    if m:
+        g, b = (None, None) if ln is None else (_vector(t, k, x.device, "ln") for t in ln)
+        check(lib().w4j_op_quantize_rows(x.device.index, x.data_ptr(), _TYPES[x.dtype], m, k, _ld(x), g, b, q.data_ptr(),
+                                         q.shape[1], scale.data_ptr(), _stream(x.device)))
+    return q, scale
+
+
+class Int8Linear:
+    """y = activation(LayerNorm?(x) W^T + bias) with x quantised row by row in the call and W (N, K) held as int8
+    ``weight`` with a float32 ``scale`` for each output channel."""
+
+    EPILOGUES = {"store": 0, "gelu": 1, "residual": 2}
+
+    def __init__(self, weight, scale, bias=None):
+        _need(weight.dim() == 2 and weight.dtype == torch.int8 and weight.is_cuda and 0 not in weight.shape,
+              "weight must be an int8 matrix on a CUDA device")
+        self.n, self.k = weight.shape
+        self.device = weight.device
+        k16 = (self.k + 15) // 16 * 16
+        if k16 != self.k or not weight.is_contiguous() or weight.data_ptr() % 16:
+            # laid out once: rows of a multiple of 16 bytes, zeros behind K
+            padded = torch.zeros(self.n, k16, dtype=torch.int8, device=weight.device)
+            padded[:, :self.k] = weight
+            weight = padded
+        _vector(scale, self.n, self.device, "scale")
+        if bias is not None:
+            _vector(bias, self.n, self.device, "bias")
+        self.weight, self.scale, self.bias = weight, scale, bias
+
+    @classmethod
+    def from_float(cls, weight, bias=None):
+        """Quantise a float weight (N, K), channel by channel."""
+        q, scale = quantize_rows(weight)
+        return cls(q[:, :weight.shape[1]], scale, bias)
+
+    def __call__(self, x, ln=None, epilogue="store", out=None, out_dtype=None):
+        """x (M, K) -> (M, N) of ``out_dtype`` (default: x's), or into ``out``; epilogue "gelu", or "residual": out += ..."""
+        _matrix(x, "x")
+        _need(x.device == self.device and x.shape[1] == self.k, f"x must be (M, {self.k}) on {self.device}")
+        _need(epilogue in self.EPILOGUES, f"epilogue must be one of {sorted(self.EPILOGUES)}")
+        m = x.shape[0]
+        if out is None:
+            _need(epilogue != "residual", "a residual needs the tensor that it is added to: out")
+            out = torch.empty(m, self.n, dtype=out_dtype or x.dtype, device=self.device)
+        _matrix(out, "out")
+        _need(out.shape == (m, self.n) and out.device == self.device, f"out must be ({m}, {self.n}) on {self.device}")
+        _need(out_dtype is None or out.dtype == out_dtype, "out is not of out_dtype")
+        if m:
+            q, xs = quantize_rows(x, ln)
+            check(lib().w4j_op_linear_i8(self.device.index, q.data_ptr(), q.shape[1], xs.data_ptr(), m, self.k,
+                                         self.weight.data_ptr(), self.weight.shape[1], self.scale.data_ptr(), self.n,
+                                         None if self.bias is None else self.bias.data_ptr(), self.EPILOGUES[epilogue],
+                                         out.data_ptr(), _TYPES[out.dtype], _ld(out), _stream(self.device)))
+        return out
