@@ -10,9 +10,11 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "attn_shared.cuh"
 #include "host_api.cuh"
-#include "w4j_internal.cuh"
+#include "tc_common.cuh"
 
 namespace w4j {
 
@@ -375,6 +377,312 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(AttnSharedArgs a)
     w.store(po[0], po[1], pm[0], pm[1]);
 }
 
+// ---------------------------------------------------------------------------
+// shared keys on the 5th-generation tensor cores: 128 query rows of a group against 128 keys at a time
+//
+// S = Q K^T (tcgen05.mma, operands in shared memory) and O += P V (P from tensor memory) with a warpgroup per
+// S buffer: warpgroup w takes tiles w, w + 2, ... with a maximum, sum and O of its own, so that one works on
+// its softmax while the tensor cores work for the other; a thread owns a row, so the softmax needs no shuffle.
+// O is rescaled only when a row's maximum has grown by more than 2^8 (weights up to 2^8 are as good as weights up
+// to 1 in either type), and by the owner itself: S of tile i is there only once tile i - 2 has been added.
+// Keys and values come page by page through TMA boxes (128-byte swizzle) into two rings; V is the MMA's B operand
+// as it lies in the pages (MN-major).
+// ---------------------------------------------------------------------------
+constexpr int kTcThreads = 320, kTcKeys = 128, kTcBlock = kTcKeys * 128;  // bytes of 128 rows of 64 numbers
+
+constexpr int tc_stages(int D) { return D == 64 ? 4 : 3; }
+constexpr size_t tc_smem(int D) { return (size_t)(D / 64) * kTcBlock * (1 + 2 * tc_stages(D)) + 1024; }
+
+__device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t *v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                   "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),
+                   "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]),
+                   "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]),
+                   "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at), "r"(v[0]),
+                   "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                   "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
+                   "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),
+                   "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A from tensor memory
+__device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// An operand whose rows (128 bytes, 64 numbers of the M or N dimension) follow one another along K, 128-byte
+// swizzle: groups of 8 rows 1024 bytes apart, the next 64 numbers of M or N `next` bytes on.
+__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t next) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(next >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)2 << 61;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_constant__ CUtensorMap kmap,
+                                                                  const __grid_constant__ CUtensorMap vmap, AttnSharedArgs a,
+                                                                  int box) {
+    constexpr int NB = D / 64, NS = tc_stages(D), kTile = NB * kTcBlock;
+    constexpr bool bf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+    extern __shared__ unsigned char raw[];
+    unsigned char *sq = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char *sk = sq + kTile, *sv = sk + NS * kTile;
+    __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], q_full, s_full[2], p_full[2], pv_done[2], drained;
+    __shared__ uint32_t slot_word;
+    __shared__ int failed, bad_page;
+    __shared__ float m1[128], l1[128];
+    pdl_wait();
+    pdl_trigger();
+    const PagesArgs &p = a.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int c = a.n_query * a.rep;
+    int tile = blockIdx.x % a.tc_tiles;
+    const int split = blockIdx.x / a.tc_tiles % a.shared_splits, head = blockIdx.x / a.tc_tiles / a.shared_splits;
+    const int gr = warp_find(a.n_group, tile, [&](int i) { return (long long)__ldg(a.group_start + i) * c / 128 + i; });
+    const int seq0 = __ldg(a.group_start + gr), seq1 = __ldg(a.group_start + gr + 1);
+    if (seq0 < 0 || seq1 <= seq0 || seq1 > a.n_seq) return;
+    tile -= (int)((long long)seq0 * c / 128) + gr;
+    const int n_rows = (seq1 - seq0) * c, r0 = __ldg(a.rows + seq0);
+    if (tile < 0 || tile * 128 >= n_rows || r0 < 0 || r0 >= p.n_rows) return;
+    const int *table = p.table + (size_t)r0 * p.width;
+    const int len = max(0, min(min(min(__ldg(a.shared + gr), a.max_shared), __ldg(p.len + r0)), p.width * p.page_tokens));
+    const int all = (len + kTcKeys - 1) / kTcKeys, per = (all + a.shared_splits - 1) / a.shared_splits;
+    const int t0 = min(all, split * per), n = min(all, t0 + per) - t0;
+    // the row of this thread: (sequence, query token, head)
+    const int r = tile * 128 + (tid & 127);
+    size_t part = 0;
+    const T *qr = nullptr;
+    if (r < n_rows && tid < 256) {
+        const size_t token = (size_t)(seq0 + r / c) * a.n_query + r % c / a.rep;
+        const int h = head * a.rep + r % a.rep;
+        qr = reinterpret_cast<const T *>(a.q) + token * a.q_stride + (size_t)h * D;
+        part = (token * a.n_head + h) * a.slots + split;
+    }
+    if (n <= 0) {
+        if (qr && tid < 128) a.part_ml[part * 2] = kNone, a.part_ml[part * 2 + 1] = 0.f;
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < NS; ++i) mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_full + i, 1), mbar_init(v_empty + i, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(s_full + i, 1), mbar_init(p_full + i, 128), mbar_init(pv_done + i, 1);
+        mbar_init(&q_full, 256), mbar_init(&drained, 1);
+        fence_mbar_init();
+        failed = bad_page = 0;
+    }
+    if (warp == 9) tmem_alloc(&slot_word, 512), tmem_relinquish();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = slot_word;  // S of the warpgroups at columns 0 and 128 (P over them), O at 256 and 256 + D
+    int issued = 0;
+    if (warp == 8) {
+        // lane b brings box b of each tile
+        for (int i = 0; i < n; ++i) {
+            const int st = i % NS, key = (t0 + i) * kTcKeys, valid = min(kTcKeys, len - key), boxes = (valid + box - 1) / box;
+            int y = 0;
+            if (lane < boxes) {
+                const int k0 = key + lane * box, j = k0 / p.page_tokens;
+                int page = __ldg(table + j);
+                if (page < 0 || page >= p.n_pages) bad_page = 1, page = 0;
+                y = (page * p.n_kv_head + head) * p.page_tokens + k0 - j * p.page_tokens;
+            }
+            bool ok = true;
+            for (int kv = 0; kv < 2 && ok; ++kv) {
+                uint64_t *full = (kv ? v_full : k_full) + st, *empty = (kv ? v_empty : k_empty) + st;
+                ok = i < NS || mbar_wait(empty, (i / NS - 1) & 1, &failed);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) mbar_expect_tx(full, boxes * box * 128 * NB);
+                __syncwarp();
+                if (lane < boxes)
+                    for (int b = 0; b < NB; ++b)
+                        tma_load_2d((kv ? sv : sk) + st * kTile + b * kTcBlock + lane * box * 128, kv ? &vmap : &kmap, 64 * b, y, full);
+                __syncwarp();
+                ++issued;  // K of tile 0, V of tile 0, K of tile 1, ...
+            }
+            if (!ok) break;
+        }
+        // after a wait that ran out: let the copies in flight land before the block's shared memory goes on
+        __syncwarp();
+        if (lane == 0 && *(volatile int *)&failed)
+            for (int x = max(0, issued - 2 * NS); x < issued; ++x) {
+                uint64_t *full = ((x & 1) ? v_full : k_full) + x / 2 % NS;
+                for (int it = 0; it < 1 << 20 && !mbar_test(full, (x / 2 / NS) & 1); ++it) {
+                }
+            }
+    } else if (warp == 9) {
+        if (lane == 0) {
+            constexpr uint32_t type = bf16 ? (1u << 7) | (1u << 10) : 0u;
+            constexpr uint32_t id_s = idesc_f16(128, kTcKeys) | type, id_o = idesc_f16(128, D) | type | (1u << 16);
+            auto scores = [&](int i) {
+                const int st = i % NS;
+                if (!mbar_wait(k_full + st, (i / NS) & 1, &failed)) return false;
+                tc_fence_after();
+                const uint32_t q0 = smem_u32(sq), k0 = smem_u32(sk + st * kTile);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    umma_f16(tmem + 128 * (i & 1), sw128_desc(q0 + k / 4 * kTcBlock) + 2 * (k % 4),
+                             sw128_desc(k0 + k / 4 * kTcBlock) + 2 * (k % 4), id_s, k > 0);
+                umma_commit(s_full + (i & 1));
+                umma_commit(k_empty + st);
+                return true;
+            };
+            bool ok = mbar_wait(&q_full, 0, &failed) && scores(0) && (n < 2 || scores(1));
+            for (int i = 0; i < n && ok; ++i) {
+                const int w = i & 1, st = i % NS;
+                ok = mbar_wait(p_full + w, (i >> 1) & 1, &failed) && mbar_wait(v_full + st, (i / NS) & 1, &failed);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t v0 = smem_u32(sv + st * kTile);
+#pragma unroll
+                for (int k = 0; k < kTcKeys / 16; ++k)
+                    umma_f16_ta(tmem + 256 + w * D, tmem + 128 * w + 8 * k, sw128_desc_mn(v0 + 2048 * k, kTcBlock), id_o, i > 1 || k > 0);
+                umma_commit(pv_done + w);
+                umma_commit(v_empty + st);
+                // S of tile i + 2 goes where P of tile i is
+                if (i + 2 < n) ok = mbar_wait(pv_done + w, (i >> 1) & 1, &failed) && scores(i + 2);
+            }
+            if (!ok) {  // nothing may be in flight when the tensor memory is given back
+                umma_commit(&drained);
+                mbar_wait(&drained, 0, &failed);
+            }
+        }
+    } else {
+        const int w = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_at = tmem + lanes + 128 * w, o_at = tmem + lanes + 256 + w * D;
+        // the query tile, rows behind the group's last as zeros: warpgroup w lays out every other 16-byte unit
+#pragma unroll
+        for (int u = w; u < D / 8; u += 2) {
+            const uint4 v = qr ? __ldg(reinterpret_cast<const uint4 *>(qr) + u) : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(sq + u / 8 * kTcBlock + row * 128 + ((u % 8 ^ (row & 7)) << 4)) = v;
+        }
+        fence_proxy_async();
+        mbar_arrive(&q_full);
+        float m = 0.f, l = 0.f;
+        bool ok = true;
+        for (int i = w; i < n; i += 2) {
+            const int valid = min(kTcKeys, len - (t0 + i) * kTcKeys);
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full + w, (i >> 1) & 1, &failed));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t s[128];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) tmem_load32(s_at + 32 * x, s + 32 * x);
+            tmem_wait_ld();
+            if (valid < kTcKeys)
+#pragma unroll
+                for (int x = 0; x < 128; ++x)
+                    if (x >= valid) s[x] = __float_as_uint(kNone);
+            float mx[4] = {kNone, kNone, kNone, kNone};
+#pragma unroll
+            for (int x = 0; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
+            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+            if (top == kNone) top = i == w ? 0.f : m;
+            if (i == w) {
+                m = top;
+            } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                const float f = top > m ? ex2(m - top) : 1.f;
+                m = fmaxf(m, top);
+                l *= f;
+#pragma unroll 1
+                for (int x = 0; x < D; x += 32) {
+                    uint32_t o[32];
+                    tmem_load32(o_at + x, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    tmem_store32(o_at + x, o);
+                }
+            }
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < 128; x += 2) {
+                const float e0 = ex2(fmaf(__uint_as_float(s[x]), a.scale_log2, -m));
+                const float e1 = ex2(fmaf(__uint_as_float(s[x + 1]), a.scale_log2, -m));
+                sum[x / 2 & 3] += e0 + e1;
+                s[x / 2] = pack2<T>(e0, e1);
+                if (x == 62) tmem_store32(s_at, s);
+            }
+            tmem_store32(s_at + 32, s + 32);
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_wait_st();
+            if (valid < kTcKeys) {  // behind the last key there may be anything: 0 x NaN is none
+                const int st = i % NS;
+                ok = __all_sync(0xffffffffu, mbar_wait(v_full + st, (i / NS) & 1, &failed));
+                if (!ok) break;
+                for (int x = row; x < (kTcKeys - valid) * 8 * NB; x += 128) {
+                    const int at = valid + x / (8 * NB), u = x % (8 * NB);
+                    *reinterpret_cast<uint4 *>(sv + st * kTile + u / 8 * kTcBlock + at * 128 + u % 8 * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async();
+            }
+            tc_fence_before();
+            mbar_arrive(p_full + w);
+        }
+        // both warpgroups' sums, joined by the first
+        // (its own first: the other's last product but one is done then, so that one parity tells its last two apart)
+        for (int x = 0; x < 2 && ok; ++x) {
+            const int b = w ^ x, mine = b ? n / 2 : (n + 1) / 2;
+            ok = mine == 0 || mbar_wait(pv_done + b, (mine - 1) & 1, &failed);
+        }
+        __syncwarp();
+        tc_fence_after();
+        float *other = reinterpret_cast<float *>(sk);  // [D][128], over the rings
+        if (w == 1 && n > 1) {
+#pragma unroll 1
+            for (int x = 0; x < D; x += 32) {
+                uint32_t o[32];
+                tmem_load32(o_at + x, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) other[(x + e) * 128 + row] = __uint_as_float(o[e]);
+            }
+            m1[row] = m, l1[row] = l;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (w == 0) {
+            const bool lost = *(volatile int *)&failed || *(volatile int *)&bad_page;
+            float f0 = 1.f, f1 = 0.f;
+            if (n > 1) {
+                const float top = fmaxf(m, m1[row]);
+                f0 = ex2(m - top), f1 = ex2(m1[row] - top);
+                l = l * f0 + l1[row] * f1;
+                m = top;
+            }
+            if (qr) a.part_ml[part * 2] = lost ? NAN : m, a.part_ml[part * 2 + 1] = lost ? NAN : l;
+            if (tid == 0 && *(volatile int *)&bad_page) atomicOr(p.status, W4J_PAGES_BAD_PAGE);
+#pragma unroll 1
+            for (int x = 0; x < D; x += 32) {
+                uint32_t o[32];
+                tmem_load32(o_at + x, o);
+                tmem_wait_ld();
+                if (n > 1)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        o[e] = __float_as_uint(__uint_as_float(o[e]) * f0 + other[(x + e) * 128 + row] * f1);
+                if (qr)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<uint4 *>(a.part_o + part * D + x + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 9) tc_fence_after(), tmem_dealloc(tmem, 512);
+}
+
 // The parts of one query joined, a warp per query and head, lane i dimensions i D / 32 on.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_attn_shared_join(AttnSharedArgs a) {
@@ -416,12 +724,30 @@ __global__ void __launch_bounds__(256) k_attn_shared_join(AttnSharedArgs a) {
 template <typename T, int D>
 cudaError_t launch(const AttnSharedArgs &a, cudaStream_t s) {
     const long long rows = (long long)a.n_seq * a.n_query * a.n_head;
-    cudaError_t e = launch_after(k_attn_shared<T, D>, (a.shared_items + a.own_items + kAsWarps - 1) / kAsWarps, kAsWarps * 32, 0, s, 1, a);
+    cudaError_t e;
+    if (a.tc_tiles) {
+        const PagesArgs &p = a.p;
+        const int head_rows = p.n_pages * p.n_kv_head * p.page_tokens;
+        int box = 128;
+        while (p.page_tokens % box) box /= 2;
+        const T *pk = reinterpret_cast<const T *>(p.pool) + (size_t)2 * a.layer * head_rows * D;
+        alignas(64) CUtensorMap km, vm;
+        if (!make_tmap_f16_box(&km, pk, head_rows, D, box) || !make_tmap_f16_box(&vm, pk + (size_t)head_rows * D, head_rows, D, box))
+            return cudaErrorInvalidValue;
+        if ((e = allow_smem<k_attn_shared_tc<T, D>>(tc_smem(D))) != cudaSuccess) return e;
+        e = launch_after(k_attn_shared_tc<T, D>, a.tc_tiles * a.shared_splits * p.n_kv_head, kTcThreads, tc_smem(D), s, 1, km, vm,
+                         a, box);
+        if (e != cudaSuccess) return e;
+    }
+    e = launch_after(k_attn_shared<T, D>, (a.shared_items + a.own_items + kAsWarps - 1) / kAsWarps, kAsWarps * 32, 0, s, 1, a);
     if (e != cudaSuccess) return e;
     return launch_after(k_attn_shared_join<T, D>, (unsigned)((rows + 7) / 8), 256, 0, s, 1, a);
 }
 
 }  // namespace
+
+// From so many query rows of a group on, the tensor cores' tiles of 128 rows take the shared keys.
+constexpr int kTcRows = 32;
 
 void attn_shared_plan(AttnSharedArgs &a) {
     const PagesArgs &p = a.p;
@@ -430,9 +756,24 @@ void attn_shared_plan(AttnSharedArgs &a) {
         const long long n = (want + items - 1) / items, most = (keys + 63) / 64;
         return (int)(n < most ? n : most);
     };
-    a.shared_tiles = (int)(a.n_seq * c / 16 + a.n_group);
-    a.shared_splits = a.max_shared > 0 ? splits((long long)a.shared_tiles * p.n_kv_head, a.max_shared) : 0;
-    a.shared_items = (unsigned)a.shared_tiles * a.shared_splits * p.n_kv_head;
+    a.tc_tiles = a.shared_tiles = a.shared_splits = 0;
+    if (a.max_shared > 0) {
+        const long long avg = a.n_seq * c / a.n_group;  // query rows of a group and key/value head
+        if (avg >= kTcRows && (long long)p.n_pages * p.n_kv_head * p.page_tokens < 1ll << 31) {
+            a.tc_tiles = (unsigned)(a.n_seq * c / 128 + a.n_group);
+            // fewest rounds of blocks over the SMs times key tiles of a block (and about four more to start and join)
+            const long long blocks = (avg + 127) / 128 * a.n_group * p.n_kv_head, tiles = (a.max_shared + kTcKeys - 1) / kTcKeys;
+            long long best = 0;
+            for (int n = 1; n <= tiles && n <= 64; ++n) {
+                const long long cost = (blocks * n + 147) / 148 * ((tiles + n - 1) / n + 4);
+                if (n == 1 || cost < best) best = cost, a.shared_splits = n;
+            }
+        } else {
+            a.shared_tiles = (unsigned)(a.n_seq * c / 16 + a.n_group);
+            a.shared_splits = splits((long long)a.shared_tiles * p.n_kv_head, a.max_shared);
+        }
+    }
+    a.shared_items = a.shared_tiles * a.shared_splits * p.n_kv_head;
     a.own_tiles = (int)((c + 15) / 16);
     const int own = a.max_own > 0 ? splits((long long)a.n_seq * p.n_kv_head * a.own_tiles, a.max_own) : 1;
     a.own_splits = own < 1 ? 1 : own;

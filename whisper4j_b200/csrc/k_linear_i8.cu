@@ -236,11 +236,11 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
         fence_mbar_init();
         failed = issued = 0;
     }
+    pdl_wait();  // before the tensor memory: a kernel that waits must not hold what the one before it may need
     if (warp == 1) tmem_alloc(&slot, kCols), tmem_relinquish();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    pdl_wait();
     const uint32_t tmem = slot;
     if (warp == 0 && lane == 0) {
         for (int i = 0; i < nk; ++i) {

@@ -1,14 +1,17 @@
 """Op-level operators over torch tensors, for hosts that drive their own decode loop.
 
 Thin bindings of the ``w4j_op_*`` entry points in include/whisper4j_cuda.h: they check what a tensor knows
-(type, device, layout, shape), hand over the current stream of the tensors' device and allocate outputs with
-torch's allocator, so calls can be captured into CUDA graphs.  Nothing is synchronised.  A refused argument is
-a ValueError; what only the device can see (a row named twice, no free page) raises a bit of the cache's
-``status``, which ``PagedCache.check`` reads.
+(type, device, layout, shape), hand over the current stream of the tensors' device and allocate outputs and
+scratch with torch's allocator, so calls can be captured into CUDA graphs.  Nothing is synchronised.  A refused
+argument is a ValueError; what only the device can see (a row named twice, no free page) raises a bit of the
+cache's ``status``, which ``PagedCache.check`` reads.
 
     PagedCache     a key/value cache of pages that rows (beams, re-decodes of a window) share
     quantize_rows  rows to 8-bit integers, a scale for each
     Int8Linear     a Linear layer in 8-bit integers
+
+A decode step lasts tens of microseconds, so the checks are written to cost little: messages are put together
+only where a check fails.
 """
 from __future__ import annotations
 
@@ -17,23 +20,26 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import GGML_BF16, GGML_F16, GGML_F32, AttnShared, IllegalStateError, Pages, check, lib
+from ._lib import GGML_BF16, GGML_F16, GGML_F32, AttnShared, IllegalStateError, Pages, check
 
 _TYPES = {torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
+_INT32 = torch.int32
 _STATUS = {_lib.PAGES_BAD_ROW: "a row is out of range or named twice", _lib.PAGES_FULL: "too few free pages",
            _lib.PAGES_TOO_LONG: "a row would outgrow its table",
            _lib.PAGES_BAD_START: "start does not ascend from 0 or does not fit the rows",
            _lib.PAGES_BAD_PAGE: "a table entry names no held page",
            _lib.PAGES_BAD_SHARED: "a shared length is over max_shared or over what a row's queries see"}
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _need(ok, what):
     if not ok:
         raise ValueError(what)
+
+
+def _shape(t):
+    return f"{t.dtype} {tuple(t.shape)} strides {tuple(t.stride())} on {t.device}"
 
 
 class PagedCache:
@@ -66,66 +72,73 @@ class PagedCache:
               "pool must be a contiguous (2 n_layer, n_pages, n_kv_head, page_tokens, head_dim) float16 or bfloat16 tensor")
         _need(pool.is_cuda, "a paged cache lives on a CUDA device")
         self.pool, self.ref, self.table, self.len, self.device = pool, ref, table, length, pool.device
+        self.dtype, self._index = pool.dtype, pool.device.index
         self.n_layer, self.n_rows = pool.shape[0] // 2, length.numel()
         self.n_kv_head, self.page_tokens, self.head_dim = pool.shape[2:]
+        self._head_strides = (self.head_dim, 1)
         for t, shape, name in ((ref, (pool.shape[1],), "ref"), (length, (self.n_rows,), "len"),
                                (table, (self.n_rows, table.shape[-1]), "table")):
-            _need(t.shape == shape, f"{name} must have shape {shape}, not {tuple(t.shape)}")
-            self._int32(t, name)
+            _need(t.shape == shape and t.dtype == _INT32 and t.device == self.device and t.is_contiguous(),
+                  f"{name} must be a contiguous int32 tensor of shape {shape} on {self.device}")
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
-        c = self._c = Pages(self.device.index, _TYPES[pool.dtype], self.n_layer, self.n_kv_head, self.head_dim,
+        self._lib = _lib.lib()
+        c = self._c = Pages(self._index, _TYPES[pool.dtype], self.n_layer, self.n_kv_head, self.head_dim,
                             self.page_tokens, pool.shape[1], self.n_rows, table.shape[1], pool.data_ptr(), ref.data_ptr(),
                             table.data_ptr(), length.data_ptr(), self.status.data_ptr())
-        self._ref = ctypes.byref(c)
-        c.work_bytes = lib().w4j_op_pages_workspace(self._ref)
-        _need(c.work_bytes, lib().w4j_last_error().decode())
+        self._ref, self._ptr = ctypes.byref(c), ctypes.pointer(c)
+        c.work_bytes = self._lib.w4j_op_pages_workspace(self._ref)
+        _need(c.work_bytes, self._lib.w4j_last_error().decode())
         self._work = torch.empty(c.work_bytes, dtype=torch.uint8, device=self.device)
         c.work = self._work.data_ptr()
 
-    def _int32(self, t, name, n=None):
-        _need(t.dtype == torch.int32 and t.device == self.device and t.is_contiguous(),
-              f"{name} must be a contiguous int32 tensor on {self.device}")
-        _need(n is None or (t.dim() == 1 and t.shape[0] == n), f"{name} must have shape ({n},), not {tuple(t.shape)}")
-        return t.data_ptr()
-
-    def _rows(self, t, name):
-        _need(t.dim() == 1, f"{name} must be one-dimensional")
-        return self._int32(t, name), t.shape[0]
+    def _ints(self, t, name, n=None):
+        """Address and length of a contiguous int32 vector on the cache's device."""
+        if t.dtype is not _INT32 or t.dim() != 1 or t.get_device() != self._index or not t.is_contiguous() or (
+                n is not None and t.numel() != n):
+            raise ValueError(f"{name} must be a contiguous int32 vector{'' if n is None else f' of {n}'} on {self.device}, "
+                             f"not {_shape(t)}")
+        return t.data_ptr(), t.numel()
 
     def extend(self, rows, start):
         """Grow row rows[i] by start[i + 1] - start[i] tokens; ``write`` brings their keys and values."""
-        r, n = self._rows(rows, "rows")
-        check(lib().w4j_op_pages_extend(self._ref, r, self._int32(start, "start", n + 1), n, _stream(self.device)))
+        r, n = self._ints(rows, "rows")
+        s, _ = self._ints(start, "start", n + 1)
+        check(self._lib.w4j_op_pages_extend(self._ref, r, s, n, _raw_stream(self._index)))
 
     def write(self, layer, rows, start, k, v):
         """Keys and values (n_tokens, n_kv_head, head_dim) of the tokens that ``extend(rows, start)`` made room for."""
-        r, n = self._rows(rows, "rows")
-        for t, name in ((k, "k"), (v, "v")):
-            _need(t.dtype == self.pool.dtype and t.device == self.device, f"{name} must be {self.pool.dtype} on {self.device}")
-            _need(t.dim() == 3 and t.shape[0] == k.shape[0] and t.shape[1:] == (self.n_kv_head, self.head_dim) and
-                  t.stride(2) == 1 and (t.stride(1) == self.head_dim or self.n_kv_head == 1),
-                  f"{name} must be (n_tokens, {self.n_kv_head}, {self.head_dim}) with contiguous heads")
-        check(lib().w4j_op_pages_write(self._ref, layer, r, self._int32(start, "start", n + 1), n, k.data_ptr(),
-                                       self._token_stride(k), v.data_ptr(), self._token_stride(v), k.shape[0],
-                                       _stream(self.device)))
+        r, n = self._ints(rows, "rows")
+        s, _ = self._ints(start, "start", n + 1)
+        ks, tokens = self._tokens(k, "k"), k.shape[0]
+        vs = self._tokens(v, "v")
+        _need(v.shape[0] == tokens, "k and v must have the same tokens")
+        check(self._lib.w4j_op_pages_write(self._ref, layer, r, s, n, k.data_ptr(), ks, v.data_ptr(), vs, tokens,
+                                           _raw_stream(self._index)))
 
-    def _token_stride(self, t):
-        return t.stride(0) if t.shape[0] > 1 else self.n_kv_head * self.head_dim
+    def _tokens(self, t, name):
+        """Elements from one token of k or v to the next."""
+        shape, stride = t.shape, t.stride()
+        if t.dtype is not self.dtype or t.get_device() != self._index or len(shape) != 3 or shape[1] != self.n_kv_head or (
+                shape[2] != self.head_dim) or (stride[1:] != self._head_strides and (self.n_kv_head > 1 or stride[2] != 1)):
+            raise ValueError(f"{name} must be (n_tokens, {self.n_kv_head}, {self.head_dim}) {self.dtype} with contiguous heads "
+                             f"on {self.device}, not {_shape(t)}")
+        return stride[0] if shape[0] > 1 else self.n_kv_head * self.head_dim
 
     def fork(self, dst, src):
         """Row dst[i] becomes what row src[i] was before the call (-1: empty), for all i at once."""
-        d, n = self._rows(dst, "dst")
-        check(lib().w4j_op_pages_fork(self._ref, d, self._int32(src, "src", n), n, _stream(self.device)))
+        d, n = self._ints(dst, "dst")
+        s, _ = self._ints(src, "src", n)
+        check(self._lib.w4j_op_pages_fork(self._ref, d, s, n, _raw_stream(self._index)))
 
     def free(self, rows):
         """Empty the rows; pages that nobody else holds become free."""
-        r, n = self._rows(rows, "rows")
-        check(lib().w4j_op_pages_free(self._ref, r, n, _stream(self.device)))
+        r, n = self._ints(rows, "rows")
+        check(self._lib.w4j_op_pages_free(self._ref, r, n, _raw_stream(self._index)))
 
     def compact(self):
         """Move the held pages to the front of the pool; returns their number as a (1,) int32 tensor."""
         live = torch.empty(1, dtype=torch.int32, device=self.device)
-        check(lib().w4j_op_pages_compact(self._ref, live.data_ptr(), _stream(self.device)))
+        check(self._lib.w4j_op_pages_compact(self._ref, live.data_ptr(), _raw_stream(self._index)))
         return live
 
     def attend(self, layer, q, rows, group_start, shared, max_shared, max_own, scale=None, out=None):
@@ -136,37 +149,39 @@ class PagedCache:
         first shared[g] tokens: they are read once for the group.  max_shared and max_own are upper bounds, known on
         the host, of shared and of the rows' tokens behind it.  ``scale`` defaults to head_dim ** -0.5.
         """
-        _need(q.dim() == 4 and q.dtype == self.pool.dtype and q.device == self.device,
-              f"q must be (n_seq, n_query, n_head, head_dim) {self.pool.dtype} on {self.device}")
-        n_seq, n_query, n_head, dim = q.shape
+        if q.dim() != 4 or q.dtype is not self.dtype or q.get_device() != self._index or q.shape[3] != self.head_dim:
+            raise ValueError(f"q must be (n_seq, n_query, n_head, {self.head_dim}) {self.dtype} on {self.device}, not {_shape(q)}")
+        n_seq, n_query, n_head, _ = q.shape
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, "out must be like q")
-        _need(dim == self.head_dim, f"q has heads of {dim} in a cache of {self.head_dim}")
+        elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != self._index:
+            raise ValueError(f"out must be like q, not {_shape(out)}")
         if q.numel() == 0:
             return out
-        r, _ = self._rows(rows, "rows")
-        _need(rows.shape[0] == n_seq, f"rows must have shape ({n_seq},)")
-        g, n = self._rows(shared, "shared")
-        a = AttnShared(ctypes.pointer(self._c), layer, n_head, n_query, n_seq, n, max_shared, max_own,
+        r, _ = self._ints(rows, "rows", n_seq)
+        sh, n = self._ints(shared, "shared")
+        g, _ = self._ints(group_start, "group_start", n + 1)
+        a = AttnShared(self._ptr, layer, n_head, n_query, n_seq, n, max_shared, max_own,
                        self.head_dim ** -0.5 if scale is None else scale, q.data_ptr(), out.data_ptr(),
-                       self._query_stride(q, "q"), self._query_stride(out, "out"), r,
-                       self._int32(group_start, "group_start", n + 1), g)
+                       self._query_stride(q, "q"), self._query_stride(out, "out"), r, g, sh)
         ref = ctypes.byref(a)
-        a.work_bytes = lib().w4j_op_attn_shared_workspace(ref)
-        _need(a.work_bytes, lib().w4j_last_error().decode())
-        work = torch.empty(a.work_bytes, dtype=torch.uint8, device=self.device)
-        a.work = work.data_ptr()
-        check(lib().w4j_op_attn_shared(ref, _stream(self.device)))
+        n_bytes = self._lib.w4j_op_attn_shared_workspace(ref)
+        if not n_bytes:
+            raise ValueError(self._lib.w4j_last_error().decode())
+        work = torch.empty(n_bytes, dtype=torch.uint8, device=self.device)
+        a.work, a.work_bytes = work.data_ptr(), n_bytes
+        check(self._lib.w4j_op_attn_shared(ref, _raw_stream(self._index)))
         return out
 
     @staticmethod
     def _query_stride(t, name):
         """Elements from one query token to the next; sequences follow one another."""
         n_seq, n_query, n_head, dim = t.shape
+        if t.is_contiguous():
+            return n_head * dim
         stride = t.stride(1) if n_query > 1 else t.stride(0) if n_seq > 1 else n_head * dim
-        _need((dim == 1 or t.stride(3) == 1) and (n_head == 1 or t.stride(2) == dim) and
-              (n_seq == 1 or t.stride(0) == n_query * stride), f"{name} must have contiguous heads and evenly spaced tokens")
+        _need(t.stride(3) == 1 and (n_head == 1 or t.stride(2) == dim) and (n_seq == 1 or t.stride(0) == n_query * stride),
+              f"{name} must have contiguous heads and evenly spaced tokens")
         return stride
 
     def check(self):
@@ -177,33 +192,42 @@ class PagedCache:
             raise IllegalStateError("; ".join(text for bit, text in _STATUS.items() if bits & bit))
 
 
-def _vector(t, n, device, name):
-    _need(t.dtype == torch.float32 and t.device == device and t.is_contiguous() and t.shape == (n,),
-          f"{name} must be a contiguous float32 tensor of shape ({n},) on {device}")
+def _vector(t, n, index, name):
+    if t.dtype is not torch.float32 or t.dim() != 1 or t.numel() != n or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 vector of {n} on cuda:{index}, not {_shape(t)}")
     return t.data_ptr()
 
 
-def _ld(t):
-    """Elements from one row of a matrix to the next."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
 def _matrix(t, name):
-    _need(t.dim() == 2 and t.dtype in _TYPES and t.is_cuda, f"{name} must be a float32, float16 or bfloat16 matrix on a CUDA device")
-    _need((t.shape[1] == 1 or t.stride(1) == 1) and _ld(t) >= t.shape[1], f"{name} must have contiguous rows")
+    """Rows, columns and elements from one row to the next of a float matrix with contiguous rows."""
+    if t.dim() != 2 or t.dtype not in _TYPES or not t.is_cuda:
+        raise ValueError(f"{name} must be a float32, float16 or bfloat16 matrix on a CUDA device, not {_shape(t)}")
+    m, n = t.shape
+    ld, inner = t.stride()
+    if m <= 1:
+        ld = n
+    if (n > 1 and inner != 1) or ld < n:
+        raise ValueError(f"{name} must have contiguous rows, not {_shape(t)}")
+    return m, n, ld
+
+
+def _norm(ln, k, index):
+    if ln is None:
+        return None, None
+    return _vector(ln[0], k, index, "gamma"), _vector(ln[1], k, index, "beta")
 
 
 def quantize_rows(x, ln=None):
     """x (M, K) -> (q, scale): q (M, K rounded up to 16) int8 = round(LayerNorm?(x) / scale), zeros behind K, and
     scale (M,) = max |row| / 127.  ``ln`` is (gamma, beta)."""
-    _matrix(x, "x")
-    m, k = x.shape
+    m, k, ld = _matrix(x, "x")
     q = torch.empty(m, (k + 15) // 16 * 16, dtype=torch.int8, device=x.device)
     scale = torch.empty(m, dtype=torch.float32, device=x.device)
     if m:
-        g, b = (None, None) if ln is None else (_vector(t, k, x.device, "ln") for t in ln)
-        check(lib().w4j_op_quantize_rows(x.device.index, x.data_ptr(), _TYPES[x.dtype], m, k, _ld(x), g, b, q.data_ptr(),
-                                         q.shape[1], scale.data_ptr(), _stream(x.device)))
+        index = x.get_device()
+        g, b = _norm(ln, k, index)
+        check(_lib.lib().w4j_op_quantize_rows(index, x.data_ptr(), _TYPES[x.dtype], m, k, ld, g, b, q.data_ptr(), q.shape[1],
+                                              scale.data_ptr(), _raw_stream(index)))
     return q, scale
 
 
@@ -217,17 +241,17 @@ class Int8Linear:
         _need(weight.dim() == 2 and weight.dtype == torch.int8 and weight.is_cuda and 0 not in weight.shape,
               "weight must be an int8 matrix on a CUDA device")
         self.n, self.k = weight.shape
-        self.device = weight.device
+        self.device, self._index = weight.device, weight.get_device()
         k16 = (self.k + 15) // 16 * 16
         if k16 != self.k or not weight.is_contiguous() or weight.data_ptr() % 16:
             # laid out once: rows of a multiple of 16 bytes, zeros behind K
             padded = torch.zeros(self.n, k16, dtype=torch.int8, device=weight.device)
             padded[:, :self.k] = weight
             weight = padded
-        _vector(scale, self.n, self.device, "scale")
-        if bias is not None:
-            _vector(bias, self.n, self.device, "bias")
+        self._scale = _vector(scale, self.n, self._index, "scale")
+        self._bias = None if bias is None else _vector(bias, self.n, self._index, "bias")
         self.weight, self.scale, self.bias = weight, scale, bias
+        self._weight, self._k16, self._lib = weight.data_ptr(), k16, _lib.lib()
 
     @classmethod
     def from_float(cls, weight, bias=None):
@@ -237,20 +261,28 @@ class Int8Linear:
 
     def __call__(self, x, ln=None, epilogue="store", out=None, out_dtype=None):
         """x (M, K) -> (M, N) of ``out_dtype`` (default: x's), or into ``out``; epilogue "gelu", or "residual": out += ..."""
-        _matrix(x, "x")
-        _need(x.device == self.device and x.shape[1] == self.k, f"x must be (M, {self.k}) on {self.device}")
-        _need(epilogue in self.EPILOGUES, f"epilogue must be one of {sorted(self.EPILOGUES)}")
-        m = x.shape[0]
+        m, k, ldx = _matrix(x, "x")
+        index, code = self._index, self.EPILOGUES.get(epilogue)
+        if k != self.k or x.get_device() != index:
+            raise ValueError(f"x must be (M, {self.k}) on {self.device}, not {_shape(x)}")
+        if code is None:
+            raise ValueError(f"epilogue must be one of {sorted(self.EPILOGUES)}")
         if out is None:
-            _need(epilogue != "residual", "a residual needs the tensor that it is added to: out")
-            out = torch.empty(m, self.n, dtype=out_dtype or x.dtype, device=self.device)
-        _matrix(out, "out")
-        _need(out.shape == (m, self.n) and out.device == self.device, f"out must be ({m}, {self.n}) on {self.device}")
-        _need(out_dtype is None or out.dtype == out_dtype, "out is not of out_dtype")
-        if m:
-            q, xs = quantize_rows(x, ln)
-            check(lib().w4j_op_linear_i8(self.device.index, q.data_ptr(), q.shape[1], xs.data_ptr(), m, self.k,
-                                         self.weight.data_ptr(), self.weight.shape[1], self.scale.data_ptr(), self.n,
-                                         None if self.bias is None else self.bias.data_ptr(), self.EPILOGUES[epilogue],
-                                         out.data_ptr(), _TYPES[out.dtype], _ld(out), _stream(self.device)))
+            _need(code != 2, "a residual needs the tensor that it is added to: out")
+            out = torch.empty(m, self.n, dtype=out_dtype or x.dtype, device=x.device)
+            ldy = self.n
+        else:
+            rows, n, ldy = _matrix(out, "out")
+            if rows != m or n != self.n or out.get_device() != index or (out_dtype is not None and out.dtype is not out_dtype):
+                raise ValueError(f"out must be ({m}, {self.n}) of out_dtype on {self.device}, not {_shape(out)}")
+        if not m:
+            return out
+        g, b = _norm(ln, k, index)
+        stream, k16 = _raw_stream(index), self._k16
+        work = torch.empty(m * (k16 + 4), dtype=torch.int8, device=x.device)  # the integers, then the rows' scales
+        q = work.data_ptr()
+        xs = q + m * k16
+        check(self._lib.w4j_op_quantize_rows(index, x.data_ptr(), _TYPES[x.dtype], m, k, ldx, g, b, q, k16, xs, stream))
+        check(self._lib.w4j_op_linear_i8(index, q, k16, xs, m, k, self._weight, k16, self._scale, self.n, self._bias, code,
+                                         out.data_ptr(), _TYPES[out.dtype], ldy, stream))
         return out
