@@ -26,7 +26,7 @@ BAD_CACHES = [(dict(type=GGML_F32), "type"), (dict(head_dim=96), "head_dim"), (d
               (dict(n_kv_head=-1), "n_kv_head"), (dict(n_pages=0), "n_pages"), (dict(n_pages=(1 << 21) + 1), "n_pages"),
               (dict(n_rows=0), "n_rows"), (dict(table_width=0), "table_width"),
               (dict(table_width=1 << 27), "table_width"),
-              (dict(n_pages=1 << 21, n_kv_head=128, page_tokens=16), "2^32")]
+              (dict(n_pages=1 << 21, n_kv_head=64, page_tokens=16), "2^31")]
 BAD_POINTERS = [(dict(pool=None), "null"), (dict(ref=None), "null"), (dict(table=None), "null"), (dict(len=None), "null"),
                 (dict(status=None), "null"), (dict(work=None), "null"), (dict(pool=P + 8), "aligned"),
                 (dict(work=P + 4), "aligned"), (dict(work_bytes=100), "work")]

@@ -83,221 +83,253 @@ __device__ __forceinline__ int warp_find(int n, long long x, Key key) {
     return lo;
 }
 
-// ---------------------------------------------------------------------------
-// one warp: up to 16 query rows against a stretch of keys
-//
-// Fragments come from global memory straight into registers.  The contraction order over the head's
-// dimensions is free, so lane (g, q) = (lane / 4, lane % 4) takes dimensions 32 u + 8 q .. + 7 of key g
-// as one 16-byte load and feeds them to two MMA steps (the queries are laid out alike); the order of the
-// output's columns is free too, so the same lane takes dimensions 8 g .. 8 g + 7 of keys 2 q, 2 q + 1,
-// 2 q + 8, 2 q + 9 and column c of MMA tile t is dimension 8 c + t.  Every load of a warp covers whole
-// 128-byte rows, and no shared memory or transposition is needed.  Bound by HBM as long as rows are few:
-// 16 rows cost 16 flop per byte of the cache.
-// ---------------------------------------------------------------------------
-template <typename T, int D>
-struct WarpTile {
-    static constexpr int KU = D / 32, NW = D / 64;
-    uint32_t qf[2 * KU][4];
-    float o[NW][8][4];
-    float m[2], l[2];
+// Bounded wait that never sleeps: the phases follow one another within a microsecond or two.
+__device__ __forceinline__ bool wait_phase(uint64_t *bar, unsigned parity, int *failed) {
+    for (int it = 0; it < 1 << 24; ++it)
+        if (mbar_test(bar, parity)) return true;
+    atomicExch(failed, 2);
+    return false;
+}
 
-    // rows g and g + 8 of the tile, null where there is none
-    __device__ __forceinline__ void load_q(const T *r0, const T *r1) {
+// ---------------------------------------------------------------------------
+// one warp: 8 NT query rows against a stretch of keys
+//
+// The products are taken the other way round, S^T = K Q^T and O^T = V^T P^T, so that the MMA's 16 rows are keys and
+// dimensions and its 8 columns the few queries; P goes from one fragment layout to the other by an 8 x 8
+// transposition.  Each warp has a ring of its own: a stage holds STEP keys and their values, brought page by page
+// as TMA boxes (128-byte swizzle, read back by ldmatrix), so that a stage is in flight while another is worked on
+// without holding registers, and no warp waits for another.  Bound by HBM.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+
+constexpr int kAsWarps = 4, kAsStages = 2, kAsStage = 8192;  // bytes of a stage: its keys, then their values
+constexpr size_t kAsSmem = (size_t)kAsWarps * kAsStages * kAsStage + 1024;
+
+template <typename T, int D, int NT>
+struct WarpTile {
+    static constexpr int NB = D / 64, STEP = 32 / NB, H = STEP / 16, kBlock = STEP * 128, kKeys = NB * kBlock;
+    uint32_t qf[NT][D / 16][2];
+    float o[NT][D / 16][4];  // dimension 16 t + g + 8 (e >> 1), query 8 n + 2 q + (e & 1)
+    float m[NT][2], l[NT][2];
+
+    // row[n]: query 8 n + g, null where there is none
+    __device__ __forceinline__ void load_q(const T *const (&row)[NT]) {
         const int q = threadIdx.x & 3;
 #pragma unroll
-        for (int u = 0; u < KU; ++u) {
-            uint4 a = make_uint4(0, 0, 0, 0), b = a;
-            if (r0) a = __ldg(reinterpret_cast<const uint4 *>(r0 + 32 * u + 8 * q));
-            if (r1) b = __ldg(reinterpret_cast<const uint4 *>(r1 + 32 * u + 8 * q));
-            qf[2 * u][0] = a.x, qf[2 * u][1] = b.x, qf[2 * u][2] = a.y, qf[2 * u][3] = b.y;
-            qf[2 * u + 1][0] = a.z, qf[2 * u + 1][1] = b.z, qf[2 * u + 1][2] = a.w, qf[2 * u + 1][3] = b.w;
-        }
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int w = 0; w < NW; ++w)
+            for (int t = 0; t < D / 16; ++t) {
 #pragma unroll
-            for (int t = 0; t < 8; ++t) o[w][t][0] = o[w][t][1] = o[w][t][2] = o[w][t][3] = 0.f;
-        m[0] = m[1] = kNone;
-        l[0] = l[1] = 0.f;
-    }
-
-    // o += P V for 16 keys; p: the A fragment, v0 .. v3: keys 2 q, 2 q + 1, 2 q + 8, 2 q + 9
-    __device__ __forceinline__ void pv(const uint32_t (&p)[4], const uint4 (&v)[NW][4]) {
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const uint32_t *x0 = &v[w][0].x, *x1 = &v[w][1].x, *x2 = &v[w][2].x, *x3 = &v[w][3].x;
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const uint32_t sel = t & 1 ? 0x7632u : 0x5410u;
-                mma<T>(o[w][t], p, __byte_perm(x0[t / 2], x1[t / 2], sel), __byte_perm(x2[t / 2], x3[t / 2], sel));
+                for (int i = 0; i < 2; ++i)
+                    qf[n][t][i] = row[n] ? __ldg(reinterpret_cast<const uint32_t *>(row[n] + 16 * t + 8 * i + 2 * q)) : 0;
+                o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.f;
             }
+            m[n][0] = m[n][1] = kNone, l[n][0] = l[n][1] = 0.f;
         }
     }
 
-    // Keys [k0, k1) of the row whose table is `table`; row r of the tile sees those below lim[r] (r = g, g + 8)
-    // and all rows see those below `all`.  plane_k / plane_v: the head rows of the layer.
-    __device__ __forceinline__ void run(const PagesArgs &p, const int *table, int head, const T *plane_k, const T *plane_v,
-                                        int k0, int k1, const int (&lim)[2], int all, float scale_log2, int *bad) {
+    // Keys [k0, k1) of the row whose table is `table`.  Query 8 n + 2 q + i sees the keys below lim[n][i], all
+    // queries see those below `all`.  sm: the warp's ring, full: a barrier for each stage; box: rows of a TMA box.
+    __device__ __forceinline__ void run(const PagesArgs &p, const int *table, int head, const CUtensorMap *kmap,
+                                        const CUtensorMap *vmap, unsigned char *sm, uint64_t *full, int box, int k0, int k1,
+                                        const int (&lim)[NT][2], int all, float scale_log2, int *bad, int *failed) {
         const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-        for (int kb = k0; kb < k1; kb += 32) {
-            // lane i finds head row kb + i
-            const int key = kb + lane;
-            uint32_t at = 0;
-            if (key < k1) {
-                const int j = key / p.page_tokens;
-                int page = __ldg(table + j);
-                if (page < 0 || page >= p.n_pages) *bad = 1, page = 0;
-                at = ((uint32_t)page * p.n_kv_head + head) * p.page_tokens + (key - j * p.page_tokens);
+        if (k0 >= k1) return;
+        const int start = k0 / box * box, n_steps = (k1 - start + STEP - 1) / STEP;  // boxes do not cross pages
+        // lane b (keys) and lane 16 + b (values) bring box b of a step; page and place in it of its first key
+        int key = start + (lane & 15) * box, j = key / p.page_tokens, tok = key - j * p.page_tokens;
+        const int dj = STEP / p.page_tokens, dt = STEP - dj * p.page_tokens;
+        const bool mine = (lane & 15) * box < STEP;
+        int page = mine && key < k1 ? __ldg(table + j) : 0;
+        auto issue = [&](int i) {
+            const int at = start + i * STEP, boxes = (min(STEP, k1 - at) + box - 1) / box, st = i % kAsStages;
+            if (lane == 0) mbar_expect_tx(full + st, 2 * NB * boxes * box * 128);
+            if (page < 0 || page >= p.n_pages) *bad = 1, page = 0;
+            const int y = (page * p.n_kv_head + head) * p.page_tokens + tok;
+            __syncwarp();
+            if ((lane & 15) < boxes) {
+                unsigned char *dst = sm + st * kAsStage + (lane >> 4) * kKeys + (lane & 15) * box * 128;
+                for (int b = 0; b < NB; ++b) tma_load_2d(dst + b * kBlock, lane < 16 ? kmap : vmap, 64 * b, y, full + st);
             }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int k16 = kb + 16 * c;
-                if (k16 >= k1) break;
-                uint4 kf[2][KU], vf[NW][4];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const size_t r = __shfl_sync(0xffffffffu, at, 16 * c + 8 * i + g);
-#pragma unroll
-                    for (int u = 0; u < KU; ++u)
-                        kf[i][u] = __ldg(reinterpret_cast<const uint4 *>(plane_k + r * D + 32 * u + 8 * q));
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int kk = (i >> 1) * 8 + 2 * q + (i & 1);
-                    const size_t r = __shfl_sync(0xffffffffu, at, 16 * c + kk);
-#pragma unroll
-                    for (int w = 0; w < NW; ++w)  // behind the last key there may be anything: zero
-                        vf[w][i] = k16 + kk < k1 ? __ldg(reinterpret_cast<const uint4 *>(plane_v + r * D + 64 * w + 8 * g))
-                                                 : make_uint4(0, 0, 0, 0);
-                }
-                float s[2][4] = {};
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int u = 0; u < KU; ++u) {
-                        mma<T>(s[i], qf[2 * u], kf[i][u].x, kf[i][u].y);
-                        mma<T>(s[i], qf[2 * u + 1], kf[i][u].z, kf[i][u].w);
-                    }
-                // s[i][e]: key k16 + 8 i + 2 q + (e & 1), row g + 8 (e >> 1)
-                float mx[2] = {m[0], m[1]};
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[i][e] = k16 + 8 * i + 2 * q + (e & 1) < min(k1, lim[e >> 1]) ? s[i][e] * scale_log2 : kNone;
-                        mx[e >> 1] = fmaxf(mx[e >> 1], s[i][e]);
-                    }
-                float f[2], sum[2] = {0.f, 0.f};
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                    f[r] = m[r] == mx[r] ? 1.f : ex2(m[r] - mx[r]);
-                    m[r] = mx[r];
-                    if (mx[r] == kNone) mx[r] = 0.f;  // nothing seen so far: all weights are 0
-                }
-                uint32_t pf[4];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[i][e] = ex2(s[i][e] - mx[e >> 1]);
-                        sum[e >> 1] += s[i][e];
-                    }
-                pf[0] = pack2<T>(s[0][0], s[0][1]), pf[1] = pack2<T>(s[0][2], s[0][3]);
-                pf[2] = pack2<T>(s[1][0], s[1][1]), pf[3] = pack2<T>(s[1][2], s[1][3]);
-#pragma unroll
-                for (int r = 0; r < 2; ++r) l[r] = l[r] * f[r] + sum[r];  // this lane's keys; summed over q at the end
-                if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f))
-#pragma unroll
-                    for (int w = 0; w < NW; ++w)
-#pragma unroll
-                        for (int t = 0; t < 8; ++t)
-                            o[w][t][0] *= f[0], o[w][t][1] *= f[0], o[w][t][2] *= f[1], o[w][t][3] *= f[1];
-                if (k16 + 16 > all && hides(vf))
-                    pv_hidden(pf, vf, k16, lim);
-                else
-                    pv(pf, vf);
+            __syncwarp();
+            key += STEP, j += dj, tok += dt;
+            if (tok >= p.page_tokens) tok -= p.page_tokens, ++j;
+            page = mine && key < k1 ? __ldg(table + j) : 0;  // for the next call
+        };
+        for (int i = 0; i < kAsStages && i < n_steps; ++i) issue(i);
+        // ldmatrix rows: keys as they lie, values transposed
+        const int kr = lane & 15, kc = lane >> 4, vr = (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;
+        int i = 0;
+        for (; i < n_steps; ++i) {
+            const int st = i % kAsStages, kb = start + i * STEP;
+            if (!__all_sync(0xffffffffu, wait_phase(full + st, (i / kAsStages) & 1, failed))) break;
+            const uint32_t sk = smem_u32(sm + st * kAsStage), sv = sk + kKeys;
+            const bool masked = kb < k0 || kb + STEP > min(k1, all);
+            if (kb + STEP > k1) {  // behind the last key there may be anything: zero
+                for (int x = lane; x < (kb + STEP - k1) * 8 * NB; x += 32)
+                    *reinterpret_cast<uint4 *>(sm + st * kAsStage + kKeys + x % NB * kBlock + (k1 - kb) * 128 + x / NB * 16) =
+                        make_uint4(0, 0, 0, 0);
+                __syncwarp();
             }
+            float s[NT][H][4];  // key 16 h + g + 8 (e >> 1), query 8 n + 2 q + (e & 1)
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s[n][h][0] = s[n][h][1] = s[n][h][2] = s[n][h][3] = 0.f;
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) {
+                    uint32_t a[4];
+                    ldsm4(a, sk + t / 4 * kBlock + (16 * h + kr) * 128 + (((2 * t + kc) & 7) ^ (kr & 7)) * 16);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma<T>(s[n][h], a, qf[n][t][0], qf[n][t][1]);
+                }
+            }
+            uint32_t pf[NT][H][2];
+            float c[NT][2];
+            bool grown = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int sees = min(k1, lim[n][x]) - kb - g, from = k0 - kb - g;
+                    float mx = kNone;
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+#pragma unroll
+                        for (int e = x; e < 4; e += 2) {
+                            const int at = 16 * h + 8 * (e >> 1);
+                            if (masked && (at >= sees || at < from)) s[n][h][e] = kNone;
+                            mx = fmaxf(mx, s[n][h][e]);
+                        }
+#pragma unroll
+                    for (int y = 4; y < 32; y *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, y));
+                    mx = fmaxf(m[n][x], mx * scale_log2);
+                    c[n][x] = m[n][x] == mx ? 1.f : ex2(m[n][x] - mx);
+                    grown |= c[n][x] != 1.f;
+                    m[n][x] = mx;
+                    if (mx == kNone) mx = 0.f;  // nothing seen so far: all weights are 0
+                    float sum = 0.f;
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+#pragma unroll
+                        for (int e = x; e < 4; e += 2) {
+                            s[n][h][e] = ex2(fmaf(s[n][h][e], scale_log2, -mx));
+                            sum += s[n][h][e];
+                        }
+                    l[n][x] = l[n][x] * c[n][x] + sum;  // this lane's keys; summed over g at the end
+                }
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) pf[n][h][x] = transpose8(pack2<T>(s[n][h][2 * x], s[n][h][2 * x + 1]));
+            }
+            if (__any_sync(0xffffffffu, grown))
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[n][t][e] *= c[n][e & 1];
+            const bool hidden = kb + STEP > all && hides(sm + st * kAsStage + kKeys);
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) {
+                    uint32_t a[4];
+                    ldsm4_t(a, sv + t / 4 * kBlock + (16 * h + vr) * 128 + (((2 * t + vc) & 7) ^ (vr & 7)) * 16);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        if (hidden)
+                            add_hidden(o[n][t], a, pf[n][h], lim[n], kb + 16 * h);
+                        else
+                            mma<T>(o[n][t], a, pf[n][h][0], pf[n][h][1]);
+                }
+            __syncwarp();
+            if (i + kAsStages < n_steps) issue(i + kAsStages);
         }
+        // after a wait that ran out: let the copies in flight land before the block's shared memory goes on
+        for (int x = i; x < min(n_steps, i + kAsStages); ++x)
+            for (int it = 0; it < 1 << 20 && !mbar_test(full + x % kAsStages, (x / kAsStages) & 1); ++it) {
+            }
     }
 
-    // Where a key that only some rows see holds an infinity or a NaN, 0 x v is none: the rows take their
+    // Where a key that only some queries see holds an infinity or a NaN, 0 x v is none: the queries take their
     // turns, each with the keys that it does not see set to zero.
-    __device__ __forceinline__ bool hides(const uint4 (&v)[NW][4]) {
+    __device__ __forceinline__ bool hides(const unsigned char *values) const {
         bool bad = false;
-#pragma unroll
-        for (int w = 0; w < NW; ++w)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                bad |= not_finite<T>(v[w][i].x) || not_finite<T>(v[w][i].y) || not_finite<T>(v[w][i].z) ||
-                       not_finite<T>(v[w][i].w);
+        for (int x = threadIdx.x & 31; x < kKeys / 16; x += 32) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(values + 16 * x);
+            bad |= not_finite<T>(v.x) || not_finite<T>(v.y) || not_finite<T>(v.z) || not_finite<T>(v.w);
+        }
         return __any_sync(0xffffffffu, bad);
     }
-    __device__ __forceinline__ void pv_hidden(const uint32_t (&p)[4], const uint4 (&v)[NW][4], int k16,
-                                              const int (&lim)[2]) {
+    __device__ __forceinline__ void add_hidden(float (&acc)[4], const uint32_t (&a)[4], const uint32_t (&pf)[2],
+                                               const int (&lim)[2], int k16) {
         const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const uint32_t *x0 = &v[w][0].x, *x1 = &v[w][1].x, *x2 = &v[w][2].x, *x3 = &v[w][3].x;
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const uint32_t sel = t & 1 ? 0x7632u : 0x5410u;
-                const uint32_t b0 = __byte_perm(x0[t / 2], x1[t / 2], sel), b1 = __byte_perm(x2[t / 2], x3[t / 2], sel);
 #pragma unroll 1
-                for (int r = 0; r < 16; ++r) {
-                    const int sees = __shfl_sync(0xffffffffu, r < 8 ? lim[0] : lim[1], (r & 7) * 4) - k16 - 2 * q;
-                    const uint32_t lo = (sees > 0 ? 0xffffu : 0u) | (sees > 1 ? 0xffff0000u : 0u);
-                    const uint32_t hi = (sees > 8 ? 0xffffu : 0u) | (sees > 9 ? 0xffff0000u : 0u);
-                    const bool mine0 = g == r, mine1 = g + 8 == r;
-                    const uint32_t pr[4] = {mine0 ? p[0] : 0, mine1 ? p[1] : 0, mine0 ? p[2] : 0, mine1 ? p[3] : 0};
-                    float acc[4] = {};
-                    mma<T>(acc, pr, b0 & lo, b1 & hi);
-                    // the other rows' 0 x v may be NaN here: only row r takes its sums
-                    if (mine0) o[w][t][0] += acc[0], o[w][t][1] += acc[1];
-                    if (mine1) o[w][t][2] += acc[2], o[w][t][3] += acc[3];
-                }
-            }
+        for (int r = 0; r < 8; ++r) {
+            const int sees = __shfl_sync(0xffffffffu, r & 1 ? lim[1] : lim[0], r >> 1) - k16 - 2 * q;
+            const uint32_t lo = (sees > 0 ? 0xffffu : 0u) | (sees > 1 ? 0xffff0000u : 0u);
+            const uint32_t hi = (sees > 8 ? 0xffffu : 0u) | (sees > 9 ? 0xffff0000u : 0u);
+            const uint32_t ar[4] = {a[0] & lo, a[1] & lo, a[2] & hi, a[3] & hi};
+            float x[4] = {};
+            mma<T>(x, ar, g == r ? pf[0] : 0, g == r ? pf[1] : 0);
+            // the other queries' 0 x v may be NaN here: only query r takes its sums
+            if (2 * q == r) acc[0] += x[0], acc[2] += x[2];
+            if (2 * q + 1 == r) acc[1] += x[1], acc[3] += x[3];
         }
     }
 
-    // o, m (base 2) and l of rows g and g + 8 to their places; null: no such row
-    __device__ __forceinline__ void store(float *o0, float *o1, float *ml0, float *ml1) {
-        const int q = threadIdx.x & 3;
+    // o, m (base 2) and l of query 8 n + 2 q + i to their places; null: no such query
+    __device__ __forceinline__ void store(float *const (&po)[NT][2], float *const (&pm)[NT][2]) {
+        const int g = (threadIdx.x & 31) >> 2;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            float *po = r ? o1 : o0, *pm = r ? ml1 : ml0;
-            if (!po) continue;
-            if (q == 0) pm[0] = m[r], pm[1] = l[r];
-            if (l[r] == 0.f) continue;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int w = 0; w < NW; ++w)
+            for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c)  // column 2 q + c of tiles 0 .. 7: dimensions 64 w + 16 q + 8 c .. + 7
+                for (int x = 4; x < 32; x *= 2) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], x);
+                if (!po[n][i]) continue;
+                if (g == 0) *reinterpret_cast<float2 *>(pm[n][i]) = make_float2(m[n][i], l[n][i]);
+                if (l[n][i] == 0.f) continue;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        *reinterpret_cast<float4 *>(po + 64 * w + 16 * q + 8 * c + 4 * h) =
-                            make_float4(o[w][4 * h][2 * r + c], o[w][4 * h + 1][2 * r + c], o[w][4 * h + 2][2 * r + c],
-                                        o[w][4 * h + 3][2 * r + c]);
-        }
+                for (int t = 0; t < D / 16; ++t) po[n][i][16 * t + g] = o[n][t][i], po[n][i][16 * t + 8 + g] = o[n][t][2 + i];
+            }
     }
 };
 
 // ---------------------------------------------------------------------------
 // items: (group tile, head, split) of the shared keys, then (row, head, tile, split) of the rows' own
 // ---------------------------------------------------------------------------
-constexpr int kAsWarps = 4;
-
-template <typename T, int D>
-__global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(AttnSharedArgs a) {
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_constant__ CUtensorMap kmap,
+                                                               const __grid_constant__ CUtensorMap vmap, AttnSharedArgs a,
+                                                               int box) {
+    extern __shared__ unsigned char raw[];
+    __shared__ uint64_t full[kAsWarps][kAsStages];
+    __shared__ int failed[kAsWarps];
     pdl_wait();
     pdl_trigger();
+    constexpr int R = 8 * NT;  // query rows of a tile
     const PagesArgs &p = a.p;
-    const int lane = threadIdx.x & 31, g = lane >> 2;
+    const int lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3;
     const int c = a.n_query * a.rep;  // query rows of one sequence and one key/value head
-    const size_t plane = (size_t)p.n_pages * p.n_kv_head * p.page_tokens * D;
-    const T *pk = reinterpret_cast<const T *>(p.pool) + 2 * a.layer * plane, *pv = pk + plane;
     const T *q = reinterpret_cast<const T *>(a.q);
     unsigned item = blockIdx.x * kAsWarps + (threadIdx.x >> 5);
     int seq0, n_rows, head, split, tile, slot, k0, k1, own_len, bad = 0;
@@ -306,15 +338,15 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(AttnSharedArgs a)
         tile = (int)(item % a.shared_tiles);
         split = (int)(item / a.shared_tiles % a.shared_splits);
         head = (int)(item / a.shared_tiles / a.shared_splits);
-        // group gr has tiles gs c / 16 + gr on (rounded down), one more than it may need
-        const int gr = warp_find(a.n_group, tile, [&](int i) { return (long long)__ldg(a.group_start + i) * c / 16 + i; });
+        // group gr has tiles gs c / R + gr on (rounded down), one more than it may need
+        const int gr = warp_find(a.n_group, tile, [&](int i) { return (long long)__ldg(a.group_start + i) * c / R + i; });
         seq0 = __ldg(a.group_start + gr);
         const int seq1 = __ldg(a.group_start + gr + 1);
         if (seq0 < 0 || seq1 <= seq0 || seq1 > a.n_seq) return;
-        tile -= (int)((long long)seq0 * c / 16) + gr;
+        tile -= (int)((long long)seq0 * c / R) + gr;
         n_rows = (seq1 - seq0) * c;
         const int r = __ldg(a.rows + seq0), s = min(__ldg(a.shared + gr), a.max_shared);
-        if (tile < 0 || tile * 16 >= n_rows || r < 0 || r >= p.n_rows) return;
+        if (tile < 0 || tile * R >= n_rows || r < 0 || r >= p.n_rows) return;
         table = p.table + (size_t)r * p.width;
         const int len = max(0, min(min(s, __ldg(p.len + r)), p.width * p.page_tokens));
         const int step = ((len + a.shared_splits - 1) / a.shared_splits + 31) / 32 * 32;
@@ -348,33 +380,47 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(AttnSharedArgs a)
         k0 = from + min(n, split * step), k1 = min(from + n, k0 + step);
         slot = a.shared_splits + split;
     }
-    WarpTile<T, D> w;
-    // rows g and g + 8 of the tile: (sequence, query token, head) of each
-    const T *qr[2];
-    float *po[2], *pm[2];
-    int lim[2];
+    // query r of the tile: (sequence, query token, head)
+    auto token_of = [&](int r) { return (size_t)(seq0 + r / c) * a.n_query + r % c / a.rep; };
+    const T *qr[NT];
+    float *po[NT][2], *pm[NT][2];
+    int lim[NT][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = tile * 16 + g + 8 * i;
-        qr[i] = nullptr, po[i] = pm[i] = nullptr, lim[i] = 0;
-        if (r >= n_rows) continue;
-        const int seq = seq0 + r / c, t = r % c / a.rep, h = head * a.rep + r % a.rep;
-        const size_t token = (size_t)seq * a.n_query + t;
-        qr[i] = q + token * a.q_stride + (size_t)h * D;
-        lim[i] = own_len - a.n_query + t + 1;
-        const size_t part = (token * a.n_head + h) * a.slots + slot;
-        po[i] = a.part_o + part * D;
-        pm[i] = a.part_ml + part * 2;
+    for (int n = 0; n < NT; ++n) {
+        const int r = tile * R + 8 * n + g;
+        qr[n] = r < n_rows ? q + token_of(r) * a.q_stride + (size_t)(head * a.rep + r % a.rep) * D : nullptr;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int x = tile * R + 8 * n + 2 * qd + i;
+            po[n][i] = pm[n][i] = nullptr, lim[n][i] = 0;
+            if (x >= n_rows) continue;
+            lim[n][i] = own_len - a.n_query + x % c / a.rep + 1;
+            const size_t part = (token_of(x) * a.n_head + head * a.rep + x % a.rep) * a.slots + slot;
+            po[n][i] = a.part_o + part * D;
+            pm[n][i] = a.part_ml + part * 2;
+        }
     }
+    const int wi = threadIdx.x >> 5;
+    if (lane == 0) {
+        for (int i = 0; i < kAsStages; ++i) mbar_init(&full[wi][i], 1);
+        fence_mbar_init();
+        failed[wi] = 0;
+    }
+    __syncwarp();
+    unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    WarpTile<T, D, NT> w;
     int bad_page = 0;
-    w.load_q(qr[0], qr[1]);
-    w.run(p, table, head, pk, pv, k0, k1, lim, own_len - a.n_query + 1, a.scale_log2, &bad_page);
+    w.load_q(qr);
+    w.run(p, table, head, &kmap, &vmap, sm + wi * kAsStages * kAsStage, full[wi], box, k0, k1, lim, own_len - a.n_query + 1,
+          a.scale_log2, &bad_page, &failed[wi]);
     if (__any_sync(0xffffffffu, bad_page)) bad |= W4J_PAGES_BAD_PAGE;
-    if (bad) {
-        w.m[0] = w.m[1] = w.l[0] = w.l[1] = NAN;  // the join hands it on to the whole row
-        if (lane == 0) atomicOr(p.status, bad);
+    __syncwarp();
+    if (bad || failed[wi]) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) w.m[n][0] = w.m[n][1] = w.l[n][0] = w.l[n][1] = NAN;  // the join hands it on
+        if (lane == 0 && bad) atomicOr(p.status, bad);
     }
-    w.store(po[0], po[1], pm[0], pm[1]);
+    w.store(po, pm);
 }
 
 // ---------------------------------------------------------------------------
@@ -500,7 +546,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
             bool ok = true;
             for (int kv = 0; kv < 2 && ok; ++kv) {
                 uint64_t *full = (kv ? v_full : k_full) + st, *empty = (kv ? v_empty : k_empty) + st;
-                ok = i < NS || mbar_wait(empty, (i / NS - 1) & 1, &failed);
+                ok = i < NS || wait_phase(empty, (i / NS - 1) & 1, &failed);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (lane == 0) mbar_expect_tx(full, boxes * box * 128 * NB);
@@ -527,7 +573,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
             constexpr uint32_t id_s = idesc_f16(128, kTcKeys) | type, id_o = idesc_f16(128, D) | type | (1u << 16);
             auto scores = [&](int i) {
                 const int st = i % NS;
-                if (!mbar_wait(k_full + st, (i / NS) & 1, &failed)) return false;
+                if (!wait_phase(k_full + st, (i / NS) & 1, &failed)) return false;
                 tc_fence_after();
                 const uint32_t q0 = smem_u32(sq), k0 = smem_u32(sk + st * kTile);
 #pragma unroll
@@ -538,10 +584,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
                 umma_commit(k_empty + st);
                 return true;
             };
-            bool ok = mbar_wait(&q_full, 0, &failed) && scores(0) && (n < 2 || scores(1));
+            bool ok = wait_phase(&q_full, 0, &failed) && scores(0) && (n < 2 || scores(1));
             for (int i = 0; i < n && ok; ++i) {
                 const int w = i & 1, st = i % NS;
-                ok = mbar_wait(p_full + w, (i >> 1) & 1, &failed) && mbar_wait(v_full + st, (i / NS) & 1, &failed);
+                ok = wait_phase(p_full + w, (i >> 1) & 1, &failed) && wait_phase(v_full + st, (i / NS) & 1, &failed);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t v0 = smem_u32(sv + st * kTile);
@@ -551,11 +597,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
                 umma_commit(pv_done + w);
                 umma_commit(v_empty + st);
                 // S of tile i + 2 goes where P of tile i is
-                if (i + 2 < n) ok = mbar_wait(pv_done + w, (i >> 1) & 1, &failed) && scores(i + 2);
+                if (i + 2 < n) ok = wait_phase(pv_done + w, (i >> 1) & 1, &failed) && scores(i + 2);
             }
             if (!ok) {  // nothing may be in flight when the tensor memory is given back
                 umma_commit(&drained);
-                mbar_wait(&drained, 0, &failed);
+                wait_phase(&drained, 0, &failed);
             }
         }
     } else {
@@ -573,7 +619,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
         bool ok = true;
         for (int i = w; i < n; i += 2) {
             const int valid = min(kTcKeys, len - (t0 + i) * kTcKeys);
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full + w, (i >> 1) & 1, &failed));
+            ok = __all_sync(0xffffffffu, wait_phase(s_full + w, (i >> 1) & 1, &failed));
             if (!ok) break;
             tc_fence_after();
             uint32_t s[128];
@@ -619,7 +665,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
             tmem_wait_st();
             if (valid < kTcKeys) {  // behind the last key there may be anything: 0 x NaN is none
                 const int st = i % NS;
-                ok = __all_sync(0xffffffffu, mbar_wait(v_full + st, (i / NS) & 1, &failed));
+                ok = __all_sync(0xffffffffu, wait_phase(v_full + st, (i / NS) & 1, &failed));
                 if (!ok) break;
                 for (int x = row; x < (kTcKeys - valid) * 8 * NB; x += 128) {
                     const int at = valid + x / (8 * NB), u = x % (8 * NB);
@@ -634,7 +680,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
         // (its own first: the other's last product but one is done then, so that one parity tells its last two apart)
         for (int x = 0; x < 2 && ok; ++x) {
             const int b = w ^ x, mine = b ? n / 2 : (n + 1) / 2;
-            ok = mine == 0 || mbar_wait(pv_done + b, (mine - 1) & 1, &failed);
+            ok = mine == 0 || wait_phase(pv_done + b, (mine - 1) & 1, &failed);
         }
         __syncwarp();
         tc_fence_after();
@@ -724,22 +770,35 @@ __global__ void __launch_bounds__(256) k_attn_shared_join(AttnSharedArgs a) {
 template <typename T, int D>
 cudaError_t launch(const AttnSharedArgs &a, cudaStream_t s) {
     const long long rows = (long long)a.n_seq * a.n_query * a.n_head;
+    const PagesArgs &p = a.p;
+    const int head_rows = p.n_pages * p.n_kv_head * p.page_tokens;
+    const T *pk = reinterpret_cast<const T *>(p.pool) + (size_t)2 * a.layer * head_rows * D, *pv = pk + (size_t)head_rows * D;
+    alignas(64) CUtensorMap km, vm;
+    // boxes of up to `most` rows that do not cross pages
+    auto maps = [&](int most) {
+        int box = most;
+        while (p.page_tokens % box) box /= 2;
+        return make_tmap_f16_box(&km, pk, head_rows, D, box) && make_tmap_f16_box(&vm, pv, head_rows, D, box) ? box : 0;
+    };
     cudaError_t e;
     if (a.tc_tiles) {
-        const PagesArgs &p = a.p;
-        const int head_rows = p.n_pages * p.n_kv_head * p.page_tokens;
-        int box = 128;
-        while (p.page_tokens % box) box /= 2;
-        const T *pk = reinterpret_cast<const T *>(p.pool) + (size_t)2 * a.layer * head_rows * D;
-        alignas(64) CUtensorMap km, vm;
-        if (!make_tmap_f16_box(&km, pk, head_rows, D, box) || !make_tmap_f16_box(&vm, pk + (size_t)head_rows * D, head_rows, D, box))
-            return cudaErrorInvalidValue;
+        const int box = maps(kTcKeys);
+        if (!box) return cudaErrorInvalidValue;
         if ((e = allow_smem<k_attn_shared_tc<T, D>>(tc_smem(D))) != cudaSuccess) return e;
         e = launch_after(k_attn_shared_tc<T, D>, a.tc_tiles * a.shared_splits * p.n_kv_head, kTcThreads, tc_smem(D), s, 1, km, vm,
                          a, box);
         if (e != cudaSuccess) return e;
     }
-    e = launch_after(k_attn_shared<T, D>, (a.shared_items + a.own_items + kAsWarps - 1) / kAsWarps, kAsWarps * 32, 0, s, 1, a);
+    const int box = maps(2048 / D);
+    if (!box) return cudaErrorInvalidValue;
+    const unsigned blocks = (a.shared_items + a.own_items + kAsWarps - 1) / kAsWarps;
+    if (a.tile_rows == 8) {
+        if ((e = allow_smem<k_attn_shared<T, D, 1>>(kAsSmem)) != cudaSuccess) return e;
+        e = launch_after(k_attn_shared<T, D, 1>, blocks, kAsWarps * 32, kAsSmem, s, 1, km, vm, a, box);
+    } else {
+        if ((e = allow_smem<k_attn_shared<T, D, 2>>(kAsSmem)) != cudaSuccess) return e;
+        e = launch_after(k_attn_shared<T, D, 2>, blocks, kAsWarps * 32, kAsSmem, s, 1, km, vm, a, box);
+    }
     if (e != cudaSuccess) return e;
     return launch_after(k_attn_shared_join<T, D>, (unsigned)((rows + 7) / 8), 256, 0, s, 1, a);
 }
@@ -756,10 +815,13 @@ void attn_shared_plan(AttnSharedArgs &a) {
         const long long n = (want + items - 1) / items, most = (keys + 63) / 64;
         return (int)(n < most ? n : most);
     };
+    // tiles of 16 query rows where a row's own part or, on the warps, a group has more than 8
+    const bool tc = a.max_shared > 0 && a.n_seq * c / a.n_group >= kTcRows;
+    a.tile_rows = c <= 8 && (tc || a.max_shared == 0 || a.n_seq * c / a.n_group <= 8) ? 8 : 16;
     a.tc_tiles = a.shared_tiles = a.shared_splits = 0;
     if (a.max_shared > 0) {
         const long long avg = a.n_seq * c / a.n_group;  // query rows of a group and key/value head
-        if (avg >= kTcRows && (long long)p.n_pages * p.n_kv_head * p.page_tokens < 1ll << 31) {
+        if (tc) {
             a.tc_tiles = (unsigned)(a.n_seq * c / 128 + a.n_group);
             // fewest rounds of blocks over the SMs times key tiles of a block (and about four more to start and join)
             const long long blocks = (avg + 127) / 128 * a.n_group * p.n_kv_head, tiles = (a.max_shared + kTcKeys - 1) / kTcKeys;
@@ -769,12 +831,12 @@ void attn_shared_plan(AttnSharedArgs &a) {
                 if (n == 1 || cost < best) best = cost, a.shared_splits = n;
             }
         } else {
-            a.shared_tiles = (unsigned)(a.n_seq * c / 16 + a.n_group);
+            a.shared_tiles = (unsigned)(a.n_seq * c / a.tile_rows + a.n_group);
             a.shared_splits = splits((long long)a.shared_tiles * p.n_kv_head, a.max_shared);
         }
     }
     a.shared_items = a.shared_tiles * a.shared_splits * p.n_kv_head;
-    a.own_tiles = (int)((c + 15) / 16);
+    a.own_tiles = (unsigned)((c + a.tile_rows - 1) / a.tile_rows);
     const int own = a.max_own > 0 ? splits((long long)a.n_seq * p.n_kv_head * a.own_tiles, a.max_own) : 1;
     a.own_splits = own < 1 ? 1 : own;
     a.own_items = (unsigned)a.n_seq * p.n_kv_head * a.own_tiles * a.own_splits;

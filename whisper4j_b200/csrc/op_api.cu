@@ -28,8 +28,8 @@ int pages_sizes(const w4j_pages *c, const char *who, PagesArgs *out) {
         return set_err(W4J_ERR_ARG, "%s: n_pages must be in [1, 2^21] and n_rows in [1, 2^20]", who);
     if (c->table_width < 1 || (int64_t)c->table_width * c->page_tokens > 1 << 30)
         return set_err(W4J_ERR_ARG, "%s: table_width must be positive and hold at most 2^30 tokens", who);
-    if ((int64_t)c->n_pages * c->n_kv_head * c->page_tokens >= (int64_t)1 << 32)
-        return set_err(W4J_ERR_ARG, "%s: a plane of the pool must have fewer than 2^32 head rows", who);
+    if ((int64_t)c->n_pages * c->n_kv_head * c->page_tokens >= (int64_t)1 << 31)
+        return set_err(W4J_ERR_ARG, "%s: a plane of the pool must have fewer than 2^31 head rows", who);
     *out = PagesArgs{c->n_layer, c->n_kv_head, c->head_dim, c->page_tokens, c->n_pages, c->n_rows, c->table_width,
                      c->pool,    c->ref,       c->table,    c->len,         c->status,  static_cast<int *>(c->work)};
     return W4J_OK;
