@@ -324,7 +324,10 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_cons
     extern __shared__ unsigned char raw[];
     __shared__ uint64_t full[kAsWarps][kAsStages];
     __shared__ int failed[kAsWarps];
-    pdl_wait();
+    // Behind k_attn_shared_tc this kernel starts while that one runs (all of its blocks have waited for whatever came
+    // before, so that is done): the two read the same inputs, write different parts, and one is bound by its
+    // exponentials, the other by HBM.  It then waits for it before it ends, so that the join need only wait for this one.
+    if (!a.tc_tiles) pdl_wait();
     pdl_trigger();
     constexpr int R = 8 * NT;  // query rows of a tile
     const PagesArgs &p = a.p;
@@ -342,7 +345,7 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_cons
         const int gr = warp_find(a.n_group, tile, [&](int i) { return (long long)__ldg(a.group_start + i) * c / R + i; });
         seq0 = __ldg(a.group_start + gr);
         const int seq1 = __ldg(a.group_start + gr + 1);
-        if (seq0 < 0 || seq1 <= seq0 || seq1 > a.n_seq) return;
+        if (seq0 < 0 || seq1 <= seq0 || seq1 > a.n_seq) return;  // (no such items behind k_attn_shared_tc)
         tile -= (int)((long long)seq0 * c / R) + gr;
         n_rows = (seq1 - seq0) * c;
         const int r = __ldg(a.rows + seq0), s = min(__ldg(a.shared + gr), a.max_shared);
@@ -355,7 +358,10 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_cons
         slot = split;
     } else {
         item -= a.shared_items;
-        if (item >= a.own_items) return;
+        if (item >= a.own_items) {
+            if (a.tc_tiles) pdl_wait();
+            return;
+        }
         tile = (int)(item % a.own_tiles);
         split = (int)(item / a.own_tiles % a.own_splits);
         head = (int)(item / a.own_tiles / a.own_splits % p.n_kv_head);
@@ -421,20 +427,23 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_cons
         if (lane == 0 && bad) atomicOr(p.status, bad);
     }
     w.store(po, pm);
+    if (a.tc_tiles) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------
 // shared keys on the 5th-generation tensor cores: 128 query rows of a group against 128 keys at a time
 //
-// S = Q K^T (tcgen05.mma, operands in shared memory) and O += P V (P from tensor memory) with a warpgroup per
-// S buffer: warpgroup w takes tiles w, w + 2, ... with a maximum, sum and O of its own, so that one works on
-// its softmax while the tensor cores work for the other; a thread owns a row, so the softmax needs no shuffle.
-// O is rescaled only when a row's maximum has grown by more than 2^8 (weights up to 2^8 are as good as weights up
-// to 1 in either type), and by the owner itself: S of tile i is there only once tile i - 2 has been added.
-// Keys and values come page by page through TMA boxes (128-byte swizzle) into two rings; V is the MMA's B operand
-// as it lies in the pages (MN-major).
+// S = Q K^T (tcgen05.mma, operands in shared memory) and O += P V (P from tensor memory).  Two warpgroups take the first
+// and the second 64 keys of every tile, each with a maximum, sum and O of its own; a thread owns a row, so the softmax
+// needs no shuffle.  There are two S buffers, P overwrites its S.  O is rescaled only when a row's maximum has grown by
+// more than 2^8 (weights up to 2^8 are as good as weights up to 1 in either type), by its owner, once the products so far
+// are in.  Keys and values come page by page through TMA boxes (128-byte swizzle) into two rings; V is the MMA's B
+// operand as it lies in the pages (MN-major).
+//
+// Bound by the exponentials: 128 x 128 of them take the 16 a cycle of an SM's special function units 1024 cycles, the
+// MMAs of a tile 512 (head 64) or 1024 (head 128).  So some are computed on the FMA pipes instead (exp2_poly).
 // ---------------------------------------------------------------------------
-constexpr int kTcThreads = 320, kTcKeys = 128, kTcBlock = kTcKeys * 128;  // bytes of 128 rows of 64 numbers
+constexpr int kTcThreads = 384, kTcKeys = 128, kTcBlock = 128 * 128;  // bytes of 64 numbers of 128 rows
 
 constexpr int tc_stages(int D) { return D == 64 ? 4 : 3; }
 constexpr size_t tc_smem(int D) { return (size_t)(D / 64) * kTcBlock * (1 + 2 * tc_stages(D)) + 1024; }
@@ -458,8 +467,33 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t *v) {
                    "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),
                    "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
 }
+// two 32-bit numbers at a time
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One lane of a warp that runs as one.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
 
 // A from tensor memory
 __device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -474,17 +508,33 @@ __device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t next)
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(next >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
            (uint64_t)2 << 61;
 }
+// 2^x of two numbers on the FMA pipes, x < 2^7: x = n + f with |f| <= 1/2 (adding 1.5 x 2^23 rounds to n), 2^f by the
+// polynomial of degree 4 with the least relative error there (2.6e-6, a hundredth of P's rounding), n into the exponent.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
+    auto both = [](float v) { return pair(__float_as_uint(v), __float_as_uint(v)); };
+    float a = __uint_as_float((uint32_t)x), b = __uint_as_float((uint32_t)(x >> 32));
+    // below 2^-125 there is nothing left of a weight; a NaN stays one
+    const uint64_t t = pair(__float_as_uint(a < -125.f ? -125.f : a), __float_as_uint(b < -125.f ? -125.f : b));
+    const uint64_t n = add2(t, both(12582912.f)), f = add2(t, neg2(add2(n, both(-12582912.f))));
+    uint64_t y = fma2(both(0.009570102207362652f), f, both(0.05591785907745361f));
+    y = fma2(y, f, both(0.240247443318367f));
+    y = fma2(y, f, both(0.6931217908859253f));
+    y = fma2(y, f, both(0.9999992847442627f));
+    return pair((uint32_t)y + ((uint32_t)n << 23), (uint32_t)(y >> 32) + ((uint32_t)(n >> 32) << 23));
+}
+
+constexpr int kPoly = 10;  // of the 32 pairs of a row of S
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_constant__ CUtensorMap kmap,
                                                                   const __grid_constant__ CUtensorMap vmap, AttnSharedArgs a,
                                                                   int box) {
     constexpr int NB = D / 64, NS = tc_stages(D), kTile = NB * kTcBlock;
-    constexpr bool bf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+    constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
     extern __shared__ unsigned char raw[];
     unsigned char *sq = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    unsigned char *sk = sq + kTile, *sv = sk + NS * kTile;
-    __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], q_full, s_full[2], p_full[2], pv_done[2], drained;
+    unsigned char *sk = sq + NB * kTcBlock, *sv = sk + NS * kTile;
+    __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], q_full, s_full[2], p_full[4], pv_done[4], drained[2];
     __shared__ uint32_t slot_word;
     __shared__ int failed, bad_page;
     __shared__ float m1[128], l1[128];
@@ -520,9 +570,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
         return;
     }
     if (tid == 0) {
-        for (int i = 0; i < NS; ++i) mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_full + i, 1), mbar_init(v_empty + i, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(s_full + i, 1), mbar_init(p_full + i, 128), mbar_init(pv_done + i, 1);
-        mbar_init(&q_full, 256), mbar_init(&drained, 1);
+        for (int i = 0; i < NS; ++i) mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_full + i, 1), mbar_init(v_empty + i, 2);
+        for (int i = 0; i < 4; ++i) mbar_init(p_full + i, 4), mbar_init(pv_done + i, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(s_full + i, 1), mbar_init(drained + i, 1);
+        mbar_init(&q_full, 256);
         fence_mbar_init();
         failed = bad_page = 0;
     }
@@ -530,83 +581,90 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = slot_word;  // S of the warpgroups at columns 0 and 128 (P over them), O at 256 and 256 + D
-    int issued = 0;
-    if (warp == 8) {
-        // lane b brings box b of each tile
-        for (int i = 0; i < n; ++i) {
-            const int st = i % NS, key = (t0 + i) * kTcKeys, valid = min(kTcKeys, len - key), boxes = (valid + box - 1) / box;
-            int y = 0;
-            if (lane < boxes) {
-                const int k0 = key + lane * box, j = k0 / p.page_tokens;
-                int page = __ldg(table + j);
+    // S of tile i at columns 128 (i % 2), a half for each warpgroup, O of warpgroup w at 256 + w D;
+    // p_full and pv_done: of warpgroup w and tile i at 2 (i % 2) + w
+    const uint32_t tmem = slot_word;
+    if (warp >= 8) {
+        // every warp of these runs as one (its descriptors stay uniform); one lane issues
+        bool ok = true;
+        if (warp == 8 || warp == 11) {
+            // warp 8 brings the keys, warp 11 the values, lane b box b of each tile
+            const CUtensorMap *map = warp == 8 ? &kmap : &vmap;
+            uint64_t *full = warp == 8 ? k_full : v_full, *empty = warp == 8 ? k_empty : v_empty;
+            unsigned char *ring = warp == 8 ? sk : sv;
+            int key = t0 * kTcKeys + lane * box, issued = 0;
+            auto page_of = [&]() { return lane * box < kTcKeys && key < len ? __ldg(table + key / p.page_tokens) : 0; };
+            int page = page_of();
+            for (int i = 0; i < n; ++i) {
+                const int st = i % NS, boxes = (min(kTcKeys, len - (t0 + i) * kTcKeys) + box - 1) / box;
                 if (page < 0 || page >= p.n_pages) bad_page = 1, page = 0;
-                y = (page * p.n_kv_head + head) * p.page_tokens + k0 - j * p.page_tokens;
-            }
-            bool ok = true;
-            for (int kv = 0; kv < 2 && ok; ++kv) {
-                uint64_t *full = (kv ? v_full : k_full) + st, *empty = (kv ? v_empty : k_empty) + st;
-                ok = i < NS || wait_phase(empty, (i / NS - 1) & 1, &failed);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                if (lane == 0) mbar_expect_tx(full, boxes * box * 128 * NB);
+                const int y = (page * p.n_kv_head + head) * p.page_tokens + key % p.page_tokens;
+                key += kTcKeys;
+                page = page_of();  // for the next tile
+                if (!__all_sync(0xffffffffu, i < NS || wait_phase(empty + st, (i / NS - 1) & 1, &failed))) break;
+                if (lane == 0) mbar_expect_tx(full + st, boxes * box * 128 * NB);
                 __syncwarp();
                 if (lane < boxes)
                     for (int b = 0; b < NB; ++b)
-                        tma_load_2d((kv ? sv : sk) + st * kTile + b * kTcBlock + lane * box * 128, kv ? &vmap : &kmap, 64 * b, y, full);
+                        tma_load_2d(ring + st * kTile + b * kTcBlock + lane * box * 128, map, 64 * b, y, full + st);
                 __syncwarp();
-                ++issued;  // K of tile 0, V of tile 0, K of tile 1, ...
+                issued = i + 1;
             }
-            if (!ok) break;
-        }
-        // after a wait that ran out: let the copies in flight land before the block's shared memory goes on
-        __syncwarp();
-        if (lane == 0 && *(volatile int *)&failed)
-            for (int x = max(0, issued - 2 * NS); x < issued; ++x) {
-                uint64_t *full = ((x & 1) ? v_full : k_full) + x / 2 % NS;
-                for (int it = 0; it < 1 << 20 && !mbar_test(full, (x / 2 / NS) & 1); ++it) {
-                }
-            }
-    } else if (warp == 9) {
-        if (lane == 0) {
-            constexpr uint32_t type = bf16 ? (1u << 7) | (1u << 10) : 0u;
-            constexpr uint32_t id_s = idesc_f16(128, kTcKeys) | type, id_o = idesc_f16(128, D) | type | (1u << 16);
-            auto scores = [&](int i) {
-                const int st = i % NS;
-                if (!wait_phase(k_full + st, (i / NS) & 1, &failed)) return false;
-                tc_fence_after();
-                const uint32_t q0 = smem_u32(sq), k0 = smem_u32(sk + st * kTile);
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k)
-                    umma_f16(tmem + 128 * (i & 1), sw128_desc(q0 + k / 4 * kTcBlock) + 2 * (k % 4),
-                             sw128_desc(k0 + k / 4 * kTcBlock) + 2 * (k % 4), id_s, k > 0);
-                umma_commit(s_full + (i & 1));
-                umma_commit(k_empty + st);
-                return true;
-            };
-            bool ok = wait_phase(&q_full, 0, &failed) && scores(0) && (n < 2 || scores(1));
+            // after a wait that ran out: let the copies in flight land before the block's shared memory goes on
+            if (lane == 0 && *(volatile int *)&failed) drain_ring(full, NS, issued);
+        } else if (warp == 9) {  // S = Q K^T
+            constexpr uint32_t id = idesc_f16(128, kTcKeys) | kType;
+            ok = __all_sync(0xffffffffu, wait_phase(&q_full, 0, &failed));
             for (int i = 0; i < n && ok; ++i) {
-                const int w = i & 1, st = i % NS;
-                ok = wait_phase(p_full + w, (i >> 1) & 1, &failed) && wait_phase(v_full + st, (i / NS) & 1, &failed);
+                const int st = i % NS, b = i & 1;
+                ok = wait_phase(k_full + st, (i / NS) & 1, &failed);
+                if (i >= 2)  // both halves of P of tile i - 2 have been read
+                    ok = ok && wait_phase(pv_done + 2 * b, ((i >> 1) - 1) & 1, &failed) &&
+                         wait_phase(pv_done + 2 * b + 1, ((i >> 1) - 1) & 1, &failed);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t v0 = smem_u32(sv + st * kTile);
+                const uint32_t q0 = smem_u32(sq), k0 = smem_u32(sk + st * kTile);
+                if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < kTcKeys / 16; ++k)
-                    umma_f16_ta(tmem + 256 + w * D, tmem + 128 * w + 8 * k, sw128_desc_mn(v0 + 2048 * k, kTcBlock), id_o, i > 1 || k > 0);
-                umma_commit(pv_done + w);
-                umma_commit(v_empty + st);
-                // S of tile i + 2 goes where P of tile i is
-                if (i + 2 < n) ok = wait_phase(pv_done + w, (i >> 1) & 1, &failed) && scores(i + 2);
+                    for (int k = 0; k < D / 16; ++k)
+                        umma_f16(tmem + 128 * b, sw128_desc(q0 + k / 4 * kTcBlock) + 2 * (k % 4),
+                                 sw128_desc(k0 + k / 4 * kTcBlock) + 2 * (k % 4), id, k > 0);
+                    umma_commit(s_full + b);
+                    umma_commit(k_empty + st);
+                }
+                __syncwarp();
             }
-            if (!ok) {  // nothing may be in flight when the tensor memory is given back
-                umma_commit(&drained);
-                wait_phase(&drained, 0, &failed);
+        } else {  // O += P V, the two halves of a tile in turn
+            constexpr uint32_t id = idesc_f16(128, D) | kType | (1u << 16);
+            for (int i = 0; i < 2 * n && ok; ++i) {
+                const int t = i >> 1, w = i & 1, st = t % NS, bi = 2 * (t & 1) + w;
+                ok = wait_phase(v_full + st, (t / NS) & 1, &failed) && wait_phase(p_full + bi, (t >> 1) & 1, &failed);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t v0 = smem_u32(sv + st * kTile) + w * 64 * 128;
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_f16_ta(tmem + 256 + w * D, tmem + 64 * bi + 8 * k, sw128_desc_mn(v0 + 2048 * k, kTcBlock), id,
+                                    t > 0 || k > 0);
+                    umma_commit(pv_done + bi);
+                    umma_commit(v_empty + st);
+                }
+                __syncwarp();
+            }
+        }
+        if (warp == 9 || warp == 10) {
+            __syncwarp();
+            if (*(volatile int *)&failed) {  // nothing may be in flight when the tensor memory is given back
+                if (elect_one()) umma_commit(drained + warp - 9);
+                wait_phase(drained + warp - 9, 0, &failed);
             }
         }
     } else {
         const int w = warp >> 2, row = tid & 127;
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_at = tmem + lanes + 128 * w, o_at = tmem + lanes + 256 + w * D;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21, o_at = tmem + lanes + 256 + w * D;
         // the query tile, rows behind the group's last as zeros: warpgroup w lays out every other 16-byte unit
 #pragma unroll
         for (int u = w; u < D / 8; u += 2) {
@@ -615,29 +673,35 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
         }
         fence_proxy_async();
         mbar_arrive(&q_full);
+        const uint64_t scale2 = pair(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
         float m = 0.f, l = 0.f;
         bool ok = true;
-        for (int i = w; i < n; i += 2) {
-            const int valid = min(kTcKeys, len - (t0 + i) * kTcKeys);
-            ok = __all_sync(0xffffffffu, wait_phase(s_full + w, (i >> 1) & 1, &failed));
+        for (int i = 0; i < n; ++i) {
+            const int valid = max(0, min(64, len - (t0 + i) * kTcKeys - 64 * w)), bi = 2 * (i & 1) + w;  // of this half
+            const uint32_t s_at = tmem + lanes + 64 * bi;
+            ok = __all_sync(0xffffffffu, wait_phase(s_full + (i & 1), (i >> 1) & 1, &failed));
             if (!ok) break;
             tc_fence_after();
-            uint32_t s[128];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) tmem_load32(s_at + 32 * x, s + 32 * x);
+            uint32_t s[64];
+            tmem_load32(s_at, s);
+            tmem_load32(s_at + 32, s + 32);
             tmem_wait_ld();
-            if (valid < kTcKeys)
+            if (valid < 64)
 #pragma unroll
-                for (int x = 0; x < 128; ++x)
+                for (int x = 0; x < 64; ++x)
                     if (x >= valid) s[x] = __float_as_uint(kNone);
             float mx[4] = {kNone, kNone, kNone, kNone};
 #pragma unroll
-            for (int x = 0; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
-            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
-            if (top == kNone) top = i == w ? 0.f : m;
-            if (i == w) {
+            for (int x = 0; x < 64; x += 2)
+                mx[x / 2 & 3] = max3(mx[x / 2 & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
+            float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * a.scale_log2;
+            if (top == kNone) top = i == 0 ? 0.f : m;
+            if (i == 0) {
                 m = top;
             } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                ok = __all_sync(0xffffffffu, wait_phase(pv_done + (bi ^ 2), ((i - 1) >> 1) & 1, &failed));
+                if (!ok) break;
+                tc_fence_after();
                 const float f = top > m ? ex2(m - top) : 1.f;
                 m = fmaxf(m, top);
                 l *= f;
@@ -651,41 +715,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
                     tmem_store32(o_at + x, o);
                 }
             }
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint64_t base2 = pair(__float_as_uint(-m), __float_as_uint(-m));
+            uint64_t sum[2] = {0, 0};
 #pragma unroll
-            for (int x = 0; x < 128; x += 2) {
-                const float e0 = ex2(fmaf(__uint_as_float(s[x]), a.scale_log2, -m));
-                const float e1 = ex2(fmaf(__uint_as_float(s[x + 1]), a.scale_log2, -m));
-                sum[x / 2 & 3] += e0 + e1;
-                s[x / 2] = pack2<T>(e0, e1);
-                if (x == 62) tmem_store32(s_at, s);
+            for (int x = 0; x < 64; x += 2) {
+                uint64_t e = fma2(pair(s[x], s[x + 1]), scale2, base2);
+                if (kPoly * (x / 2 + 1) / 32 != kPoly * (x / 2) / 32)
+                    e = exp2_poly(e);
+                else
+                    e = pair(__float_as_uint(ex2(__uint_as_float((uint32_t)e))), __float_as_uint(ex2(__uint_as_float((uint32_t)(e >> 32)))));
+                sum[x / 2 & 1] = add2(sum[x / 2 & 1], e);
+                s[x / 2] = pack2<T>(__uint_as_float((uint32_t)e), __uint_as_float((uint32_t)(e >> 32)));
             }
-            tmem_store32(s_at + 32, s + 32);
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_wait_st();
-            if (valid < kTcKeys) {  // behind the last key there may be anything: 0 x NaN is none
+            tmem_store32(s_at, s);
+            sum[0] = add2(sum[0], sum[1]);
+            l += __uint_as_float((uint32_t)sum[0]) + __uint_as_float((uint32_t)(sum[0] >> 32));
+            if (valid < 64) {  // behind the last key there may be anything: 0 x NaN is none
                 const int st = i % NS;
                 ok = __all_sync(0xffffffffu, wait_phase(v_full + st, (i / NS) & 1, &failed));
                 if (!ok) break;
-                for (int x = row; x < (kTcKeys - valid) * 8 * NB; x += 128) {
-                    const int at = valid + x / (8 * NB), u = x % (8 * NB);
+                for (int x = row; x < (64 - valid) * 8 * NB; x += 128) {
+                    const int at = 64 * w + valid + x / (8 * NB), u = x % (8 * NB);
                     *reinterpret_cast<uint4 *>(sv + st * kTile + u / 8 * kTcBlock + at * 128 + u % 8 * 16) = make_uint4(0, 0, 0, 0);
                 }
                 fence_proxy_async();
             }
+            tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(p_full + w);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + bi);
         }
         // both warpgroups' sums, joined by the first
-        // (its own first: the other's last product but one is done then, so that one parity tells its last two apart)
-        for (int x = 0; x < 2 && ok; ++x) {
-            const int b = w ^ x, mine = b ? n / 2 : (n + 1) / 2;
-            ok = mine == 0 || wait_phase(pv_done + b, (mine - 1) & 1, &failed);
-        }
+        ok = ok && wait_phase(pv_done + 2 * ((n - 1) & 1) + w, ((n - 1) >> 1) & 1, &failed);
         __syncwarp();
         tc_fence_after();
-        float *other = reinterpret_cast<float *>(sk);  // [D][128], over the rings
-        if (w == 1 && n > 1) {
+        float *other = reinterpret_cast<float *>(sk);  // [D][128], over the keys: every S is there
+        if (w == 1) {
 #pragma unroll 1
             for (int x = 0; x < D; x += 32) {
                 uint32_t o[32];
@@ -699,13 +764,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (w == 0) {
             const bool lost = *(volatile int *)&failed || *(volatile int *)&bad_page;
-            float f0 = 1.f, f1 = 0.f;
-            if (n > 1) {
-                const float top = fmaxf(m, m1[row]);
-                f0 = ex2(m - top), f1 = ex2(m1[row] - top);
-                l = l * f0 + l1[row] * f1;
-                m = top;
-            }
+            // (a warpgroup without a key has m = 0, l = 0 and O = 0)
+            const float top = l1[row] == 0.f ? m : fmaxf(m, m1[row]), f0 = ex2(m - top), f1 = l1[row] == 0.f ? 0.f : ex2(m1[row] - top);
+            l = l * f0 + l1[row] * f1;
+            m = top;
             if (qr) a.part_ml[part * 2] = lost ? NAN : m, a.part_ml[part * 2 + 1] = lost ? NAN : l;
             if (tid == 0 && *(volatile int *)&bad_page) atomicOr(p.status, W4J_PAGES_BAD_PAGE);
 #pragma unroll 1
@@ -713,10 +775,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
                 uint32_t o[32];
                 tmem_load32(o_at + x, o);
                 tmem_wait_ld();
-                if (n > 1)
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        o[e] = __float_as_uint(__uint_as_float(o[e]) * f0 + other[(x + e) * 128 + row] * f1);
+                for (int e = 0; e < 32; ++e)
+                    o[e] = __float_as_uint(__uint_as_float(o[e]) * f0 + other[(x + e) * 128 + row] * f1);
                 if (qr)
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
@@ -824,7 +885,7 @@ void attn_shared_plan(AttnSharedArgs &a) {
         if (tc) {
             a.tc_tiles = (unsigned)(a.n_seq * c / 128 + a.n_group);
             // fewest rounds of blocks over the SMs times key tiles of a block (and about four more to start and join)
-            const long long blocks = (avg + 127) / 128 * a.n_group * p.n_kv_head, tiles = (a.max_shared + kTcKeys - 1) / kTcKeys;
+            const long long blocks = (avg + 127) / 128 * a.n_group * p.n_kv_head, tiles = (a.max_shared + 127) / 128;
             long long best = 0;
             for (int n = 1; n <= tiles && n <= 64; ++n) {
                 const long long cost = (blocks * n + 147) / 148 * ((tiles + n - 1) / n + 4);
