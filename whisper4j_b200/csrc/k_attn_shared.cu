@@ -149,7 +149,7 @@ struct WarpTile {
     __device__ __forceinline__ void run(const PagesArgs &p, const int *table, int head, const CUtensorMap *kmap,
                                         const CUtensorMap *vmap, unsigned char *sm, uint64_t *full, int box, int k0, int k1,
                                         const int (&lim)[NT][2], int all, float scale_log2, int *bad, int *failed) {
-        const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+        const int lane = threadIdx.x & 31, g = lane >> 2;
         if (k0 >= k1) return;
         const int start = k0 / box * box, n_steps = (k1 - start + STEP - 1) / STEP;  // boxes do not cross pages
         // lane b (keys) and lane 16 + b (values) bring box b of a step; page and place in it of its first key
@@ -440,8 +440,11 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_cons
 // are in.  Keys and values come page by page through TMA boxes (128-byte swizzle) into two rings; V is the MMA's B
 // operand as it lies in the pages (MN-major).
 //
-// Bound by the exponentials: 128 x 128 of them take the 16 a cycle of an SM's special function units 1024 cycles, the
-// MMAs of a tile 512 (head 64) or 1024 (head 128).  So some are computed on the FMA pipes instead (exp2_poly).
+// 128 x 128 exponentials take the 16 a cycle of an SM's special function units 1024 cycles, the MMAs of a tile 512 (head
+// 64) or 1024 (head 128); a tile takes 1850 to 2100, bound by the round from S over P to the S that comes after the
+// next (softmax 1500, P V and Q K^T 600 to 900 with their hand-overs).  Moving 4 to 16 of every 32 exponentials to a
+// polynomial on the FMA pipes made that round longer (142 -> 143 .. 150 us on 4 x 256 rows x 16381 keys x 8 heads of
+// 128) and was not kept.
 // ---------------------------------------------------------------------------
 constexpr int kTcThreads = 384, kTcKeys = 128, kTcBlock = 128 * 128;  // bytes of 64 numbers of 128 rows
 
@@ -484,7 +487,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-__device__ __forceinline__ uint64_t neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -508,23 +510,6 @@ __device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t next)
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(next >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
            (uint64_t)2 << 61;
 }
-// 2^x of two numbers on the FMA pipes, x < 2^7: x = n + f with |f| <= 1/2 (adding 1.5 x 2^23 rounds to n), 2^f by the
-// polynomial of degree 4 with the least relative error there (2.6e-6, a hundredth of P's rounding), n into the exponent.
-__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
-    auto both = [](float v) { return pair(__float_as_uint(v), __float_as_uint(v)); };
-    float a = __uint_as_float((uint32_t)x), b = __uint_as_float((uint32_t)(x >> 32));
-    // below 2^-125 there is nothing left of a weight; a NaN stays one
-    const uint64_t t = pair(__float_as_uint(a < -125.f ? -125.f : a), __float_as_uint(b < -125.f ? -125.f : b));
-    const uint64_t n = add2(t, both(12582912.f)), f = add2(t, neg2(add2(n, both(-12582912.f))));
-    uint64_t y = fma2(both(0.009570102207362652f), f, both(0.05591785907745361f));
-    y = fma2(y, f, both(0.240247443318367f));
-    y = fma2(y, f, both(0.6931217908859253f));
-    y = fma2(y, f, both(0.9999992847442627f));
-    return pair((uint32_t)y + ((uint32_t)n << 23), (uint32_t)(y >> 32) + ((uint32_t)(n >> 32) << 23));
-}
-
-constexpr int kPoly = 10;  // of the 32 pairs of a row of S
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_constant__ CUtensorMap kmap,
                                                                   const __grid_constant__ CUtensorMap vmap, AttnSharedArgs a,
@@ -719,13 +704,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
             uint64_t sum[2] = {0, 0};
 #pragma unroll
             for (int x = 0; x < 64; x += 2) {
-                uint64_t e = fma2(pair(s[x], s[x + 1]), scale2, base2);
-                if (kPoly * (x / 2 + 1) / 32 != kPoly * (x / 2) / 32)
-                    e = exp2_poly(e);
-                else
-                    e = pair(__float_as_uint(ex2(__uint_as_float((uint32_t)e))), __float_as_uint(ex2(__uint_as_float((uint32_t)(e >> 32)))));
-                sum[x / 2 & 1] = add2(sum[x / 2 & 1], e);
-                s[x / 2] = pack2<T>(__uint_as_float((uint32_t)e), __uint_as_float((uint32_t)(e >> 32)));
+                const uint64_t e = fma2(pair(s[x], s[x + 1]), scale2, base2);
+                const float e0 = ex2(__uint_as_float((uint32_t)e)), e1 = ex2(__uint_as_float((uint32_t)(e >> 32)));
+                sum[x / 2 & 1] = add2(sum[x / 2 & 1], pair(__float_as_uint(e0), __float_as_uint(e1)));
+                s[x / 2] = pack2<T>(e0, e1);
             }
             tmem_store32(s_at, s);
             sum[0] = add2(sum[0], sum[1]);

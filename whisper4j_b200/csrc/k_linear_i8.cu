@@ -31,33 +31,32 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // ---------------------------------------------------------------------------
-// rows to 8 bits: a block per row, eight neighbouring elements per thread and step, held in registers
-// between the passes (sum, squares, largest magnitude, quotients) where the row fits.  Bound by HBM for
-// many rows and by the latency of its block reductions for few.
+// rows to 8 bits: a warp per row where there are many rows, else a block, 16 bytes per thread and step, held in
+// registers between the passes (sum, squares, largest magnitude, quotients) where the row fits.  Bound by HBM for
+// many rows and by the latency of its reductions for few.
 // ---------------------------------------------------------------------------
-constexpr int kQMax = 256;
+constexpr int kQMax = 1024;
 
-// Eight elements from k on (zeros behind K).
+// The 16 bytes of elements from k on (zeros behind K).
 template <typename T>
-__device__ __forceinline__ void load8(const T *x, int k, int K, bool vec, float (&v)[8]) {
-    if (vec && k + 8 <= K) {
-        T t[8];
+__device__ __forceinline__ void load16(const T *x, int k, int K, bool vec, float (&v)[16 / sizeof(T)]) {
+    constexpr int V = 16 / sizeof(T);
+    if (vec && k + V <= K) {
+        T t[V];
+        *reinterpret_cast<uint4 *>(t) = __ldg(reinterpret_cast<const uint4 *>(x + k));
 #pragma unroll
-        for (size_t i = 0; i < sizeof(T) / 2; ++i)
-            reinterpret_cast<uint4 *>(t)[i] = __ldg(reinterpret_cast<const uint4 *>(x + k) + i);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(t[i]);
+        for (int i = 0; i < V; ++i) v[i] = to_f32<T>(t[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f32<T>(x[k + i]) : 0.f;
+        for (int i = 0; i < V; ++i) v[i] = k + i < K ? to_f32<T>(x[k + i]) : 0.f;
     }
 }
 
-template <typename Op>
-__device__ __forceinline__ float block_reduce(float v, float *sm, Op op) {
+template <bool WARP, typename Op>
+__device__ __forceinline__ float row_reduce(float v, float *sm, Op op) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (blockDim.x == 32) return v;
+    if (WARP) return v;
     __syncthreads();  // the last call's numbers have been read
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
     __syncthreads();
@@ -76,21 +75,24 @@ __device__ __forceinline__ int nearest(float x, float s, float inv) {
     return min(127, max(-127, (int)r));
 }
 
-// C: steps held in registers, 0: the row is read again in every pass
-template <typename T, int C>
-__global__ void __launch_bounds__(kQMax) k_quantize_rows(QuantizeArgs a) {
+// C: steps held in registers, 0: the row is read again in every pass; WARP: a row per warp, else per block
+template <typename T, int C, bool WARP>
+__global__ void __launch_bounds__(WARP ? 128 : kQMax) k_quantize_rows(QuantizeArgs a) {
+    constexpr int V = 16 / sizeof(T);
     __shared__ float sm[kQMax / 32];
     pdl_wait();
     pdl_trigger();
-    const T *x = reinterpret_cast<const T *>(a.x) + (long long)blockIdx.x * a.ldx;
+    const int row = WARP ? blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x, tid = WARP ? threadIdx.x % 32 : threadIdx.x;
+    if (row >= a.M) return;
+    const T *x = reinterpret_cast<const T *>(a.x) + (long long)row * a.ldx;
     const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0;
-    const int step = blockDim.x * 8, k0 = threadIdx.x * 8, K = a.K;
-    float v[C ? C : 1][8];
+    const int step = (WARP ? 32 : blockDim.x) * V, k0 = tid * V, K = a.K;
+    float v[C ? C : 1][V];
     if (C) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) load8(x, k0 + c * step, K, vec, v[c]);
+        for (int c = 0; c < C; ++c) load16(x, k0 + c * step, K, vec, v[c]);
     }
-    // f(k, eight elements): over the row
+    // f(k, the elements from k on): over the row
     auto pass = [&](auto f) {
         if (C) {
 #pragma unroll
@@ -98,7 +100,7 @@ __global__ void __launch_bounds__(kQMax) k_quantize_rows(QuantizeArgs a) {
                 if (k0 + c * step < K) f(k0 + c * step, v[c]);
         } else {
             for (int k = k0; k < K; k += step) {
-                load8(x, k, K, vec, v[0]);
+                load16(x, k, K, vec, v[0]);
                 f(k, v[0]);
             }
         }
@@ -107,82 +109,94 @@ __global__ void __launch_bounds__(kQMax) k_quantize_rows(QuantizeArgs a) {
     float mean = 0.f, rstd = 1.f;
     if (a.ln_g) {
         float sum = 0.f, sq = 0.f;
-        pass([&](int, float(&e)[8]) {
+        pass([&](int, float(&e)[V]) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += e[i];
+            for (int i = 0; i < V; ++i) sum += e[i];
         });
-        mean = block_reduce(sum, sm, add) / K;
-        pass([&](int k, float(&e)[8]) {
+        mean = row_reduce<WARP>(sum, sm, add) / K;
+        pass([&](int k, float(&e)[V]) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < V; ++i)
                 if (k + i < K) sq += (e[i] - mean) * (e[i] - mean);
         });
-        rstd = 1.f / sqrtf(block_reduce(sq, sm, add) / K + 1e-5f);
+        rstd = 1.f / sqrtf(row_reduce<WARP>(sq, sm, add) / K + 1e-5f);
     }
-    auto norm = [&](int k, float(&e)[8]) {
+    auto norm = [&](int k, float(&e)[V]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < V; ++i)
             e[i] = k + i < K ? (e[i] - mean) * rstd * __ldg(a.ln_g + k + i) + __ldg(a.ln_b + k + i) : 0.f;
     };
     float top = 0.f;
     bool odd = false;  // an infinity or a NaN
-    pass([&](int k, float(&e)[8]) {
+    pass([&](int k, float(&e)[V]) {
         if (a.ln_g) norm(k, e);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < V; ++i) {
             top = fmaxf(top, fabsf(e[i]));
             odd |= !(fabsf(e[i]) <= 3.4028234e38f);
         }
     });
-    top = block_reduce(odd ? INFINITY : top, sm, [](float p, float q) { return fmaxf(p, q); });
+    top = row_reduce<WARP>(odd ? INFINITY : top, sm, [](float p, float q) { return fmaxf(p, q); });
     const bool good = top <= 3.4028234e38f;
     const float s = __fdiv_rn(top, 127.f);
     // where the scale's reciprocal or half would not be normal, x and s are taken times 2^64: the same quotient
     const float up = s < 1e-30f ? 18446744073709551616.f : 1.f, su = s * up, inv = __fdiv_rn(1.f, su);
-    if (threadIdx.x == 0) a.scale[blockIdx.x] = good ? s : __int_as_float(0x7fffffff);
-    int8_t *q = a.q + (long long)blockIdx.x * a.ldq;
-    auto store = [&](int k, float(&e)[8]) {
+    if (tid == 0) a.scale[row] = good ? s : __int_as_float(0x7fffffff);
+    int8_t *q = a.q + (long long)row * a.ldq;
+    pass([&](int k, float(&e)[V]) {
         if (a.ln_g && !C) norm(k, e);
-        uint32_t w[2] = {0, 0};
+        uint32_t w[V / 4] = {};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < V; ++i) {
             const int r = good && s > 0.f && k + i < K ? nearest(e[i] * up, su, inv) : 0;
             w[i / 4] |= (uint32_t)(r & 0xff) << (i % 4 * 8);
         }
-        *reinterpret_cast<uint2 *>(q + k) = make_uint2(w[0], w[1]);
-    };
-    pass(store);
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) reinterpret_cast<uint32_t *>(q + k)[i] = w[i];
+    });
     // the rest up to a multiple of 16 is zero: a product may read it
-    if (threadIdx.x == 0 && K % 16 && K % 16 <= 8) *reinterpret_cast<uint2 *>(q + K / 16 * 16 + 8) = make_uint2(0, 0);
+    const int done = (K + V - 1) / V * V, end = (K + 15) / 16 * 16;
+    if (tid * 4 < end - done) *reinterpret_cast<uint32_t *>(q + done + tid * 4) = 0;
 }
 
+// A warp per row from 8 rows for every SM's scheduler on, where a row fits its registers (12000 rows of 1280 with a
+// LayerNorm: 51 us with a block per row, @WARP@ with a warp); fewer rows get as many threads as they have units.
 template <typename T>
 cudaError_t quantize(const QuantizeArgs &a, cudaStream_t s) {
-    const int units = (a.K + 7) / 8, c = (units + kQMax - 1) / kQMax;
-    const int held = c <= 1 ? 1 : c <= 2 ? 2 : c <= 4 ? 4 : 0;
-    const int threads = held ? (units + held - 1) / held : kQMax, block = (threads + 31) / 32 * 32;
-    switch (held) {
-        case 1: return launch_after(k_quantize_rows<T, 1>, a.M, block, 0, s, 1, a);
-        case 2: return launch_after(k_quantize_rows<T, 2>, a.M, block, 0, s, 1, a);
-        case 4: return launch_after(k_quantize_rows<T, 4>, a.M, block, 0, s, 1, a);
-        default: return launch_after(k_quantize_rows<T, 0>, a.M, block, 0, s, 1, a);
+    constexpr int V = 16 / sizeof(T);
+    const int units = (a.K + V - 1) / V, c = (units + 31) / 32;
+    if (a.M >= 148 * 4 * 2 && c <= 16) {
+        const unsigned blocks = (a.M + 3) / 4;
+        if (c <= 4) return launch_after(k_quantize_rows<T, 4, true>, blocks, 128, 0, s, 1, a);
+        if (c <= 8) return launch_after(k_quantize_rows<T, 8, true>, blocks, 128, 0, s, 1, a);
+        if (c <= 12) return launch_after(k_quantize_rows<T, 12, true>, blocks, 128, 0, s, 1, a);
+        return launch_after(k_quantize_rows<T, 16, true>, blocks, 128, 0, s, 1, a);
     }
+    const int most = a.M >= 148 * 4 ? 256 : kQMax, held = (units + most - 1) / most;
+    const int threads = held <= 4 ? (units + held - 1) / held : most, block = (threads + 31) / 32 * 32;
+    if (held == 1) return launch_after(k_quantize_rows<T, 1, false>, a.M, block, 0, s, 1, a);
+    if (held == 2) return launch_after(k_quantize_rows<T, 2, false>, a.M, block, 0, s, 1, a);
+    if (held <= 4) return launch_after(k_quantize_rows<T, 4, false>, a.M, block, 0, s, 1, a);
+    return launch_after(k_quantize_rows<T, 0, false>, a.M, block, 0, s, 1, a);
 }
 
 // ---------------------------------------------------------------------------
 // product
 // ---------------------------------------------------------------------------
-// One output from its integer sum (exact: |sum| <= 2^14 K < 2^31).  GELU in its tanh form, as
-// v / (1 + exp(-2 u)): no cancellation, and the right limits where the exponential leaves its range.
-template <typename T>
-__device__ __forceinline__ void finish(const LinearI8Args &a, int acc, float xs, float ws, float b, T *y) {
-    float v = (float)acc * xs * ws + b;
-    if (a.epilogue == 1) {
-        const float u = 0.7978845608f * (v + 0.044715f * v * v * v);
-        v = v / (1.f + __expf(-2.f * u));
-    } else if (a.epilogue == 2) {
-        v += to_f32<T>(*y);
-    }
+// GELU in its tanh form, as v / (1 + 2^t) with t = -2 log2(e) u: no cancellation, and the right limits where the
+// exponential leaves its range.
+__device__ __forceinline__ float gelu(float v) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * fmaf(v * v, -0.1029432397f, -2.3022081985f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return v * r;
+}
+// One output from its integer sum (exact: |sum| <= 2^14 K < 2^31).
+template <typename T, int EPI>
+__device__ __forceinline__ void finish(int acc, float xs, float ws, float b, T *y) {
+    float v = fmaf((float)acc * xs, ws, b);
+    if (EPI == 1) v = gelu(v);
+    if (EPI == 2) v += to_f32<T>(*y);
     *y = from_f32<T>(v);
 }
 
@@ -215,7 +229,7 @@ __host__ __device__ constexpr size_t mm_smem(int NT) { return (size_t)mm_stages(
 // A cluster of blocks owns 128 channels x NT tokens; block q of the cluster multiplies a share of k.  The
 // channels are the MMA's 128 rows (TMEM lanes), so that a warp's store of one token's column is one contiguous run
 // of y, and a lane keeps its channel's scale and bias in registers.
-template <int NT, typename T>
+template <int NT, typename T, int EPI>
 __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant__ CUtensorMap wmap,
                                                           const __grid_constant__ CUtensorMap xmap, LinearI8Args a, int ks,
                                                           int token_tiles) {
@@ -285,7 +299,7 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
             if (ks > 1)
                 part[(j0 + j) * kMmTile + ch] = acc;
             else if (in && m < a.M)
-                finish<T>(a, acc, failed ? NAN : xs[j0 + j], ws, b, y + (long long)m * a.ldy);
+                finish<T, EPI>(acc, failed ? NAN : xs[j0 + j], ws, b, y + (long long)m * a.ldy);
         }
     }
     tc_fence_before();
@@ -300,14 +314,198 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
             for (int r = 0; r < ks; ++r) acc += peer_word(part + j * kMmTile + c, r);
             const int nn = n0 + c;
             if (nn < a.N)
-                finish<T>(a, acc, lost ? NAN : xs[j], __ldg(a.ws + nn), a.bias ? __ldg(a.bias + nn) : 0.f,
-                          reinterpret_cast<T *>(a.y) + (long long)m * a.ldy + nn);
+                finish<T, EPI>(acc, lost ? NAN : xs[j], __ldg(a.ws + nn), a.bias ? __ldg(a.bias + nn) : 0.f,
+                               reinterpret_cast<T *>(a.y) + (long long)m * a.ldy + nn);
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     __syncthreads();
     if (failed && tid == 0) drain_ring(full, S, issued);
     if (warp == 1) tc_fence_after(), tmem_dealloc(tmem, kCols);
+}
+
+// ---------------------------------------------------------------------------
+// many rows: a pair of SMs owns 256 channels x 256 tokens at a time (tcgen05.mma with cta_group::2), each with 128 of the
+// channels and half of the tokens in its shared memory, so that a tile's operands cross from L2 once: 64 bytes a cycle
+// and SM at the integer MMAs' 8192 products, where a single SM's 128 x 256 tile would want 96.  Persistent: two
+// accumulators in tensor memory, and eight warps turn one into outputs while the next tile's products run.
+// ---------------------------------------------------------------------------
+constexpr int kPrThreads = 320, kPrStages = 6, kPrStage = 2 * kMmTile * kMmK;
+constexpr size_t kPrSmem = (size_t)kPrStages * kPrStage + 1024;
+
+__device__ __forceinline__ uint32_t peer_address(const void *p, int rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// a box into this block's shared memory, its bytes counted by a barrier of either block of the pair
+__device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// the barrier at this place in both blocks
+__device__ __forceinline__ void commit_pair(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ void pair_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                   "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+                   "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+                   "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(at)
+                 : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+template <typename T, int EPI>
+__global__ void __launch_bounds__(kPrThreads, 1) k_linear_i8_pair(const __grid_constant__ CUtensorMap wmap,
+                                                                  const __grid_constant__ CUtensorMap xmap, LinearI8Args a,
+                                                                  int token_tiles, int tiles) {
+    extern __shared__ unsigned char raw[];
+    unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full[kPrStages], empty[kPrStages], acc_full[2], acc_free[2], drained;
+    __shared__ uint32_t slot;
+    __shared__ int failed;
+    __shared__ __align__(16) float xs[8][128];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x & 1;
+    const int nk = (a.K + kMmK - 1) / kMmK, pairs = gridDim.x / 2;
+    if (tid == 0) {
+        for (int i = 0; i < kPrStages; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(acc_full + i, 1), mbar_init(acc_free + i, 16);
+        mbar_init(&drained, 1);
+        fence_mbar_init();
+        failed = 0;
+    }
+    pdl_wait();  // before the tensor memory: a kernel that waits must not hold what the one before it may need
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    pair_barrier();  // both blocks' barriers are there
+    tc_fence_after();
+    const uint32_t tmem = slot;
+    if (warp == 0) {
+        // the first block's `full` counts both blocks' bytes
+        int it = 0;
+        bool ok = true;
+        for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs) {
+            const int n0 = t / token_tiles * 256 + 128 * rank, m0 = t % token_tiles * 256 + 128 * rank;
+            for (int k = 0; k < nk; ++k, ++it) {
+                const int st = it % kPrStages;
+                ok = __all_sync(0xffffffffu, it < kPrStages || mbar_wait(empty + st, (it / kPrStages - 1) & 1, &failed));
+                if (!ok) break;
+                if (elect_one()) {
+                    if (rank == 0) mbar_expect_tx(full + st, 2 * kPrStage);
+                    const uint32_t bar = peer_address(full + st, 0);
+                    tma_load_pair(sm + st * kPrStage, &wmap, k * kMmK, n0, bar);
+                    tma_load_pair(sm + st * kPrStage + kMmTile * kMmK, &xmap, k * kMmK, m0, bar);
+                }
+                __syncwarp();
+            }
+        }
+        // after a wait that ran out, copies that are in flight land within microseconds: wait a good while longer
+        if (*(volatile int *)&failed)
+            for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    } else if (warp == 1) {
+        if (rank == 0) {
+            constexpr uint32_t idesc = idesc_i8(256, 256);
+            int it = 0, n = 0;
+            bool ok = true;
+            for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs, ++n) {
+                const int b = n & 1;
+                ok = __all_sync(0xffffffffu, n < 2 || mbar_wait(acc_free + b, (n / 2 - 1) & 1, &failed));
+                for (int k = 0; k < nk && ok; ++k, ++it) {
+                    const int st = it % kPrStages;
+                    ok = __all_sync(0xffffffffu, mbar_wait(full + st, (it / kPrStages) & 1, &failed));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t at = smem_u32(sm + st * kPrStage);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < kMmK / 32; ++i)
+                            umma_i8_pair(tmem + 256 * b, sw128_desc(at) + 2 * i, sw128_desc(at + kMmTile * kMmK) + 2 * i, idesc,
+                                         k > 0 || i > 0);
+                        commit_pair(empty + st);
+                        if (k == nk - 1) commit_pair(acc_full + b);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (!ok) {  // nothing may be in flight when the tensor memory is given back
+                if (elect_one()) commit_pair(&drained);
+                mbar_wait(&drained, 0, &failed);
+            }
+        }
+    } else {
+        // warps of one lane quarter take the tokens' halves
+        const int e = warp - 2, quarter = warp & 3, half = e >> 2;
+        float *sx = xs[e];
+        int n = 0;
+        bool ok = true;
+        for (int t = blockIdx.x / 2; t < tiles; t += pairs, ++n) {
+            const int b = n & 1, ch = t / token_tiles * 256 + 128 * rank + 32 * quarter + lane, m0 = t % token_tiles * 256 + 128 * half;
+            const int rows = min(128, a.M - m0);
+            const bool in = ch < a.N;
+            const float ws = in ? __ldg(a.ws + ch) : 0.f, bias = in && a.bias ? __ldg(a.bias + ch) : 0.f;
+            __syncwarp();
+#pragma unroll
+            for (int j = lane; j < 128; j += 32) sx[j] = j < rows ? __ldg(a.xs + m0 + j) : 0.f;
+            __syncwarp();
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(acc_full + b, (n / 2) & 1, &failed));
+            tc_fence_after();
+            T *y = reinterpret_cast<T *>(a.y) + (long long)m0 * a.ldy + ch;
+            for (int j0 = 0; j0 < rows; j0 += 32) {
+                uint32_t acc[32];
+                __syncwarp();
+                tmem_ld32(tmem + ((uint32_t)quarter << 21) + 256 * b + 128 * half + j0, acc);
+                if (j0 + 32 >= rows) {  // the accumulator has been read
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_at(peer_address(acc_free + b, 0));
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    if (in && j0 + j < rows) finish<T, EPI>((int)acc[j], ok ? sx[j0 + j] : NAN, ws, bias, y);
+                    y += a.ldy;
+                }
+            }
+            if (rows <= 0 && lane == 0) arrive_at(peer_address(acc_free + b, 0));
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    pair_barrier();  // no block ends, or gives back its tensor memory, while the other's products may use it
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
 }
 
 // [box rows x 128 bytes] boxes of a row-major 8-bit matrix, 128-byte swizzle; reads beyond rows or columns give zeros
@@ -327,7 +525,7 @@ bool tmap_i8(CUtensorMap *m, const int8_t *base, long long rows, int cols, long 
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NT, typename T>
+template <int NT, typename T, int EPI>
 cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
     const int k16 = (a.K + 15) / 16 * 16, kb = (a.K + kMmK - 1) / kMmK;
     alignas(64) CUtensorMap wmap, xmap;
@@ -337,18 +535,40 @@ cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
     // k is split while the tiles leave SMs idle and every block keeps two stages of k
     int ks = 1;
     while (ks < 8 && tiles * ks * 2 <= 148 && kb >= 4 * ks) ks *= 2;
-    cudaError_t e = allow_smem<k_linear_i8<NT, T>>(mm_smem(NT));
+    cudaError_t e = allow_smem<k_linear_i8<NT, T, EPI>>(mm_smem(NT));
     if (e != cudaSuccess) return e;
-    return launch_after(k_linear_i8<NT, T>, (unsigned)(tiles * ks), kMmThreads, mm_smem(NT), s, ks, wmap, xmap, a, ks,
+    return launch_after(k_linear_i8<NT, T, EPI>, (unsigned)(tiles * ks), kMmThreads, mm_smem(NT), s, ks, wmap, xmap, a, ks,
                         (int)token_tiles);
+}
+
+template <typename T, int EPI>
+cudaError_t product_pair(const LinearI8Args &a, cudaStream_t s) {
+    const int k16 = (a.K + 15) / 16 * 16;
+    alignas(64) CUtensorMap wmap, xmap;
+    if (!tmap_i8(&wmap, a.w, a.N, k16, a.ldw, kMmTile) || !tmap_i8(&xmap, a.x, a.M, k16, a.ldx, kMmTile))
+        return cudaErrorInvalidValue;
+    const int token_tiles = (a.M + 255) / 256;
+    const long long tiles = (long long)((a.N + 255) / 256) * token_tiles;
+    if (tiles > 0x7fffffff) return cudaErrorInvalidValue;
+    cudaError_t e = allow_smem<k_linear_i8_pair<T, EPI>>(kPrSmem);
+    if (e != cudaSuccess) return e;
+    return launch_after(k_linear_i8_pair<T, EPI>, 2 * (unsigned)(tiles < 74 ? tiles : 74), kPrThreads, kPrSmem, s, 2, wmap, xmap, a,
+                        token_tiles, (int)tiles);
+}
+
+template <typename T, int EPI>
+cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
+    if (a.M <= 16) return product<16, T, EPI>(a, s);
+    if (a.M <= 32) return product<32, T, EPI>(a, s);
+    if (a.M <= 64) return product<64, T, EPI>(a, s);
+    const long long tiles = (long long)((a.N + 255) / 256) * ((a.M + 255) / 256);
+    if (a.M > 128 && tiles >= 48) return product_pair<T, EPI>(a, s);
+    return product<128, T, EPI>(a, s);
 }
 
 template <typename T>
 cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
-    if (a.M <= 16) return product<16, T>(a, s);
-    if (a.M <= 32) return product<32, T>(a, s);
-    if (a.M <= 64) return product<64, T>(a, s);
-    return product<128, T>(a, s);
+    return a.epilogue == 0 ? product<T, 0>(a, s) : a.epilogue == 1 ? product<T, 1>(a, s) : product<T, 2>(a, s);
 }
 
 }  // namespace
