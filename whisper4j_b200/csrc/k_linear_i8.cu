@@ -52,8 +52,8 @@ __device__ __forceinline__ void load16(const T *x, int k, int K, bool vec, float
     }
 }
 
-template <bool WARP, typename Op>
-__device__ __forceinline__ float row_reduce(float v, float *sm, Op op) {
+template <bool WARP, typename U, typename Op>
+__device__ __forceinline__ U row_reduce(U v, U *sm, Op op) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
     if (WARP) return v;
@@ -73,6 +73,24 @@ __device__ __forceinline__ int nearest(float x, float s, float inv) {
     const float e = fmaf(-r, s, x), h = 0.5f * s;
     if (fabsf(e) > h || (fabsf(e) == h && ((int)r & 1))) r += e > 0.f ? 1.f : -1.f;
     return min(127, max(-127, (int)r));
+}
+
+// Four of them, packed.  Adding 1.5 x 2^23 rounds to the whole number and leaves it in the low byte; only where that lies
+// at or beyond a half (one in some hundred thousand) the exact rule is asked.
+__device__ __forceinline__ uint32_t nearest4(const float *x, float s, float inv) {
+    const float h = 0.5f * s;
+    uint32_t t[4];
+    bool close = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float y = fmaf(x[i], inv, 12582912.f);
+        t[i] = __float_as_uint(y);
+        close |= fabsf(fmaf(12582912.f - y, s, x[i])) >= h;
+    }
+    if (close)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = (uint32_t)nearest(x[i], s, inv);
+    return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
 
 // C: steps held in registers, 0: the row is read again in every pass; WARP: a row per warp, else per block
@@ -121,38 +139,45 @@ __global__ void __launch_bounds__(WARP ? 128 : kQMax) k_quantize_rows(QuantizeAr
         });
         rstd = 1.f / sqrtf(row_reduce<WARP>(sq, sm, add) / K + 1e-5f);
     }
+    const bool vec_ln = (reinterpret_cast<uintptr_t>(a.ln_g) | reinterpret_cast<uintptr_t>(a.ln_b)) % 16 == 0;
     auto norm = [&](int k, float(&e)[V]) {
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            e[i] = k + i < K ? (e[i] - mean) * rstd * __ldg(a.ln_g + k + i) + __ldg(a.ln_b + k + i) : 0.f;
+        for (int i = 0; i < V; i += 4) {
+            float g[4], b[4];
+            load16(a.ln_g, k + i, K, vec_ln, g);
+            load16(a.ln_b, k + i, K, vec_ln, b);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[i + j] = (e[i + j] - mean) * rstd * g[j] + b[j];  // behind K both are 0
+        }
     };
-    float top = 0.f;
-    bool odd = false;  // an infinity or a NaN
+    // the largest magnitude by its bits: an infinity or a NaN is above every number
+    uint32_t bits = 0;
     pass([&](int k, float(&e)[V]) {
         if (a.ln_g) norm(k, e);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            top = fmaxf(top, fabsf(e[i]));
-            odd |= !(fabsf(e[i]) <= 3.4028234e38f);
-        }
+        for (int i = 0; i < V; ++i) bits = max(bits, __float_as_uint(e[i]) & 0x7fffffffu);
     });
-    top = row_reduce<WARP>(odd ? INFINITY : top, sm, [](float p, float q) { return fmaxf(p, q); });
-    const bool good = top <= 3.4028234e38f;
-    const float s = __fdiv_rn(top, 127.f);
+    bits = row_reduce<WARP>(bits, reinterpret_cast<uint32_t *>(sm), [](uint32_t p, uint32_t q) { return max(p, q); });
+    const bool good = bits < 0x7f800000u;
+    const float s = __fdiv_rn(__uint_as_float(bits), 127.f);
     // where the scale's reciprocal or half would not be normal, x and s are taken times 2^64: the same quotient
-    const float up = s < 1e-30f ? 18446744073709551616.f : 1.f, su = s * up, inv = __fdiv_rn(1.f, su);
+    const bool tiny = s < 1e-30f;
+    const float up = tiny ? 18446744073709551616.f : 1.f, su = s * up, inv = __fdiv_rn(1.f, su);
     if (tid == 0) a.scale[row] = good ? s : __int_as_float(0x7fffffff);
     int8_t *q = a.q + (long long)row * a.ldq;
     pass([&](int k, float(&e)[V]) {
         if (a.ln_g && !C) norm(k, e);
-        uint32_t w[V / 4] = {};
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int r = good && s > 0.f && k + i < K ? nearest(e[i] * up, su, inv) : 0;
-            w[i / 4] |= (uint32_t)(r & 0xff) << (i % 4 * 8);
+        for (int i = 0; i < V; i += 4) {
+            uint32_t w = 0;
+            if (!tiny && good) {
+                w = nearest4(e + i, s, inv);
+            } else if (good && s > 0.f) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w |= (uint32_t)(nearest(e[i + j] * up, su, inv) & 0xff) << (8 * j);
+            }
+            *reinterpret_cast<uint32_t *>(q + k + i) = w;
         }
-#pragma unroll
-        for (int i = 0; i < V / 4; ++i) reinterpret_cast<uint32_t *>(q + k)[i] = w[i];
     });
     // the rest up to a multiple of 16 is zero: a product may read it
     const int done = (K + V - 1) / V * V, end = (K + 15) / 16 * 16;
@@ -192,10 +217,14 @@ __device__ __forceinline__ float gelu(float v) {
     return v * r;
 }
 // One output from its integer sum (exact: |sum| <= 2^14 K < 2^31).
+template <int EPI>
+__device__ __forceinline__ float output(int acc, float xs, float ws, float b) {
+    const float v = fmaf((float)acc * xs, ws, b);
+    return EPI == 1 ? gelu(v) : v;
+}
 template <typename T, int EPI>
 __device__ __forceinline__ void finish(int acc, float xs, float ws, float b, T *y) {
-    float v = fmaf((float)acc * xs, ws, b);
-    if (EPI == 1) v = gelu(v);
+    float v = output<EPI>(acc, xs, ws, b);
     if (EPI == 2) v += to_f32<T>(*y);
     *y = from_f32<T>(v);
 }
@@ -211,18 +240,22 @@ __host__ __device__ constexpr uint32_t idesc_i8(int M, int N) {
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// The word at the same place in the shared memory of block `rank` of the cluster.
-__device__ __forceinline__ int peer_word(const int *p, int rank) {
+// The same place in the shared memory of block `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_address(const void *p, int rank) {
     uint32_t at;
-    int v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ int peer_load(uint32_t at) {
+    int v;
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
     return v;
 }
+__device__ __forceinline__ int peer_word(const int *p, int rank) { return peer_load(peer_address(p, rank)); }
 
 constexpr int kMmThreads = 256, kMmTile = 128, kMmK = 128;  // 128 channels x NT tokens, 128 bytes of k a stage
 
-__host__ __device__ constexpr int mm_stages(int NT) { return NT <= 64 ? 6 : NT <= 128 ? 3 : 4; }
+__host__ __device__ constexpr int mm_stages(int NT) { return 6; }
 __host__ __device__ constexpr int mm_stage_bytes(int NT) { return (kMmTile + NT) * kMmK; }
 __host__ __device__ constexpr size_t mm_smem(int NT) { return (size_t)mm_stages(NT) * mm_stage_bytes(NT) + 1024; }
 
@@ -293,13 +326,25 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
         float f[16];
         __syncwarp();
         tmem_ld16(tmem + ((uint32_t)(warp & 3) << 21) + j0, f);
+        if (ks > 1) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int acc = __float_as_int(f[j]), m = m0 + j0 + j;
-            if (ks > 1)
-                part[(j0 + j) * kMmTile + ch] = acc;
-            else if (in && m < a.M)
-                finish<T, EPI>(acc, failed ? NAN : xs[j0 + j], ws, b, y + (long long)m * a.ldy);
+            for (int j = 0; j < 16; ++j) part[(j0 + j) * kMmTile + ch] = __float_as_int(f[j]);
+        } else {
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = output<EPI>(__float_as_int(f[j]), xs[j0 + j], ws, b);
+            T *at = y + (long long)(m0 + j0) * a.ldy;
+            if (EPI == 2) {
+                T old[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (in && m0 + j0 + j < a.M) old[j] = at[j * a.ldy];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] += to_f32<T>(old[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (in && m0 + j0 + j < a.M) at[j * a.ldy] = from_f32<T>(failed ? NAN : v[j]);
         }
     }
     tc_fence_before();
@@ -307,21 +352,76 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         int lost = 0;
         for (int r = 0; r < ks; ++r) lost |= peer_word(&failed, r);
-        for (int j = q + (tid >> 7) * ks; j < NT; j += 2 * ks) {
-            const int m = m0 + j, c = tid & 127;
-            if (m >= a.M) break;
-            int acc = 0;
-            for (int r = 0; r < ks; ++r) acc += peer_word(part + j * kMmTile + c, r);
-            const int nn = n0 + c;
-            if (nn < a.N)
-                finish<T, EPI>(acc, lost ? NAN : xs[j], __ldg(a.ws + nn), a.bias ? __ldg(a.bias + nn) : 0.f,
-                               reinterpret_cast<T *>(a.y) + (long long)m * a.ldy + nn);
+        const int c = tid & 127, nn = n0 + c, last = min(NT, a.M - m0);
+        const bool mine = nn < a.N;
+        const float sc = mine ? __ldg(a.ws + nn) : 0.f, bi = mine && a.bias ? __ldg(a.bias + nn) : 0.f;
+        for (int j0 = q + (tid >> 7) * ks; j0 < last; j0 += 8 * ks) {  // four tokens at a time
+            int acc[4] = {};
+            T old[4] = {};
+            for (int r = 0; r < ks; ++r) {
+                const uint32_t at = peer_address(part + c, r);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (j0 + 2 * i * ks < last) acc[i] += peer_load(at + (j0 + 2 * i * ks) * kMmTile * 4);
+            }
+            T *at = reinterpret_cast<T *>(a.y) + (long long)(m0 + j0) * a.ldy + nn;
+            if (EPI == 2)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (mine && j0 + 2 * i * ks < last) old[i] = at[2 * i * ks * a.ldy];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (mine && j0 + 2 * i * ks < last) {
+                    float v = output<EPI>(acc[i], xs[j0 + 2 * i * ks], sc, bi);
+                    if (EPI == 2) v += to_f32<T>(old[i]);
+                    at[2 * i * ks * a.ldy] = from_f32<T>(lost ? NAN : v);
+                }
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     __syncthreads();
     if (failed && tid == 0) drain_ring(full, S, issued);
     if (warp == 1) tc_fence_after(), tmem_dealloc(tmem, kCols);
+}
+
+// ---------------------------------------------------------------------------
+// a few rows: a warp per channel, 16 bytes of its weights per lane and step against MT rows (dp4a), the next steps' weights
+// on their way.  Bound by the latency of one trip to HBM and by its launch; no tensor memory, barriers or cluster.
+// ---------------------------------------------------------------------------
+constexpr int kFewWarps = 8;
+
+template <int MT, typename T, int EPI>
+__global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_few(LinearI8Args a) {
+    const int n = blockIdx.x * kFewWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31, units = (a.K + 15) / 16;
+    pdl_wait();
+    if (n >= a.N) return;
+    const uint4 *w = reinterpret_cast<const uint4 *>(a.w + (long long)n * a.ldw);
+    const float ws = __ldg(a.ws + n), b = a.bias ? __ldg(a.bias + n) : 0.f;
+    int acc[MT] = {};
+    constexpr int U = 4;
+    for (int u0 = lane; u0 < units; u0 += 32 * U) {
+        uint4 v[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) v[i] = u0 + 32 * i < units ? __ldg(w + u0 + 32 * i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (m >= a.M) break;
+            const uint4 *x = reinterpret_cast<const uint4 *>(a.x + m * a.ldx);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (u0 + 32 * i >= units) break;
+                const uint4 t = __ldg(x + u0 + 32 * i);
+                acc[m] = __dp4a((int)v[i].x, (int)t.x, acc[m]), acc[m] = __dp4a((int)v[i].y, (int)t.y, acc[m]);
+                acc[m] = __dp4a((int)v[i].z, (int)t.z, acc[m]), acc[m] = __dp4a((int)v[i].w, (int)t.w, acc[m]);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
+        if (m < a.M && lane == m) finish<T, EPI>(acc[m], __ldg(a.xs + m), ws, b, reinterpret_cast<T *>(a.y) + (long long)m * a.ldy + n);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -333,11 +433,6 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
 constexpr int kPrThreads = 320, kPrStages = 6, kPrStage = 2 * kMmTile * kMmK;
 constexpr size_t kPrSmem = (size_t)kPrStages * kPrStage + 1024;
 
-__device__ __forceinline__ uint32_t peer_address(const void *p, int rank) {
-    uint32_t at;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    return at;
-}
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -490,11 +585,26 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_linear_i8_pair(const __grid_c
                     __syncwarp();
                     if (lane == 0) arrive_at(peer_address(acc_free + b, 0));
                 }
+                // all of them first, then the stores: each 32 neighbouring channels of one token
+                float v[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    if (in && j0 + j < rows) finish<T, EPI>((int)acc[j], ok ? sx[j0 + j] : NAN, ws, bias, y);
-                    y += a.ldy;
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(sx + j0 + j);
+                    v[j] = output<EPI>((int)acc[j], x.x, ws, bias), v[j + 1] = output<EPI>((int)acc[j + 1], x.y, ws, bias);
+                    v[j + 2] = output<EPI>((int)acc[j + 2], x.z, ws, bias), v[j + 3] = output<EPI>((int)acc[j + 3], x.w, ws, bias);
                 }
+                if (EPI == 2) {
+                    T old[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (in && j0 + j < rows) old[j] = y[j * a.ldy];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] += to_f32<T>(old[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (in && j0 + j < rows) y[j * a.ldy] = from_f32<T>(ok ? v[j] : NAN);
+                y += 32 * a.ldy;
             }
             if (rows <= 0 && lane == 0) arrive_at(peer_address(acc_free + b, 0));
         }
@@ -556,8 +666,14 @@ cudaError_t product_pair(const LinearI8Args &a, cudaStream_t s) {
                         token_tiles, (int)tiles);
 }
 
+constexpr int kFewRows = 8;
+
 template <typename T, int EPI>
 cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
+    const unsigned few = (a.N + kFewWarps - 1) / kFewWarps;
+    if (a.M == 1) return launch_after(k_linear_i8_few<1, T, EPI>, few, kFewWarps * 32, 0, s, 1, a);
+    if (a.M <= 4) return launch_after(k_linear_i8_few<4, T, EPI>, few, kFewWarps * 32, 0, s, 1, a);
+    if (a.M <= kFewRows) return launch_after(k_linear_i8_few<8, T, EPI>, few, kFewWarps * 32, 0, s, 1, a);
     if (a.M <= 16) return product<16, T, EPI>(a, s);
     if (a.M <= 32) return product<32, T, EPI>(a, s);
     if (a.M <= 64) return product<64, T, EPI>(a, s);
