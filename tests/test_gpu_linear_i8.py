@@ -101,11 +101,11 @@ def test_quantize_behind_a_layer_norm(m, k, dtype):
     assert ((back - y).abs() <= 0.5 * s.double()[:, None] * (1 + 1e-6) + off).all()
 
 
-def product_case(m, k, n, ytype, epilogue, bias, seed=0, big=False):
+def product_case(m, k, n, ytype, epilogue, bias, seed=0, big=False, ldy=None):
     from whisper4j_b200 import _lib
     from whisper4j_b200._lib import check, lib
     g = torch.Generator("cuda").manual_seed(seed + m + 3 * k + 7 * n)
-    k16, ldy = (k + 15) // 16 * 16, n + 3
+    k16, ldy = (k + 15) // 16 * 16, ldy or n + 3
     xq = torch.zeros(m, k16 + 32, dtype=torch.int8, device="cuda")
     wq = torch.zeros(n, k16 + 16, dtype=torch.int8, device="cuda")
     if big:  # the largest sums there are
@@ -155,6 +155,14 @@ def test_product(m, k, n, epilogue, ytype):
 @pytest.mark.parametrize("epilogue,ytype", [(0, torch.float32), (1, torch.float16), (2, torch.bfloat16)])
 def test_large_products(m, k, n, epilogue, ytype):
     product_case(m, k, n, ytype, epilogue, True)
+
+
+@pytest.mark.parametrize("m,k,n", [(3000, 1280, 5120), (2049, 1008, 2050), (1537, 200, 2000), (12000, 48, 264)])
+@pytest.mark.parametrize("epilogue", [0, 1, 2])
+@pytest.mark.parametrize("ytype", TYPES)
+def test_large_products_with_aligned_rows(m, k, n, epilogue, ytype):
+    """Rows of y a multiple of 16 bytes apart: outputs may leave in boxes."""
+    product_case(m, k, n, ytype, epilogue, epilogue == 1, ldy=(n + 23) // 8 * 8)
 
 
 @pytest.mark.parametrize("m", [1, 4, 60, 300])

@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "host_api.cuh"
 #include "linear_i8.cuh"
 #include "tc_common.cuh"
@@ -68,28 +70,34 @@ __device__ __forceinline__ U row_reduce(U v, U *sm, Op op) {
 // The whole number nearest to x / s, ties to even, by the exact quotient: r from the rounded reciprocal is at most
 // one off, and x - r s, exact in one FMA wherever it matters, says on which side of a half x / s lies.  Within
 // +-127: a subnormal scale may have been rounded far down.
-__device__ __forceinline__ int nearest(float x, float s, float inv) {
+__device__ __noinline__ int nearest(float x, float s, float inv) {
     float r = rintf(x * inv);
     const float e = fmaf(-r, s, x), h = 0.5f * s;
     if (fabsf(e) > h || (fabsf(e) == h && ((int)r & 1))) r += e > 0.f ? 1.f : -1.f;
     return min(127, max(-127, (int)r));
 }
 
+// A row's scale s, and its reciprocal.  Where that or s / 2 would not be normal, x and s are taken times `up` = 2^64: the
+// same quotient.
+struct Step {
+    float s, inv, up;
+    bool tiny;
+};
 // Four of them, packed.  Adding 1.5 x 2^23 rounds to the whole number and leaves it in the low byte; only where that lies
 // at or beyond a half (one in some hundred thousand) the exact rule is asked.
-__device__ __forceinline__ uint32_t nearest4(const float *x, float s, float inv) {
-    const float h = 0.5f * s;
+__device__ __forceinline__ uint32_t nearest4(const float *x, const Step &p) {
+    const float h = 0.5f * p.s;
     uint32_t t[4];
-    bool close = false;
+    bool close = p.tiny;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float y = fmaf(x[i], inv, 12582912.f);
+        const float y = fmaf(x[i], p.inv, 12582912.f);
         t[i] = __float_as_uint(y);
-        close |= fabsf(fmaf(12582912.f - y, s, x[i])) >= h;
+        close |= fabsf(fmaf(12582912.f - y, p.s, x[i])) >= h;
     }
     if (close)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = (uint32_t)nearest(x[i], s, inv);
+        for (int i = 0; i < 4; ++i) t[i] = (uint32_t)nearest(x[i] * p.up, p.s * p.up, p.inv);
     return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
 
@@ -160,22 +168,16 @@ __global__ void __launch_bounds__(WARP ? 128 : kQMax) k_quantize_rows(QuantizeAr
     bits = row_reduce<WARP>(bits, reinterpret_cast<uint32_t *>(sm), [](uint32_t p, uint32_t q) { return max(p, q); });
     const bool good = bits < 0x7f800000u;
     const float s = __fdiv_rn(__uint_as_float(bits), 127.f);
-    // where the scale's reciprocal or half would not be normal, x and s are taken times 2^64: the same quotient
-    const bool tiny = s < 1e-30f;
-    const float up = tiny ? 18446744073709551616.f : 1.f, su = s * up, inv = __fdiv_rn(1.f, su);
+    Step p;
+    p.s = s, p.tiny = s < 1e-30f, p.up = p.tiny ? 18446744073709551616.f : 1.f, p.inv = __fdiv_rn(1.f, s * p.up);
+    const bool any = good && s > 0.f;
     if (tid == 0) a.scale[row] = good ? s : __int_as_float(0x7fffffff);
     int8_t *q = a.q + (long long)row * a.ldq;
     pass([&](int k, float(&e)[V]) {
         if (a.ln_g && !C) norm(k, e);
 #pragma unroll
         for (int i = 0; i < V; i += 4) {
-            uint32_t w = 0;
-            if (!tiny && good) {
-                w = nearest4(e + i, s, inv);
-            } else if (good && s > 0.f) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w |= (uint32_t)(nearest(e[i + j] * up, su, inv) & 0xff) << (8 * j);
-            }
+            const uint32_t w = any ? nearest4(e + i, p) : 0;  // (zeros behind K: x is 0 there)
             *reinterpret_cast<uint32_t *>(q + k + i) = w;
         }
     });
@@ -208,19 +210,53 @@ cudaError_t quantize(const QuantizeArgs &a, cudaStream_t s) {
 // ---------------------------------------------------------------------------
 // product
 // ---------------------------------------------------------------------------
-// GELU in its tanh form, as v / (1 + 2^t) with t = -2 log2(e) u: no cancellation, and the right limits where the
-// exponential leaves its range.
-__device__ __forceinline__ float gelu(float v) {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * fmaf(v * v, -0.1029432397f, -2.3022081985f)));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    return v * r;
+__device__ __forceinline__ uint64_t pack(float lo, float hi) {
+    return (uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo);
 }
+__device__ __forceinline__ uint64_t both(float v) { return pack(v, v); }
+__device__ __forceinline__ float lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// GELU of two numbers in its tanh form, as v / (1 + 2^t) with t = -2 log2(e) u: no cancellation.  t stops at 63 (what is
+// beyond is below 1e-18), so that one reciprocal of the product serves both denominators.
+__device__ __forceinline__ uint64_t gelu2(uint64_t v) {
+    const uint64_t t = mul2(v, fma2(mul2(v, v), both(-0.1029432397f), both(-2.3022081985f)));
+    const uint64_t d = add2(pack(ex2(fminf(lo(t), 63.f)), ex2(fminf(hi(t), 63.f))), both(1.f));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(lo(d) * hi(d)));
+    return mul2(mul2(v, both(r)), pack(hi(d), lo(d)));
+}
+__device__ __forceinline__ float gelu(float v) { return lo(gelu2(both(v))); }
 // One output from its integer sum (exact: |sum| <= 2^14 K < 2^31).
 template <int EPI>
 __device__ __forceinline__ float output(int acc, float xs, float ws, float b) {
     const float v = fmaf((float)acc * xs, ws, b);
     return EPI == 1 ? gelu(v) : v;
+}
+// Two outputs of one channel.
+template <int EPI>
+__device__ __forceinline__ uint64_t output2(int a0, int a1, uint64_t xs, uint64_t ws, uint64_t b) {
+    const uint64_t v = fma2(mul2(pack((float)a0, (float)a1), xs), ws, b);
+    return EPI == 1 ? gelu2(v) : v;
 }
 template <typename T, int EPI>
 __device__ __forceinline__ void finish(int acc, float xs, float ws, float b, T *y) {
@@ -430,8 +466,10 @@ __global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_few(LinearI8Args a
 // and SM at the integer MMAs' 8192 products, where a single SM's 128 x 256 tile would want 96.  Persistent: two
 // accumulators in tensor memory, and eight warps turn one into outputs while the next tile's products run.
 // ---------------------------------------------------------------------------
-constexpr int kPrThreads = 320, kPrStages = 6, kPrStage = 2 * kMmTile * kMmK;
-constexpr size_t kPrSmem = (size_t)kPrStages * kPrStage + 1024;
+constexpr int kPrThreads = 320, kPrStage = 2 * kMmTile * kMmK;
+constexpr int pr_stages(int bytes) { return bytes == 4 ? 4 : 5; }
+constexpr int pr_out(int bytes) { return 2 * 32 * 32 * bytes; }  // a warp's two outgoing boxes
+constexpr size_t pr_smem(int bytes) { return (size_t)pr_stages(bytes) * kPrStage + 8 * pr_out(bytes) + 1024; }
 
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -477,10 +515,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-template <typename T, int EPI>
+// TMA: outputs leave as boxes of 32 channels x 32 tokens through shared memory (ymap; not with a residual)
+template <typename T, int EPI, bool TMA>
 __global__ void __launch_bounds__(kPrThreads, 1) k_linear_i8_pair(const __grid_constant__ CUtensorMap wmap,
-                                                                  const __grid_constant__ CUtensorMap xmap, LinearI8Args a,
+                                                                  const __grid_constant__ CUtensorMap xmap,
+                                                                  const __grid_constant__ CUtensorMap ymap, LinearI8Args a,
                                                                   int token_tiles, int tiles) {
+    constexpr int kPrStages = pr_stages(sizeof(T)), kPrOut = pr_out(sizeof(T));
     extern __shared__ unsigned char raw[];
     unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t full[kPrStages], empty[kPrStages], acc_full[2], acc_free[2], drained;
@@ -562,19 +603,23 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_linear_i8_pair(const __grid_c
         // warps of one lane quarter take the tokens' halves
         const int e = warp - 2, quarter = warp & 3, half = e >> 2;
         float *sx = xs[e];
-        int n = 0;
+        unsigned char *out = sm + kPrStages * kPrStage + e * kPrOut;
+        int n = 0, sent = 0;
         bool ok = true;
         for (int t = blockIdx.x / 2; t < tiles; t += pairs, ++n) {
             const int b = n & 1, ch = t / token_tiles * 256 + 128 * rank + 32 * quarter + lane, m0 = t % token_tiles * 256 + 128 * half;
             const int rows = min(128, a.M - m0);
             const bool in = ch < a.N;
-            const float ws = in ? __ldg(a.ws + ch) : 0.f, bias = in && a.bias ? __ldg(a.bias + ch) : 0.f;
+            float ws = in ? __ldg(a.ws + ch) : 0.f;
+            const float bias = in && a.bias ? __ldg(a.bias + ch) : 0.f;
             __syncwarp();
 #pragma unroll
             for (int j = lane; j < 128; j += 32) sx[j] = j < rows ? __ldg(a.xs + m0 + j) : 0.f;
             __syncwarp();
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(acc_full + b, (n / 2) & 1, &failed));
+            if (!ok) ws = NAN;  // after a wait that ran out every output is NaN
             tc_fence_after();
+            const uint64_t ws2 = both(ws), bias2 = both(bias);
             T *y = reinterpret_cast<T *>(a.y) + (long long)m0 * a.ldy + ch;
             for (int j0 = 0; j0 < rows; j0 += 32) {
                 uint32_t acc[32];
@@ -585,29 +630,49 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_linear_i8_pair(const __grid_c
                     __syncwarp();
                     if (lane == 0) arrive_at(peer_address(acc_free + b, 0));
                 }
-                // all of them first, then the stores: each 32 neighbouring channels of one token
-                float v[32];
+                uint64_t v[16];
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 x = *reinterpret_cast<const float4 *>(sx + j0 + j);
-                    v[j] = output<EPI>((int)acc[j], x.x, ws, bias), v[j + 1] = output<EPI>((int)acc[j + 1], x.y, ws, bias);
-                    v[j + 2] = output<EPI>((int)acc[j + 2], x.z, ws, bias), v[j + 3] = output<EPI>((int)acc[j + 3], x.w, ws, bias);
+                for (int j = 0; j < 16; j += 2) {
+                    const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(sx + j0 + 2 * j);
+                    v[j] = output2<EPI>((int)acc[2 * j], (int)acc[2 * j + 1], x.x, ws2, bias2);
+                    v[j + 1] = output2<EPI>((int)acc[2 * j + 2], (int)acc[2 * j + 3], x.y, ws2, bias2);
                 }
+                if (TMA) {
+                    T *box = reinterpret_cast<T *>(out + (sent & 1) * (kPrOut / 2));
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        box[64 * j + lane] = from_f32<T>(lo(v[j])), box[64 * j + 32 + lane] = from_f32<T>(hi(v[j]));
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {  // rows and channels beyond y are left out by the map
+                        if (ch < a.N)
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&ymap),
+                                         "r"(ch), "r"(m0 + j0), "r"(smem_u32(box))
+                                         : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                    ++sent;
+                    continue;
+                }
+                // each store 32 neighbouring channels of one token
                 if (EPI == 2) {
                     T old[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
                         if (in && j0 + j < rows) old[j] = y[j * a.ldy];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] += to_f32<T>(old[j]);
+                    for (int j = 0; j < 16; ++j) v[j] = add2(v[j], pack(to_f32<T>(old[2 * j]), to_f32<T>(old[2 * j + 1])));
                 }
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
-                    if (in && j0 + j < rows) y[j * a.ldy] = from_f32<T>(ok ? v[j] : NAN);
+                    if (in && j0 + j < rows) y[j * a.ldy] = from_f32<T>(j & 1 ? hi(v[j / 2]) : lo(v[j / 2]));
                 y += 32 * a.ldy;
             }
             if (rows <= 0 && lane == 0) arrive_at(peer_address(acc_free + b, 0));
         }
+        if (TMA && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
@@ -618,8 +683,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_linear_i8_pair(const __grid_c
     }
 }
 
-// [box rows x 128 bytes] boxes of a row-major 8-bit matrix, 128-byte swizzle; reads beyond rows or columns give zeros
-bool tmap_i8(CUtensorMap *m, const int8_t *base, long long rows, int cols, long long ld, int box) {
+// Boxes of a row-major matrix, ld bytes from row to row; reads beyond its rows or columns give zeros, writes there are
+// left out.
+bool tmap_2d(CUtensorMap *m, CUtensorMapDataType type, const void *base, long long rows, int cols, long long ld, int box_cols,
+             int box_rows, CUtensorMapSwizzle swizzle) {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult r;
@@ -629,10 +696,13 @@ bool tmap_i8(CUtensorMap *m, const int8_t *base, long long rows, int cols, long 
     }();
     if (!fn) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
-    const cuuint32_t boxes[2] = {(cuuint32_t)kMmK, (cuuint32_t)box}, estr[2] = {1, 1};
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(base), dims, strides, boxes, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    return fn(m, type, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// [box x 128 bytes] of an operand, with the 128-byte swizzle of the MMA's K-major operands
+bool tmap_i8(CUtensorMap *m, const int8_t *base, long long rows, int cols, long long ld, int box) {
+    return tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, cols, ld, kMmK, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int NT, typename T, int EPI>
@@ -660,10 +730,21 @@ cudaError_t product_pair(const LinearI8Args &a, cudaStream_t s) {
     const int token_tiles = (a.M + 255) / 256;
     const long long tiles = (long long)((a.N + 255) / 256) * token_tiles;
     if (tiles > 0x7fffffff) return cudaErrorInvalidValue;
-    cudaError_t e = allow_smem<k_linear_i8_pair<T, EPI>>(kPrSmem);
-    if (e != cudaSuccess) return e;
-    return launch_after(k_linear_i8_pair<T, EPI>, 2 * (unsigned)(tiles < 74 ? tiles : 74), kPrThreads, kPrSmem, s, 2, wmap, xmap, a,
-                        token_tiles, (int)tiles);
+    const unsigned blocks = 2 * (unsigned)(tiles < 74 ? tiles : 74);
+    cudaError_t e;
+    CUtensorMap ymap = {};
+    // (a box that ends inside 16 bytes of y would write all of them: then the last channel has to end on their border)
+    if (EPI != 2 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.ldy * sizeof(T) % 16 == 0 && a.N * sizeof(T) % 16 == 0) {
+        const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                         : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        if (!tmap_2d(&ymap, type, a.y, a.M, a.N, a.ldy * sizeof(T), 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE)) return cudaErrorInvalidValue;
+        if ((e = allow_smem<k_linear_i8_pair<T, EPI, true>>(pr_smem(sizeof(T)))) != cudaSuccess) return e;
+        return launch_after(k_linear_i8_pair<T, EPI, true>, blocks, kPrThreads, pr_smem(sizeof(T)), s, 2, wmap, xmap, ymap, a, token_tiles,
+                            (int)tiles);
+    }
+    if ((e = allow_smem<k_linear_i8_pair<T, EPI, false>>(pr_smem(sizeof(T)))) != cudaSuccess) return e;
+    return launch_after(k_linear_i8_pair<T, EPI, false>, blocks, kPrThreads, pr_smem(sizeof(T)), s, 2, wmap, xmap, ymap, a, token_tiles,
+                        (int)tiles);
 }
 
 constexpr int kFewRows = 8;
