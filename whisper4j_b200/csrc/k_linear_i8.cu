@@ -39,11 +39,11 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 // ---------------------------------------------------------------------------
 constexpr int kQMax = 1024;
 
-// The 16 bytes of elements from k on (zeros behind K).
-template <typename T>
-__device__ __forceinline__ void load16(const T *x, int k, int K, bool vec, float (&v)[16 / sizeof(T)]) {
+// The 16 bytes of elements from k on; one by one, with zeros behind K, where rows are not whole 16-byte units.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void load16(const T *x, int k, int K, float (&v)[16 / sizeof(T)]) {
     constexpr int V = 16 / sizeof(T);
-    if (vec && k + V <= K) {
+    if (WHOLE) {
         T t[V];
         *reinterpret_cast<uint4 *>(t) = __ldg(reinterpret_cast<const uint4 *>(x + k));
 #pragma unroll
@@ -101,22 +101,24 @@ __device__ __forceinline__ uint32_t nearest4(const float *x, const Step &p) {
     return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
 
-// C: steps held in registers, 0: the row is read again in every pass; WARP: a row per warp, else per block
+// C: steps held in registers, 0: any rows, read again in every pass (C > 0: K, x, ldx and a LayerNorm's vectors are whole
+// 16-byte units); WARP: a row per warp, else per block
 template <typename T, int C, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : kQMax) k_quantize_rows(QuantizeArgs a) {
     constexpr int V = 16 / sizeof(T);
+    constexpr bool WHOLE = C > 0;
     __shared__ float sm[kQMax / 32];
     pdl_wait();
     pdl_trigger();
     const int row = WARP ? blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x, tid = WARP ? threadIdx.x % 32 : threadIdx.x;
     if (row >= a.M) return;
     const T *x = reinterpret_cast<const T *>(a.x) + (long long)row * a.ldx;
-    const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0;
     const int step = (WARP ? 32 : blockDim.x) * V, k0 = tid * V, K = a.K;
     float v[C ? C : 1][V];
     if (C) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) load16(x, k0 + c * step, K, vec, v[c]);
+        for (int c = 0; c < C; ++c)
+            if (k0 + c * step < K) load16<T, WHOLE>(x, k0 + c * step, K, v[c]);
     }
     // f(k, the elements from k on): over the row
     auto pass = [&](auto f) {
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kQMax) k_quantize_rows(QuantizeAr
                 if (k0 + c * step < K) f(k0 + c * step, v[c]);
         } else {
             for (int k = k0; k < K; k += step) {
-                load16(x, k, K, vec, v[0]);
+                load16<T, WHOLE>(x, k, K, v[0]);
                 f(k, v[0]);
             }
         }
@@ -143,17 +145,16 @@ __global__ void __launch_bounds__(WARP ? 128 : kQMax) k_quantize_rows(QuantizeAr
         pass([&](int k, float(&e)[V]) {
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (k + i < K) sq += (e[i] - mean) * (e[i] - mean);
+                if (WHOLE || k + i < K) sq += (e[i] - mean) * (e[i] - mean);
         });
         rstd = 1.f / sqrtf(row_reduce<WARP>(sq, sm, add) / K + 1e-5f);
     }
-    const bool vec_ln = (reinterpret_cast<uintptr_t>(a.ln_g) | reinterpret_cast<uintptr_t>(a.ln_b)) % 16 == 0;
     auto norm = [&](int k, float(&e)[V]) {
 #pragma unroll
         for (int i = 0; i < V; i += 4) {
             float g[4], b[4];
-            load16(a.ln_g, k + i, K, vec_ln, g);
-            load16(a.ln_b, k + i, K, vec_ln, b);
+            load16<float, WHOLE>(a.ln_g, k + i, K, g);
+            load16<float, WHOLE>(a.ln_b, k + i, K, b);
 #pragma unroll
             for (int j = 0; j < 4; ++j) e[i + j] = (e[i + j] - mean) * rstd * g[j] + b[j];  // behind K both are 0
         }
@@ -192,7 +193,9 @@ template <typename T>
 cudaError_t quantize(const QuantizeArgs &a, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
     const int units = (a.K + V - 1) / V, c = (units + 31) / 32;
-    if (a.M >= 148 * 4 * 2 && c <= 16) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.ln_g) | reinterpret_cast<uintptr_t>(a.ln_b);
+    const bool whole = at % 16 == 0 && a.K % V == 0 && a.ldx % V == 0;
+    if (a.M >= 148 * 4 * 2 && c <= 16 && whole) {
         const unsigned blocks = (a.M + 3) / 4;
         if (c <= 4) return launch_after(k_quantize_rows<T, 4, true>, blocks, 128, 0, s, 1, a);
         if (c <= 8) return launch_after(k_quantize_rows<T, 8, true>, blocks, 128, 0, s, 1, a);
@@ -201,6 +204,7 @@ cudaError_t quantize(const QuantizeArgs &a, cudaStream_t s) {
     }
     const int most = a.M >= 148 * 4 ? 256 : kQMax, held = (units + most - 1) / most;
     const int threads = held <= 4 ? (units + held - 1) / held : most, block = (threads + 31) / 32 * 32;
+    if (!whole) return launch_after(k_quantize_rows<T, 0, false>, a.M, block, 0, s, 1, a);
     if (held == 1) return launch_after(k_quantize_rows<T, 1, false>, a.M, block, 0, s, 1, a);
     if (held == 2) return launch_after(k_quantize_rows<T, 2, false>, a.M, block, 0, s, 1, a);
     if (held <= 4) return launch_after(k_quantize_rows<T, 4, false>, a.M, block, 0, s, 1, a);
@@ -464,12 +468,12 @@ __global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_few(LinearI8Args a
 // many rows: a pair of SMs owns 256 channels x 256 tokens at a time (tcgen05.mma with cta_group::2), each with 128 of the
 // channels and half of the tokens in its shared memory, so that a tile's operands cross from L2 once: 64 bytes a cycle
 // and SM at the integer MMAs' 8192 products, where a single SM's 128 x 256 tile would want 96.  Persistent: two
-// accumulators in tensor memory, and eight warps turn one into outputs while the next tile's products run.
+// accumulators in tensor memory, and sixteen warps turn one into outputs while the next tile's products run.
 // ---------------------------------------------------------------------------
-constexpr int kPrThreads = 320, kPrStage = 2 * kMmTile * kMmK;
+constexpr int kPrWarps = 16, kPrThreads = 64 + 32 * kPrWarps, kPrTokens = 1024 / kPrWarps, kPrStage = 2 * kMmTile * kMmK;
 constexpr int pr_stages(int bytes) { return bytes == 4 ? 4 : 5; }
-constexpr int pr_out(int bytes) { return 2 * 32 * 32 * bytes; }  // a warp's two outgoing boxes
-constexpr size_t pr_smem(int bytes) { return (size_t)pr_stages(bytes) * kPrStage + 8 * pr_out(bytes) + 1024; }
+constexpr int pr_out(int bytes) { return 32 * 32 * bytes; }  // a warp's outgoing box
+constexpr size_t pr_smem(int bytes) { return (size_t)pr_stages(bytes) * kPrStage + kPrWarps * pr_out(bytes) + 1024; }
 
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -527,12 +531,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_linear_i8_pair(const __grid_c
     __shared__ uint64_t full[kPrStages], empty[kPrStages], acc_full[2], acc_free[2], drained;
     __shared__ uint32_t slot;
     __shared__ int failed;
-    __shared__ __align__(16) float xs[8][128];
+    __shared__ __align__(16) float xs[kPrWarps][kPrTokens];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x & 1;
     const int nk = (a.K + kMmK - 1) / kMmK, pairs = gridDim.x / 2;
     if (tid == 0) {
         for (int i = 0; i < kPrStages; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(acc_full + i, 1), mbar_init(acc_free + i, 16);
+        for (int i = 0; i < 2; ++i) mbar_init(acc_full + i, 1), mbar_init(acc_free + i, 2 * kPrWarps);
         mbar_init(&drained, 1);
         fence_mbar_init();
         failed = 0;
@@ -600,21 +604,21 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_linear_i8_pair(const __grid_c
             }
         }
     } else {
-        // warps of one lane quarter take the tokens' halves
-        const int e = warp - 2, quarter = warp & 3, half = e >> 2;
+        // the warps of one lane quarter share the tokens
+        const int e = warp - 2, quarter = warp & 3, first = e / 4 * kPrTokens;
         float *sx = xs[e];
         unsigned char *out = sm + kPrStages * kPrStage + e * kPrOut;
-        int n = 0, sent = 0;
+        int n = 0;
         bool ok = true;
         for (int t = blockIdx.x / 2; t < tiles; t += pairs, ++n) {
-            const int b = n & 1, ch = t / token_tiles * 256 + 128 * rank + 32 * quarter + lane, m0 = t % token_tiles * 256 + 128 * half;
-            const int rows = min(128, a.M - m0);
+            const int b = n & 1, ch = t / token_tiles * 256 + 128 * rank + 32 * quarter + lane, m0 = t % token_tiles * 256 + first;
+            const int rows = min(kPrTokens, a.M - m0);
             const bool in = ch < a.N;
             float ws = in ? __ldg(a.ws + ch) : 0.f;
             const float bias = in && a.bias ? __ldg(a.bias + ch) : 0.f;
             __syncwarp();
 #pragma unroll
-            for (int j = lane; j < 128; j += 32) sx[j] = j < rows ? __ldg(a.xs + m0 + j) : 0.f;
+            for (int j = lane; j < kPrTokens; j += 32) sx[j] = j < rows ? __ldg(a.xs + m0 + j) : 0.f;
             __syncwarp();
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(acc_full + b, (n / 2) & 1, &failed));
             if (!ok) ws = NAN;  // after a wait that ran out every output is NaN
@@ -624,7 +628,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_linear_i8_pair(const __grid_c
             for (int j0 = 0; j0 < rows; j0 += 32) {
                 uint32_t acc[32];
                 __syncwarp();
-                tmem_ld32(tmem + ((uint32_t)quarter << 21) + 256 * b + 128 * half + j0, acc);
+                tmem_ld32(tmem + ((uint32_t)quarter << 21) + 256 * b + first + j0, acc);
                 if (j0 + 32 >= rows) {  // the accumulator has been read
                     tc_fence_before();
                     __syncwarp();
@@ -638,8 +642,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_linear_i8_pair(const __grid_c
                     v[j + 1] = output2<EPI>((int)acc[2 * j + 2], (int)acc[2 * j + 3], x.y, ws2, bias2);
                 }
                 if (TMA) {
-                    T *box = reinterpret_cast<T *>(out + (sent & 1) * (kPrOut / 2));
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    T *box = reinterpret_cast<T *>(out);
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
@@ -653,7 +657,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_linear_i8_pair(const __grid_c
                                          : "memory");
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
-                    ++sent;
                     continue;
                 }
                 // each store 32 neighbouring channels of one token
