@@ -458,6 +458,17 @@ int w4j_op_linear_i8(int device, const int8_t *x, int64_t ldx, const float *x_sc
                      int64_t ldw, const float *w_scale, int N, const float *bias, int epilogue, void *y, int y_type,
                      int64_t ldy, void *stream);
 
+/*
+ * The two in one call, x in floats (as w4j_op_quantize_rows) and y as w4j_op_linear_i8 makes it: up to 8 rows that fit
+ * 48 KB as integers take one launch.  Behind a LayerNorm its sums may run in another order there, so that a quotient
+ * next to a half may fall to its other side.  work: w4j_op_linear_i8_layer_workspace(M, K) bytes (0 for those few rows),
+ * 16-byte aligned, for this call alone until it has run.
+ */
+size_t w4j_op_linear_i8_layer_workspace(int M, int K);
+int w4j_op_linear_i8_layer(int device, const void *x, int x_type, int64_t ldx, const float *ln_g, const float *ln_b, int M,
+                           int K, const int8_t *w, int64_t ldw, const float *w_scale, int N, const float *bias,
+                           int epilogue, void *y, int y_type, int64_t ldy, void *work, size_t work_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -31,7 +31,7 @@ def quantised(x):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,k", [(1, 1), (1, 1280), (3, 7), (5, 8), (2, 9), (4, 16), (7, 100), (33, 1000), (300, 1280), (64, 2049),
-                                 (10, 5120), (3, 8200), (2, 20001)])
+                                 (10, 5120), (3, 8200), (2, 20001), (1300, 1280), (1500, 130), (1201, 2048), (1200, 4096)])
 def test_quantize_is_exact(m, k, dtype):
     from whisper4j_b200 import ops
     g = torch.Generator("cuda").manual_seed(m + k)
@@ -79,10 +79,11 @@ def test_rows_that_are_not_finite():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("m,k", [(1, 16), (4, 1280), (33, 777), (2, 5120), (2, 9001)])
+@pytest.mark.parametrize("m,k", [(1, 16), (4, 1280), (33, 777), (2, 5120), (2, 9001), (1500, 1280), (1200, 2048)])
 def test_quantize_behind_a_layer_norm(m, k, dtype):
-    """The normalised row is off by 32-bit sums of depth d = 8 ceil(K / 2048) + 20 (a thread's run, the warp, the block):
-    the mean by d E mean|x|, the deviation's factor by (d + 8) E; a quantised number by half a step more."""
+    """The normalised row is off by 32-bit sums of depth d, a thread's run of 8 ceil(K / 2048) elements (ceil(K / 32) where
+    rows are many) and 20 for the warp and the block: the mean by d E mean|x|, the deviation's factor by (d + 8) E; a
+    quantised number by half a step more."""
     from whisper4j_b200 import ops
     g = torch.Generator("cuda").manual_seed(k)
     x = (torch.randn(m, k, device="cuda", generator=g) * 3 + 1).to(dtype)
@@ -93,7 +94,7 @@ def test_quantize_behind_a_layer_norm(m, k, dtype):
     mean = x.mean(1, keepdim=True)
     rstd = 1 / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + 1e-5)
     y = (x - mean) * rstd * gamma.double() + beta.double()
-    d = 8 * math.ceil(k / 2048) + 20
+    d = (8 * math.ceil(k / 2048) if m < 1000 else math.ceil(k / 32)) + 20
     off = gamma.double().abs() * rstd * d * E * x.abs().mean(1, keepdim=True) + (y - beta.double()).abs() * (d + 8) * E + y.abs() * 2 * E
     want = y.abs().amax(1) / 127
     assert ((s.double() - want).abs() <= off.amax(1) / 127 + 2 * E * want).all()
@@ -192,6 +193,49 @@ def test_layer(xtype, ytype):
     again = layer(x, epilogue="residual", out=y.clone())
     assert ((again.double() - 2 * v).abs() <= (16 * E + 3 * half) * (2 * v.abs() + b.double().abs())).all()
     assert layer(x[:0]).shape == (0, 700)
+
+
+@pytest.mark.parametrize("ln", [False, True])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("k,n,xtype", [(1, 3, torch.float32), (384, 1152, torch.float16), (1000, 50, torch.bfloat16),
+                                       (5120, 129, torch.float32), (6200, 40, torch.float32), (20000, 10, torch.float32)])
+def test_layer_of_a_few_rows(m, k, n, xtype, ln):
+    """One launch where the rows are few and short, two where not; behind a LayerNorm against its exact value: a
+    quantised number may be half a step off, and more by the LayerNorm's own sums (a run of ceil(K / 32) + 20 at most)."""
+    from whisper4j_b200 import ops
+    g = torch.Generator("cuda").manual_seed(m + k)
+    w, b = torch.randn(n, k, device="cuda", generator=g) * k ** -0.5, torch.randn(n, device="cuda", generator=g)
+    x = (torch.randn(m, k + 3, device="cuda", generator=g) * 2 + 0.5).to(xtype)[:, 1:k + 1]
+    norm = (1 + 0.1 * torch.randn(k, device="cuda", generator=g), 0.1 * torch.randn(k, device="cuda", generator=g)) if ln else None
+    layer = ops.Int8Linear.from_float(w, b)
+    y = layer(x, ln=norm, out_dtype=torch.float32)
+    wq, ws = quantised(w)
+    v = x.double()
+    if not ln:
+        q, s = quantised(x.float())
+        want = (q.double() @ wq.double().T) * s.double()[:, None] * ws.double() + b.double()
+        assert ((y.double() - want).abs() <= 8 * E * (want.abs() + b.double().abs())).all()
+        return
+    mean = v.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((v - mean) ** 2).mean(1, keepdim=True) + 1e-5)
+    z = (v - mean) * rstd * norm[0].double() + norm[1].double()
+    d = math.ceil(k / 32) + 20
+    off = norm[0].double().abs() * rstd * d * E * v.abs().mean(1, keepdim=True) + (z - norm[1].double()).abs() * (d + 8) * E + z.abs() * 2 * E
+    step = z.abs().amax(1, keepdim=True) / 127
+    wide = wq.double().abs() * ws.double()[:, None]
+    want = z @ (wq.double() * ws.double()[:, None]).T + b.double()
+    tol = (0.5 * step * (1 + 1e-5) + off).expand_as(z) @ wide.T
+    assert ((y.double() - want).abs() <= tol + 8 * E * (want.abs() + b.double().abs())).all()
+
+
+def test_a_few_rows_that_are_not_finite():
+    from whisper4j_b200 import ops
+    layer = ops.Int8Linear.from_float(torch.randn(20, 70, device="cuda"))
+    x = torch.randn(5, 70, device="cuda")
+    x[1, 69], x[2], x[3, 0], x[4] = float("nan"), 0, float("-inf"), 1e-42
+    y = layer(x)
+    assert torch.isnan(y).all(1).tolist() == [False, True, False, True, False]
+    assert not y[2].any()
 
 
 def test_captured_on_a_side_stream():

@@ -172,3 +172,26 @@ def linear(device=0, x=P, ldx=112, xs=P, m=2, k=100, w=P, ldw=112, ws=P, n=30, b
     (dict(epilogue=-1), "epilogue")])
 def test_linear_refusals(kw, text):
     refused(linear(**kw), text)
+
+
+def layer(device=0, x=P, x_type=GGML_F32, ldx=100, g=None, b=None, m=9, k=100, w=P, ldw=112, ws=P, n=30, bias=None, epilogue=0, y=P,
+          y_type=GGML_F32, ldy=30, work=P, work_bytes=9 * 116):
+    return lib().w4j_op_linear_i8_layer(device, x, x_type, ldx, g, b, m, k, w, ldw, ws, n, bias, epilogue, y, y_type, ldy, work,
+                                        work_bytes, None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(x=None), "null"), (dict(w=None), "null"), (dict(ws=None), "null"), (dict(y=None), "null"), (dict(x_type=8), "x_type"),
+    (dict(y_type=2), "y_type"), (dict(m=0), "shape"), (dict(n=0), "shape"), (dict(k=0), "shape"), (dict(ldx=99), "ldx"),
+    (dict(g=P), "gamma"), (dict(k=131057, ldx=131057, ldw=131072, work_bytes=1 << 30), "131056"), (dict(ldw=104), "rows"),
+    (dict(w=P + 8), "aligned"), (dict(ldy=29), "ldy"), (dict(y=P + 2), "aligned"), (dict(x=P + 2), "aligned"),
+    (dict(epilogue=3), "epilogue"), (dict(work=None), "work"), (dict(work=P + 4), "work"), (dict(work_bytes=9 * 116 - 1), "work")])
+def test_layer_refusals(kw, text):
+    refused(layer(**kw), text)
+
+
+def test_layer_workspace():
+    w = lib().w4j_op_linear_i8_layer_workspace
+    assert w(9, 100) == 9 * (112 + 4) and w(8, 1280) == 0 and w(1, 40000) == 0 and w(8, 7000) == 8 * (7008 + 4)
+    for m, k in ((0, 1), (1, 0), (1, 131057), ((1 << 24) + 1, 1)):
+        assert w(m, k) == 0 and b"shape" in lib().w4j_last_error()

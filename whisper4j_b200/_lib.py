@@ -127,6 +127,8 @@ SIGNATURES = {
     "w4j_op_attn_shared_workspace": (_SZ, [_P]),
     "w4j_op_attn_shared": (_I, [_P, _P]),
     "w4j_op_quantize_rows": (_I, [_I, _P, _I, _I, _I, _I64, _P, _P, _P, _I64, _P, _P]),
+    "w4j_op_linear_i8_layer_workspace": (_SZ, [_I, _I]),
+    "w4j_op_linear_i8_layer": (_I, [_I, _P, _I, _I64, _P, _P, _I, _I, _P, _I64, _P, _I, _P, _I, _P, _I, _I64, _P, _SZ, _P]),
     "w4j_op_linear_i8": (_I, [_I, _P, _I64, _P, _I, _I, _P, _I64, _P, _I, _P, _I, _P, _I, _I64, _P]),
 }
 

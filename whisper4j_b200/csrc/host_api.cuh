@@ -15,11 +15,15 @@ int set_err(int code, const char *fmt, ...);
 class DeviceGuard {
   public:
     explicit DeviceGuard(int device) {
-        int n = 0;
-        if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+        static std::atomic<int> count{0};  // devices do not come and go
+        int n = count.load(std::memory_order_relaxed);
+        if (n == 0 && (cudaGetDeviceCount(&n) != cudaSuccess || n == 0)) {
             cudaGetLastError();
             rc_ = set_err(W4J_ERR_CUDA, "no CUDA device available");
-        } else if (device < 0 || device >= n) {
+            return;
+        }
+        count.store(n, std::memory_order_relaxed);
+        if (device < 0 || device >= n) {
             rc_ = set_err(W4J_ERR_ARG, "device %d out of range (%d devices)", device, n);
         } else if (cudaGetDevice(&before_) != cudaSuccess ||
                    (before_ != device && cudaSetDevice(device) != cudaSuccess)) {

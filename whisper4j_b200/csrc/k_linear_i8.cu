@@ -464,6 +464,119 @@ __global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_few(LinearI8Args a
     }
 }
 
+// The whole layer for a few rows in one launch: every block quantises the rows for itself (8, 4, 2 or 1 warps to a row)
+// into shared memory while the first 2 KB of its channels' weights are on their way.
+constexpr size_t kLayerSmem = 48 * 1024;
+
+__device__ __forceinline__ float load1(const void *x, int type, long long i) {
+    return type == W4J_GGML_F32 ? __ldg(static_cast<const float *>(x) + i)
+           : type == W4J_GGML_F16 ? __half2float(__ldg(static_cast<const __half *>(x) + i))
+                                  : __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(x) + i));
+}
+
+template <int MT, typename T, int EPI>
+__global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_layer(LinearI8Args a, QuantizeArgs in) {
+    extern __shared__ __align__(16) int8_t sq[];  // [M][K rounded up to 16]
+    __shared__ uint32_t sm[kFewWarps];
+    __shared__ float sxs[MT];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = blockIdx.x * kFewWarps + warp;
+    const int K = a.K, units = (K + 15) / 16, k16 = 16 * units;
+    const int8_t *w = a.w + (long long)n * a.ldw;
+    if (n < a.N)  // into L2 only: the weights may be what the kernel before this one writes
+        for (int k = lane * 128; k < K; k += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(w + k));
+    pdl_wait();
+    constexpr int U = 4, E = 8;
+    uint4 v[U];
+    auto weights = [&](int u0) {
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            v[i] = n < a.N && u0 + 32 * i < units ? __ldg(reinterpret_cast<const uint4 *>(w) + u0 + 32 * i) : make_uint4(0, 0, 0, 0);
+    };
+    weights(lane);
+    // row `row` by `per` warps; the first E of a thread's elements stay in registers
+    constexpr int per = kFewWarps / MT, nt = 32 * per;
+    const int row = warp / per, t = tid % nt, rows = min(MT, a.M);
+    const long long x0 = (long long)min(row, rows - 1) * in.ldx;
+    float c[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) c[e] = t + e * nt < K ? load1(in.x, in.type, x0 + t + e * nt) : 0.f;
+    auto pass = [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (t + e * nt < K) f(t + e * nt, c[e]);
+        for (int k = t + E * nt; k < K; k += nt) f(k, load1(in.x, in.type, x0 + k));
+    };
+    auto reduce = [&](auto r, auto op) {
+        using R = decltype(r);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) r = op(r, __shfl_xor_sync(0xffffffffu, r, o));
+        if (per == 1) return r;
+        R *to = reinterpret_cast<R *>(sm);
+        __syncthreads();
+        if (lane == 0) to[warp] = r;
+        __syncthreads();
+        r = to[row * per];
+#pragma unroll
+        for (int i = 1; i < per; ++i) r = op(r, to[row * per + i]);
+        return r;
+    };
+    auto add = [](float p, float q) { return p + q; };
+    float mean = 0.f, rstd = 1.f;
+    if (in.ln_g) {
+        float sum = 0.f, sum2 = 0.f;
+        pass([&](int, float x) { sum += x; });
+        mean = reduce(sum, add) / K;
+        pass([&](int, float x) { sum2 += (x - mean) * (x - mean); });
+        rstd = 1.f / sqrtf(reduce(sum2, add) / K + 1e-5f);
+    }
+    auto value = [&](int k, float x) { return in.ln_g ? (x - mean) * rstd * __ldg(in.ln_g + k) + __ldg(in.ln_b + k) : x; };
+    uint32_t bits = 0;  // the largest magnitude by its bits: an infinity or a NaN is above every number
+    pass([&](int k, float x) { bits = max(bits, __float_as_uint(value(k, x)) & 0x7fffffffu); });
+    bits = reduce(bits, [](uint32_t p, uint32_t q) { return max(p, q); });
+    const bool good = bits < 0x7f800000u;
+    Step p;
+    p.s = __fdiv_rn(__uint_as_float(bits), 127.f);
+    p.tiny = p.s < 1e-30f, p.up = p.tiny ? 18446744073709551616.f : 1.f, p.inv = __fdiv_rn(1.f, p.s * p.up);
+    if (row < rows) {
+        if (t == 0) sxs[row] = good ? p.s : __int_as_float(0x7fffffff);
+        int8_t *q = sq + row * k16;
+        pass([&](int k, float x) {
+            x = value(k, x);
+            const float y = fmaf(x, p.inv, 12582912.f);
+            int r = (int)(__float_as_uint(y) & 0xffu);
+            if (p.tiny || fabsf(fmaf(12582912.f - y, p.s, x)) >= 0.5f * p.s) r = nearest(x * p.up, p.s * p.up, p.inv);
+            q[k] = (int8_t)(good && p.s > 0.f ? r : 0);
+        });
+        for (int k = K + t; k < k16; k += nt) q[k] = 0;
+    }
+    __syncthreads();
+    int acc[MT] = {};
+    for (int u0 = lane;;) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (m >= rows) break;
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (u0 + 32 * i >= units) break;
+                const uint4 x = *reinterpret_cast<const uint4 *>(sq + m * k16 + 16 * (u0 + 32 * i));
+                acc[m] = __dp4a((int)v[i].x, (int)x.x, acc[m]), acc[m] = __dp4a((int)v[i].y, (int)x.y, acc[m]);
+                acc[m] = __dp4a((int)v[i].z, (int)x.z, acc[m]), acc[m] = __dp4a((int)v[i].w, (int)x.w, acc[m]);
+            }
+        }
+        u0 += 32 * U;
+        if (u0 - lane >= units) break;
+        weights(u0);
+    }
+    if (n >= a.N) return;
+    const float ws = __ldg(a.ws + n), b = a.bias ? __ldg(a.bias + n) : 0.f;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
+        if (m < rows && lane == m) finish<T, EPI>(acc[m], sxs[m], ws, b, reinterpret_cast<T *>(a.y) + (long long)m * a.ldy + n);
+    }
+}
+
 // ---------------------------------------------------------------------------
 // many rows: a pair of SMs owns 256 channels x 256 tokens at a time (tcgen05.mma with cta_group::2), each with 128 of the
 // channels and half of the tokens in its shared memory, so that a tile's operands cross from L2 once: 64 bytes a cycle
@@ -766,6 +879,21 @@ cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
     return product<128, T, EPI>(a, s);
 }
 
+template <typename T, int EPI>
+cudaError_t layer(const LinearI8Args &a, const QuantizeArgs &q, cudaStream_t s) {
+    const unsigned blocks = (a.N + kFewWarps - 1) / kFewWarps;
+    const size_t smem = (size_t)a.M * ((a.K + 15) / 16 * 16);
+    if (a.M == 1) return launch_after(k_linear_i8_layer<1, T, EPI>, blocks, kFewWarps * 32, smem, s, 1, a, q);
+    if (a.M == 2) return launch_after(k_linear_i8_layer<2, T, EPI>, blocks, kFewWarps * 32, smem, s, 1, a, q);
+    if (a.M <= 4) return launch_after(k_linear_i8_layer<4, T, EPI>, blocks, kFewWarps * 32, smem, s, 1, a, q);
+    return launch_after(k_linear_i8_layer<8, T, EPI>, blocks, kFewWarps * 32, smem, s, 1, a, q);
+}
+
+template <typename T>
+cudaError_t layer(const LinearI8Args &a, const QuantizeArgs &q, cudaStream_t s) {
+    return a.epilogue == 0 ? layer<T, 0>(a, q, s) : a.epilogue == 1 ? layer<T, 1>(a, q, s) : layer<T, 2>(a, q, s);
+}
+
 template <typename T>
 cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
     return a.epilogue == 0 ? product<T, 0>(a, s) : a.epilogue == 1 ? product<T, 1>(a, s) : product<T, 2>(a, s);
@@ -781,6 +909,24 @@ cudaError_t launch_quantize_rows(const QuantizeArgs &a, cudaStream_t s) {
 cudaError_t launch_linear_i8(const LinearI8Args &a, cudaStream_t s) {
     return a.type == W4J_GGML_F32 ? product<float>(a, s) : a.type == W4J_GGML_F16 ? product<__half>(a, s)
                                                                                  : product<__nv_bfloat16>(a, s);
+}
+
+size_t linear_i8_layer_work(int M, int K) {
+    const size_t k16 = ((size_t)K + 15) / 16 * 16;
+    return M <= kFewRows && M * k16 <= kLayerSmem ? 0 : M * (k16 + 4);
+}
+
+cudaError_t launch_linear_i8_layer(LinearI8Args a, QuantizeArgs q, void *work, cudaStream_t s) {
+    if (linear_i8_layer_work(a.M, a.K) == 0)
+        return a.type == W4J_GGML_F32 ? layer<float>(a, q, s) : a.type == W4J_GGML_F16 ? layer<__half>(a, q, s)
+                                                                                      : layer<__nv_bfloat16>(a, q, s);
+    // the integers, then the rows' scales
+    q.ldq = a.ldx = ((long long)a.K + 15) / 16 * 16;
+    q.q = static_cast<int8_t *>(work);
+    q.scale = reinterpret_cast<float *>(q.q + a.M * q.ldq);
+    a.x = q.q, a.xs = q.scale;
+    const cudaError_t e = launch_quantize_rows(q, s);
+    return e == cudaSuccess ? launch_linear_i8(a, s) : e;
 }
 
 }  // namespace w4j

@@ -28,4 +28,8 @@ struct LinearI8Args {
 cudaError_t launch_quantize_rows(const QuantizeArgs &a, cudaStream_t s);
 cudaError_t launch_linear_i8(const LinearI8Args &a, cudaStream_t s);
 
+// both in one; `work`: linear_i8_layer_work bytes (0 for a few rows, which take one launch)
+size_t linear_i8_layer_work(int M, int K);
+cudaError_t launch_linear_i8_layer(LinearI8Args a, QuantizeArgs q, void *work, cudaStream_t s);
+
 }  // namespace w4j

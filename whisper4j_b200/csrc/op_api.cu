@@ -177,18 +177,36 @@ extern "C" int w4j_op_attn_shared(const w4j_attn_shared *x, void *stream) {
 
 static bool float_type(int t) { return t == W4J_GGML_F32 || t == W4J_GGML_F16 || t == W4J_GGML_BF16; }
 
+static int check_rows(const char *who, const void *x, int x_type, int M, int K, int64_t ldx, const float *ln_g, const float *ln_b) {
+    if (!float_type(x_type)) return set_err(W4J_ERR_ARG, "%s: x_type must be F32 (0), F16 (1) or BF16 (30), not %d", who, x_type);
+    if (M < 1 || K < 1 || M > 1 << 24 || K > 1 << 24) return set_err(W4J_ERR_ARG, "%s: bad shape (%d x %d)", who, M, K);
+    if (ldx < K) return set_err(W4J_ERR_ARG, "%s: ldx must be at least K", who);
+    if (!aligned(x, x_type == W4J_GGML_F32 ? 4 : 2)) return set_err(W4J_ERR_ARG, "%s: x must be aligned to its type", who);
+    if ((ln_g == nullptr) != (ln_b == nullptr)) return set_err(W4J_ERR_ARG, "LayerNorm needs both gamma and beta");
+    return W4J_OK;
+}
+
+static int check_product(const char *who, int M, int K, const int8_t *w, int64_t ldw, int N, int epilogue, const void *y, int y_type,
+                         int64_t ldy) {
+    if (!float_type(y_type)) return set_err(W4J_ERR_ARG, "%s: y_type must be F32 (0), F16 (1) or BF16 (30), not %d", who, y_type);
+    if (M < 1 || N < 1 || K < 1 || M > 1 << 24 || N > 1 << 24) return set_err(W4J_ERR_ARG, "%s: bad shape (%d x %d x %d)", who, M, K, N);
+    if (K > 131056) return set_err(W4J_ERR_ARG, "%s: K = %d: sums of more than 131056 products may leave 32 bits", who, K);
+    if (ldw < K || ldw % 16 || !aligned(w, 16))
+        return set_err(W4J_ERR_ARG, "%s: w must be 16-byte aligned with rows a multiple of 16 bytes of at least K apart", who);
+    if (ldy < N || !aligned(y, y_type == W4J_GGML_F32 ? 4 : 2))
+        return set_err(W4J_ERR_ARG, "%s: y must be aligned to its type with ldy at least N", who);
+    if (epilogue < 0 || epilogue > 2) return set_err(W4J_ERR_ARG, "epilogue must be 0, 1 or 2");
+    return W4J_OK;
+}
+
 extern "C" int w4j_op_quantize_rows(int device, const void *x, int x_type, int M, int K, int64_t ldx, const float *ln_g,
                                     const float *ln_b, int8_t *q, int64_t ldq, float *scale, void *stream) {
     const char *who = "w4j_op_quantize_rows";
     if (!x || !q || !scale) return set_err(W4J_ERR_ARG, "%s: null argument", who);
-    if (!float_type(x_type)) return set_err(W4J_ERR_ARG, "%s: x_type must be F32 (0), F16 (1) or BF16 (30), not %d", who, x_type);
-    if (M < 1 || K < 1 || K > 1 << 24) return set_err(W4J_ERR_ARG, "%s: bad shape (%d x %d)", who, M, K);
-    if (ldx < K) return set_err(W4J_ERR_ARG, "%s: ldx must be at least K", who);
+    TRY(check_rows(who, x, x_type, M, K, ldx, ln_g, ln_b));
     if (ldq < K || ldq % 16 || !aligned(q, 16))
         return set_err(W4J_ERR_ARG, "%s: q must be 16-byte aligned with ldq a multiple of 16 of at least K", who);
-    if (!aligned(x, x_type == W4J_GGML_F32 ? 4 : 2) || !aligned(scale, 4))
-        return set_err(W4J_ERR_ARG, "%s: x and scale must be aligned to their type", who);
-    if ((ln_g == nullptr) != (ln_b == nullptr)) return set_err(W4J_ERR_ARG, "LayerNorm needs both gamma and beta");
+    if (!aligned(scale, 4)) return set_err(W4J_ERR_ARG, "%s: scale must be aligned to its type", who);
     DeviceGuard g(device);
     TRY(g.rc());
     CUDA_TRY(launch_quantize_rows(QuantizeArgs{x, x_type, M, K, ldx, ln_g, ln_b, q, ldq, scale}, stream_of(stream)));
@@ -200,17 +218,38 @@ extern "C" int w4j_op_linear_i8(int device, const int8_t *x, int64_t ldx, const 
                                 void *y, int y_type, int64_t ldy, void *stream) {
     const char *who = "w4j_op_linear_i8";
     if (!x || !x_scale || !w || !w_scale || !y) return set_err(W4J_ERR_ARG, "%s: null argument", who);
-    if (!float_type(y_type)) return set_err(W4J_ERR_ARG, "%s: y_type must be F32 (0), F16 (1) or BF16 (30), not %d", who, y_type);
-    if (M < 1 || N < 1 || K < 1 || M > 1 << 24 || N > 1 << 24) return set_err(W4J_ERR_ARG, "%s: bad shape (%d x %d x %d)", who, M, K, N);
-    if (K > 131056) return set_err(W4J_ERR_ARG, "%s: K = %d: sums of more than 131056 products may leave 32 bits", who, K);
-    if (ldx < K || ldw < K || ldx % 16 || ldw % 16 || !aligned(x, 16) || !aligned(w, 16))
-        return set_err(W4J_ERR_ARG, "%s: x and w must be 16-byte aligned with rows a multiple of 16 bytes of at least K apart", who);
-    if (ldy < N || !aligned(y, y_type == W4J_GGML_F32 ? 4 : 2))
-        return set_err(W4J_ERR_ARG, "%s: y must be aligned to its type with ldy at least N", who);
-    if (epilogue < 0 || epilogue > 2) return set_err(W4J_ERR_ARG, "epilogue must be 0, 1 or 2");
+    TRY(check_product(who, M, K, w, ldw, N, epilogue, y, y_type, ldy));
+    if (ldx < K || ldx % 16 || !aligned(x, 16))
+        return set_err(W4J_ERR_ARG, "%s: x must be 16-byte aligned with rows a multiple of 16 bytes of at least K apart", who);
     DeviceGuard g(device);
     TRY(g.rc());
     CUDA_TRY(launch_linear_i8(LinearI8Args{x, w, ldx, ldw, x_scale, w_scale, bias, M, N, K, epilogue, y_type, y, ldy},
                               stream_of(stream)));
+    return W4J_OK;
+}
+
+extern "C" size_t w4j_op_linear_i8_layer_workspace(int M, int K) {
+    if (M < 1 || K < 1 || M > 1 << 24 || K > 131056) {
+        set_err(W4J_ERR_ARG, "w4j_op_linear_i8_layer_workspace: bad shape (%d x %d)", M, K);
+        return 0;
+    }
+    return linear_i8_layer_work(M, K);
+}
+
+extern "C" int w4j_op_linear_i8_layer(int device, const void *x, int x_type, int64_t ldx, const float *ln_g, const float *ln_b, int M,
+                                      int K, const int8_t *w, int64_t ldw, const float *w_scale, int N, const float *bias,
+                                      int epilogue, void *y, int y_type, int64_t ldy, void *work, size_t work_bytes, void *stream) {
+    const char *who = "w4j_op_linear_i8_layer";
+    if (!x || !w || !w_scale || !y) return set_err(W4J_ERR_ARG, "%s: null argument", who);
+    TRY(check_rows(who, x, x_type, M, K, ldx, ln_g, ln_b));
+    TRY(check_product(who, M, K, w, ldw, N, epilogue, y, y_type, ldy));
+    const size_t need = linear_i8_layer_work(M, K);
+    if (need && (!work || !aligned(work, 16) || work_bytes < need))
+        return set_err(W4J_ERR_ARG, "%s: work must be 16-byte aligned and hold the %zu bytes that w4j_op_linear_i8_layer_workspace asks for",
+                       who, need);
+    DeviceGuard g(device);
+    TRY(g.rc());
+    CUDA_TRY(launch_linear_i8_layer(LinearI8Args{nullptr, w, 0, ldw, nullptr, w_scale, bias, M, N, K, epilogue, y_type, y, ldy},
+                                    QuantizeArgs{x, x_type, M, K, ldx, ln_g, ln_b, nullptr, 0, nullptr}, work, stream_of(stream)));
     return W4J_OK;
 }

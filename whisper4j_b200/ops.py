@@ -278,11 +278,9 @@ class Int8Linear:
         if not m:
             return out
         g, b = _norm(ln, k, index)
-        stream, k16 = _raw_stream(index), self._k16
-        work = torch.empty(m * (k16 + 4), dtype=torch.int8, device=x.device)  # the integers, then the rows' scales
-        q = work.data_ptr()
-        xs = q + m * k16
-        check(self._lib.w4j_op_quantize_rows(index, x.data_ptr(), _TYPES[x.dtype], m, k, ldx, g, b, q, k16, xs, stream))
-        check(self._lib.w4j_op_linear_i8(index, q, k16, xs, m, k, self._weight, k16, self._scale, self.n, self._bias, code,
-                                         out.data_ptr(), _TYPES[out.dtype], ldy, stream))
+        n_bytes = self._lib.w4j_op_linear_i8_layer_workspace(m, k)
+        work = torch.empty(n_bytes, dtype=torch.int8, device=x.device) if n_bytes else None
+        check(self._lib.w4j_op_linear_i8_layer(index, x.data_ptr(), _TYPES[x.dtype], ldx, g, b, m, k, self._weight, self._k16,
+                                               self._scale, self.n, self._bias, code, out.data_ptr(), _TYPES[out.dtype], ldy,
+                                               work.data_ptr() if n_bytes else None, n_bytes, _raw_stream(index)))
         return out
