@@ -148,7 +148,7 @@ def refused(c, m, text, call):
     same(c, m)  # nothing has changed, and the next call goes on
 
 
-@pytest.mark.parametrize("n_rows", [8, 5000])
+@pytest.mark.parametrize("n_rows", [8, 5000, 30000])
 def test_calls_that_cannot_be_done_change_nothing(n_rows):
     c, m = new_cache(n_rows=n_rows, n_pages=10)
     grow(c, m, [0, 1], [70, 20])  # 5 + 2 pages of 10

@@ -45,11 +45,30 @@ class DeviceGuard {
     int before_ = -1, rc_ = W4J_OK;
 };
 
+// Once for each device: lets a kernel use all of the opt-in shared memory beside its static arrays.
+template <auto Kern>
+inline cudaError_t prepare() {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0, optin = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    cudaFuncAttributes fa;
+    if ((e = cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev)) != cudaSuccess) return e;
+    if ((e = cudaFuncGetAttributes(&fa, Kern)) != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, optin - (int)fa.sharedSizeBytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+
 // Launch with programmatic dependent launch: the kernel may be scheduled while its predecessor in the
 // stream still runs, so every one of its threads executes griddepcontrol.wait before it touches global
 // memory that the predecessor may write or still read.
-template <typename Kern, typename... Args>
-inline cudaError_t launch_after(Kern kern, dim3 grid, dim3 block, size_t smem, cudaStream_t s, int cluster, Args... args) {
+template <auto Kern, typename... Args>
+inline cudaError_t launch_after(dim3 grid, dim3 block, size_t smem, cudaStream_t s, int cluster, Args... args) {
+    const cudaError_t e = prepare<Kern>();
+    if (e != cudaSuccess) return e;
     cudaLaunchAttribute at[2];
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
@@ -66,21 +85,7 @@ inline cudaError_t launch_after(Kern kern, dim3 grid, dim3 block, size_t smem, c
         at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
         cfg.numAttrs = 2;
     }
-    return cudaLaunchKernelEx(&cfg, kern, args...);
-}
-
-// Lets a kernel use `bytes` of dynamic shared memory on the current device, once for each device.
-template <auto Kern>
-inline cudaError_t allow_smem(size_t bytes) {
-    static std::atomic<uint64_t> done{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
-    e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
-    return e;
+    return cudaLaunchKernelEx(&cfg, Kern, args...);
 }
 
 }  // namespace w4j

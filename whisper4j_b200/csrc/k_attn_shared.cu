@@ -776,6 +776,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_attn_shared_join(AttnSharedArgs a) {
     pdl_wait();
+    pdl_trigger();
     const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (r >= (long long)a.n_seq * a.n_query * a.n_head) return;
@@ -827,8 +828,7 @@ cudaError_t launch(const AttnSharedArgs &a, cudaStream_t s) {
     if (a.tc_tiles) {
         const int box = maps(kTcKeys);
         if (!box) return cudaErrorInvalidValue;
-        if ((e = allow_smem<k_attn_shared_tc<T, D>>(tc_smem(D))) != cudaSuccess) return e;
-        e = launch_after(k_attn_shared_tc<T, D>, a.tc_tiles * a.shared_splits * p.n_kv_head, kTcThreads, tc_smem(D), s, 1, km, vm,
+        e = launch_after<k_attn_shared_tc<T, D>>(a.tc_tiles * a.shared_splits * p.n_kv_head, kTcThreads, tc_smem(D), s, 1, km, vm,
                          a, box);
         if (e != cudaSuccess) return e;
     }
@@ -836,14 +836,12 @@ cudaError_t launch(const AttnSharedArgs &a, cudaStream_t s) {
     if (!box) return cudaErrorInvalidValue;
     const unsigned blocks = (a.shared_items + a.own_items + kAsWarps - 1) / kAsWarps;
     if (a.tile_rows == 8) {
-        if ((e = allow_smem<k_attn_shared<T, D, 1>>(kAsSmem)) != cudaSuccess) return e;
-        e = launch_after(k_attn_shared<T, D, 1>, blocks, kAsWarps * 32, kAsSmem, s, 1, km, vm, a, box);
+        e = launch_after<k_attn_shared<T, D, 1>>(blocks, kAsWarps * 32, kAsSmem, s, 1, km, vm, a, box);
     } else {
-        if ((e = allow_smem<k_attn_shared<T, D, 2>>(kAsSmem)) != cudaSuccess) return e;
-        e = launch_after(k_attn_shared<T, D, 2>, blocks, kAsWarps * 32, kAsSmem, s, 1, km, vm, a, box);
+        e = launch_after<k_attn_shared<T, D, 2>>(blocks, kAsWarps * 32, kAsSmem, s, 1, km, vm, a, box);
     }
     if (e != cudaSuccess) return e;
-    return launch_after(k_attn_shared_join<T, D>, (unsigned)((rows + 7) / 8), 256, 0, s, 1, a);
+    return launch_after<k_attn_shared_join<T, D>>((unsigned)((rows + 7) / 8), 256, 0, s, 1, a);
 }
 
 }  // namespace

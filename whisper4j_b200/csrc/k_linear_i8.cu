@@ -197,18 +197,18 @@ cudaError_t quantize(const QuantizeArgs &a, cudaStream_t s) {
     const bool whole = at % 16 == 0 && a.K % V == 0 && a.ldx % V == 0;
     if (a.M >= 148 * 4 * 2 && c <= 16 && whole) {
         const unsigned blocks = (a.M + 3) / 4;
-        if (c <= 4) return launch_after(k_quantize_rows<T, 4, true>, blocks, 128, 0, s, 1, a);
-        if (c <= 8) return launch_after(k_quantize_rows<T, 8, true>, blocks, 128, 0, s, 1, a);
-        if (c <= 12) return launch_after(k_quantize_rows<T, 12, true>, blocks, 128, 0, s, 1, a);
-        return launch_after(k_quantize_rows<T, 16, true>, blocks, 128, 0, s, 1, a);
+        if (c <= 4) return launch_after<k_quantize_rows<T, 4, true>>(blocks, 128, 0, s, 1, a);
+        if (c <= 8) return launch_after<k_quantize_rows<T, 8, true>>(blocks, 128, 0, s, 1, a);
+        if (c <= 12) return launch_after<k_quantize_rows<T, 12, true>>(blocks, 128, 0, s, 1, a);
+        return launch_after<k_quantize_rows<T, 16, true>>(blocks, 128, 0, s, 1, a);
     }
     const int most = a.M >= 148 * 4 ? 256 : kQMax, held = (units + most - 1) / most;
     const int threads = held <= 4 ? (units + held - 1) / held : most, block = (threads + 31) / 32 * 32;
-    if (!whole) return launch_after(k_quantize_rows<T, 0, false>, a.M, block, 0, s, 1, a);
-    if (held == 1) return launch_after(k_quantize_rows<T, 1, false>, a.M, block, 0, s, 1, a);
-    if (held == 2) return launch_after(k_quantize_rows<T, 2, false>, a.M, block, 0, s, 1, a);
-    if (held <= 4) return launch_after(k_quantize_rows<T, 4, false>, a.M, block, 0, s, 1, a);
-    return launch_after(k_quantize_rows<T, 0, false>, a.M, block, 0, s, 1, a);
+    if (!whole) return launch_after<k_quantize_rows<T, 0, false>>(a.M, block, 0, s, 1, a);
+    if (held == 1) return launch_after<k_quantize_rows<T, 1, false>>(a.M, block, 0, s, 1, a);
+    if (held == 2) return launch_after<k_quantize_rows<T, 2, false>>(a.M, block, 0, s, 1, a);
+    if (held <= 4) return launch_after<k_quantize_rows<T, 4, false>>(a.M, block, 0, s, 1, a);
+    return launch_after<k_quantize_rows<T, 0, false>>(a.M, block, 0, s, 1, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -324,6 +324,7 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
         failed = issued = 0;
     }
     pdl_wait();  // before the tensor memory: a kernel that waits must not hold what the one before it may need
+    pdl_trigger();
     if (warp == 1) tmem_alloc(&slot, kCols), tmem_relinquish();
     tc_fence_before();
     __syncthreads();
@@ -434,6 +435,7 @@ template <int MT, typename T, int EPI>
 __global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_few(LinearI8Args a) {
     const int n = blockIdx.x * kFewWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31, units = (a.K + 15) / 16;
     pdl_wait();
+    pdl_trigger();
     if (n >= a.N) return;
     const uint4 *w = reinterpret_cast<const uint4 *>(a.w + (long long)n * a.ldw);
     const float ws = __ldg(a.ws + n), b = a.bias ? __ldg(a.bias + n) : 0.f;
@@ -485,6 +487,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_layer(LinearI8Args
     if (n < a.N)  // into L2 only: the weights may be what the kernel before this one writes
         for (int k = lane * 128; k < K; k += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(w + k));
     pdl_wait();
+    pdl_trigger();
     constexpr int U = 4, E = 8;
     uint4 v[U];
     auto weights = [&](int u0) {
@@ -831,9 +834,7 @@ cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
     // k is split while the tiles leave SMs idle and every block keeps two stages of k
     int ks = 1;
     while (ks < 8 && tiles * ks * 2 <= 148 && kb >= 4 * ks) ks *= 2;
-    cudaError_t e = allow_smem<k_linear_i8<NT, T, EPI>>(mm_smem(NT));
-    if (e != cudaSuccess) return e;
-    return launch_after(k_linear_i8<NT, T, EPI>, (unsigned)(tiles * ks), kMmThreads, mm_smem(NT), s, ks, wmap, xmap, a, ks,
+    return launch_after<k_linear_i8<NT, T, EPI>>((unsigned)(tiles * ks), kMmThreads, mm_smem(NT), s, ks, wmap, xmap, a, ks,
                         (int)token_tiles);
 }
 
@@ -847,19 +848,16 @@ cudaError_t product_pair(const LinearI8Args &a, cudaStream_t s) {
     const long long tiles = (long long)((a.N + 255) / 256) * token_tiles;
     if (tiles > 0x7fffffff) return cudaErrorInvalidValue;
     const unsigned blocks = 2 * (unsigned)(tiles < 74 ? tiles : 74);
-    cudaError_t e;
     CUtensorMap ymap = {};
     // (a box that ends inside 16 bytes of y would write all of them: then the last channel has to end on their border)
     if (EPI != 2 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.ldy * sizeof(T) % 16 == 0 && a.N * sizeof(T) % 16 == 0) {
         const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                          : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
         if (!tmap_2d(&ymap, type, a.y, a.M, a.N, a.ldy * sizeof(T), 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE)) return cudaErrorInvalidValue;
-        if ((e = allow_smem<k_linear_i8_pair<T, EPI, true>>(pr_smem(sizeof(T)))) != cudaSuccess) return e;
-        return launch_after(k_linear_i8_pair<T, EPI, true>, blocks, kPrThreads, pr_smem(sizeof(T)), s, 2, wmap, xmap, ymap, a, token_tiles,
+        return launch_after<k_linear_i8_pair<T, EPI, true>>(blocks, kPrThreads, pr_smem(sizeof(T)), s, 2, wmap, xmap, ymap, a, token_tiles,
                             (int)tiles);
     }
-    if ((e = allow_smem<k_linear_i8_pair<T, EPI, false>>(pr_smem(sizeof(T)))) != cudaSuccess) return e;
-    return launch_after(k_linear_i8_pair<T, EPI, false>, blocks, kPrThreads, pr_smem(sizeof(T)), s, 2, wmap, xmap, ymap, a, token_tiles,
+    return launch_after<k_linear_i8_pair<T, EPI, false>>(blocks, kPrThreads, pr_smem(sizeof(T)), s, 2, wmap, xmap, ymap, a, token_tiles,
                         (int)tiles);
 }
 
@@ -868,9 +866,9 @@ constexpr int kFewRows = 8;
 template <typename T, int EPI>
 cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
     const unsigned few = (a.N + kFewWarps - 1) / kFewWarps;
-    if (a.M == 1) return launch_after(k_linear_i8_few<1, T, EPI>, few, kFewWarps * 32, 0, s, 1, a);
-    if (a.M <= 4) return launch_after(k_linear_i8_few<4, T, EPI>, few, kFewWarps * 32, 0, s, 1, a);
-    if (a.M <= kFewRows) return launch_after(k_linear_i8_few<8, T, EPI>, few, kFewWarps * 32, 0, s, 1, a);
+    if (a.M == 1) return launch_after<k_linear_i8_few<1, T, EPI>>(few, kFewWarps * 32, 0, s, 1, a);
+    if (a.M <= 4) return launch_after<k_linear_i8_few<4, T, EPI>>(few, kFewWarps * 32, 0, s, 1, a);
+    if (a.M <= kFewRows) return launch_after<k_linear_i8_few<8, T, EPI>>(few, kFewWarps * 32, 0, s, 1, a);
     if (a.M <= 16) return product<16, T, EPI>(a, s);
     if (a.M <= 32) return product<32, T, EPI>(a, s);
     if (a.M <= 64) return product<64, T, EPI>(a, s);
@@ -883,10 +881,10 @@ template <typename T, int EPI>
 cudaError_t layer(const LinearI8Args &a, const QuantizeArgs &q, cudaStream_t s) {
     const unsigned blocks = (a.N + kFewWarps - 1) / kFewWarps;
     const size_t smem = (size_t)a.M * ((a.K + 15) / 16 * 16);
-    if (a.M == 1) return launch_after(k_linear_i8_layer<1, T, EPI>, blocks, kFewWarps * 32, smem, s, 1, a, q);
-    if (a.M == 2) return launch_after(k_linear_i8_layer<2, T, EPI>, blocks, kFewWarps * 32, smem, s, 1, a, q);
-    if (a.M <= 4) return launch_after(k_linear_i8_layer<4, T, EPI>, blocks, kFewWarps * 32, smem, s, 1, a, q);
-    return launch_after(k_linear_i8_layer<8, T, EPI>, blocks, kFewWarps * 32, smem, s, 1, a, q);
+    if (a.M == 1) return launch_after<k_linear_i8_layer<1, T, EPI>>(blocks, kFewWarps * 32, smem, s, 1, a, q);
+    if (a.M == 2) return launch_after<k_linear_i8_layer<2, T, EPI>>(blocks, kFewWarps * 32, smem, s, 1, a, q);
+    if (a.M <= 4) return launch_after<k_linear_i8_layer<4, T, EPI>>(blocks, kFewWarps * 32, smem, s, 1, a, q);
+    return launch_after<k_linear_i8_layer<8, T, EPI>>(blocks, kFewWarps * 32, smem, s, 1, a, q);
 }
 
 template <typename T>

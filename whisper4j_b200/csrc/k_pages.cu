@@ -10,7 +10,8 @@
 // over `ref` with a cluster barrier between them (barrier.cluster, no grid barrier and no second launch),
 // the free list by prefix sums over slices of `ref`.  The tokens are moved by a second kernel on all SMs
 // from a list of (source, destination, tokens) that the first one leaves.  The first is bound by the
-// latency of its four or five dependent passes over L2, the second by HBM.
+// latency of its dependent passes over L2, the second by HBM.  A call whose lists fit one block's registers and
+// shared memory takes one block that reads everything once (k_pages_small): three passes instead of five.
 //
 // Every call is all or nothing: the cluster checks all rows, lengths and the number of free pages before
 // its first write, and a call that cannot be done raises a bit of `status` and changes nothing else.
@@ -389,12 +390,270 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_compact(PagesArgs p, int
 }
 
 // ---------------------------------------------------------------------------
+// the same calls by one block: the call's lists, the marks of the rows and the free list in shared memory, `ref` (kRefs
+// neighbouring pages a thread) and the tables' entries (32 neighbouring ones a warp and step, kEntries steps) in
+// registers, each read once.  As many warps as that takes and no more: with all 32 every instruction holds a scheduler
+// for eight cycles (a beam reorder of 5 rows: 8.4 us with 1024 threads, @SMALL@ with as many as it needs).
+// ---------------------------------------------------------------------------
+enum PagesOp { OP_FORK, OP_EXTEND, OP_FREE, OP_COMPACT };
+constexpr int kSmallThreads = 1024, kRefs = 8, kEntries = 12;
+
+// Exclusive prefix sum over the block's threads.
+__device__ __forceinline__ int small_scan(int v, int *sm, int &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();  // the last call's sums have been read
+    if (lane == 31) sm[warp] = x;
+    __syncthreads();
+    int y = lane < (int)blockDim.x / 32 ? sm[lane] : 0;
+    const int mine = y;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int z = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) y += z;
+    }
+    total = __shfl_sync(0xffffffffu, y, 31);
+    return __shfl_sync(0xffffffffu, y - mine, warp) + x - v;
+}
+
+struct SmallRows {  // of the n rows of a call, and of all rows
+    int *a, *b, *len_a, *len_b, *rank, *mark, *owner, *list, *more;  // more: what the call adds to each page's count
+    __device__ SmallRows(int *sm, int n, int n_rows, int n_pages) {
+        a = sm, b = a + n, len_a = b + n, len_b = len_a + n, rank = len_b + n, mark = rank + n, owner = mark + n_rows, list = owner + n_rows;
+        more = list + n_pages;
+    }
+};
+size_t small_bytes(const PagesArgs &p, int n) { return 4 * (5 * (size_t)n + 2 * (size_t)p.n_rows + 2 * (size_t)p.n_pages); }
+
+// a, b: dst and src (fork), rows and start (extend), rows (free), n_live (compact: the call's rows are all of them)
+template <PagesOp OP>
+__global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, const int *__restrict__ a, const int *__restrict__ b,
+                                                               int *live_out, int n) {
+    extern __shared__ int dyn[];
+    __shared__ int sm[32], bad;
+    const Work w(p);
+    const SmallRows s(dyn, n, p.n_rows, p.n_pages);
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, T = p.page_tokens, W = p.width;
+    // step x of a warp: 32 entries (runs of 32 in each row) of row i from j0 on
+    const int runs = (W + 31) / 32, steps = n * runs, warps = threads / 32;
+    auto row_of = [&](int step, int &j) {
+        const int i = runs == 1 ? step : step / runs;
+        j = (step - i * runs) * 32 + lane;
+        return i;
+    };
+    pdl_wait();
+    pdl_trigger();
+    int ref[kRefs];
+    if (tid * kRefs + kRefs <= p.n_pages && reinterpret_cast<uintptr_t>(p.ref) % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < kRefs; i += 4) *reinterpret_cast<int4 *>(ref + i) = *reinterpret_cast<const int4 *>(p.ref + tid * kRefs + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kRefs; ++i) ref[i] = tid * kRefs + i < p.n_pages ? p.ref[tid * kRefs + i] : 1;
+    }
+    if (OP != OP_COMPACT) {
+        for (int i = tid; i < n; i += threads) {
+            s.a[i] = a[i];
+            if (OP != OP_FREE) s.b[i] = b[i];
+        }
+        for (int i = tid; i < p.n_rows; i += threads) s.mark[i] = -1, s.owner[i] = 0x7fffffff;
+        for (int i = tid; i < p.n_pages; i += threads) s.more[i] = 0;
+    }
+    if (tid == 0) bad = OP == OP_EXTEND && b[0] != 0 ? W4J_PAGES_BAD_START : 0, w.head[H_PAIRS] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += threads) {
+        const int r = OP == OP_COMPACT ? i : s.a[i];
+        if (r < 0 || r >= p.n_rows || (OP != OP_COMPACT && atomicExch(s.mark + r, i) != -1)) {
+            atomicOr(&bad, W4J_PAGES_BAD_ROW);
+            s.len_a[i] = s.len_b[i] = 0;
+            continue;
+        }
+        s.len_a[i] = row_len(p, r);
+        if (OP == OP_FORK) {
+            const int from = s.b[i];
+            if (from < -1 || from >= p.n_rows) atomicOr(&bad, W4J_PAGES_BAD_ROW);
+            const bool ok = from >= 0 && from < p.n_rows;
+            if (ok) atomicMin(s.owner + from, i);
+            s.len_b[i] = ok ? row_len(p, from) : 0;
+        }
+        if (OP == OP_EXTEND) {
+            const long long add = (long long)(i + 1 < n ? s.b[i + 1] : b[n]) - s.b[i], len = s.len_a[i] + add;
+            if (add < 0) atomicOr(&bad, W4J_PAGES_BAD_START);
+            if (len > (long long)W * T) atomicOr(&bad, W4J_PAGES_TOO_LONG);
+            s.len_b[i] = add < 0 || len > (long long)W * T ? s.len_a[i] : (int)len;
+        }
+    }
+    __syncthreads();
+    // what row a holds at the entries of this thread's steps, and what it shall hold (-1: nothing): all of them on
+    // their way before the first is looked at
+    int was[kEntries], shall[kEntries];
+#pragma unroll
+    for (int x = 0; x < kEntries; ++x) {
+        was[x] = shall[x] = -1;
+        const int step = tid / 32 + x * warps;
+        if (OP == OP_EXTEND || step >= steps) continue;
+        int j;
+        const int i = row_of(step, j), r = OP == OP_COMPACT ? i : s.a[i];
+        if (j * T < s.len_a[i]) was[x] = __ldcg(p.table + (size_t)r * W + j);
+        if (OP == OP_FORK && j * T < s.len_b[i]) shall[x] = __ldcg(p.table + (size_t)s.b[i] * W + j);
+    }
+    if (OP != OP_EXTEND) {
+        bool out = false;
+#pragma unroll
+        for (int x = 0; x < kEntries; ++x) {
+            const int step = tid / 32 + x * warps;
+            if (step >= steps) continue;
+            int j;
+            const int i = row_of(step, j);
+            const bool in_a = j * T < s.len_a[i], in_b = OP == OP_FORK && j * T < s.len_b[i];
+            if (in_a && (was[x] < 0 || was[x] >= p.n_pages)) out = true, was[x] = -1;
+            if (in_b && (shall[x] < 0 || shall[x] >= p.n_pages)) out = true, shall[x] = -1;
+        }
+        if (out) atomicOr(&bad, W4J_PAGES_BAD_PAGE);
+    }
+    auto add_more = [&]() {
+#pragma unroll
+        for (int i = 0; i < kRefs; ++i) {
+            const int page = tid * kRefs + i;
+            if (page < p.n_pages && s.more[page]) p.ref[page] = ref[i] + s.more[page];
+        }
+    };
+    if (OP == OP_FREE) {
+        __syncthreads();
+        if (bad) {
+            if (tid == 0) atomicOr(p.status, bad);
+            return;
+        }
+#pragma unroll
+        for (int x = 0; x < kEntries; ++x)
+            if (was[x] >= 0) atomicSub(s.more + was[x], 1);
+        for (int i = tid; i < n; i += threads) p.len[s.a[i]] = 0;
+        __syncthreads();
+        add_more();
+        return;
+    }
+    // free pages below this thread's
+    int mine = 0, free_pages;
+#pragma unroll
+    for (int i = 0; i < kRefs; ++i) mine += ref[i] <= 0;
+    const int free_before = small_scan(mine, sm, free_pages);
+    if (OP == OP_COMPACT) {
+        const int live = p.n_pages - free_pages;
+#pragma unroll
+        for (int x = 0; x < kEntries; ++x)  // an entry whose page nobody holds
+            if (was[x] >= 0 && __ldcg(p.ref + was[x]) <= 0) atomicOr(&bad, W4J_PAGES_BAD_PAGE);
+        __syncthreads();
+        if (bad) {
+            if (tid == 0) atomicOr(p.status, bad);
+            return;
+        }
+        // the i-th hole below `live` and the i-th held page from it on, by their places in the list
+        int *to = s.list, hole = free_before, moves, highs = 0;
+#pragma unroll
+        for (int i = 0; i < kRefs; ++i) {
+            const int page = tid * kRefs + i;
+            if (page < live && ref[i] <= 0) to[hole++] = page;
+            highs += page >= live && page < p.n_pages && ref[i] > 0;
+        }
+        int high = small_scan(highs, sm, moves);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kRefs; ++i) {
+            const int page = tid * kRefs + i;
+            if (page < live || page >= p.n_pages || ref[i] <= 0) continue;
+            w.from[high] = page, w.to[high] = to[high], w.tokens[high] = T;
+            p.ref[to[high]] = ref[i];
+            p.ref[page] = 0;
+            w.stage[page] = to[high++];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < kEntries; ++x)
+            if (was[x] >= live) {
+                int j;
+                const int i = row_of(tid / 32 + x * warps, j);
+                p.table[(size_t)i * W + j] = w.stage[was[x]];
+            }
+        if (tid == 0) {
+            w.head[H_PAIRS] = moves;
+            if (live_out) *live_out = live;
+        }
+        return;
+    }
+    // pages that each row needs
+    int need = 0;
+    for (int i0 = 0; i0 < n; i0 += threads) {
+        const int i = i0 + tid;
+        int want = 0, total;
+        if (i < n && OP == OP_FORK) {
+            const int from = s.b[i];
+            if (from >= 0 && from < p.n_rows && from != s.a[i] && s.len_b[i] % T) {
+                const int at = s.mark[from];  // -1: the source row goes on by itself
+                want = at < 0 || s.b[at] == from || s.owner[from] != i;
+            }
+        }
+        if (i < n && OP == OP_EXTEND) want = min(held_pages(p, s.len_b[i]) - held_pages(p, s.len_a[i]), free_pages + 1);
+        const int r = need + small_scan(want, sm, total);
+        if (i < n) s.rank[i] = OP == OP_FORK && !want ? -1 : r;
+        need = min(need + total, free_pages + 1);
+    }
+    int at = free_before;
+#pragma unroll
+    for (int i = 0; i < kRefs; ++i)
+        if (ref[i] <= 0 && at < need) s.list[at++] = tid * kRefs + i;
+    if (need > free_pages && tid == 0) atomicOr(&bad, W4J_PAGES_FULL);
+    __syncthreads();
+    if (bad) {
+        if (tid == 0) atomicOr(p.status, bad);
+        return;
+    }
+#pragma unroll
+    for (int x = 0; x < kEntries; ++x) {
+        const int step = tid / 32 + x * warps;
+        if (step >= steps) break;
+        int j;
+        const int i = row_of(step, j);
+        if (j >= W) continue;
+        int *entry = p.table + (size_t)s.a[i] * W + j;
+        if (OP == OP_EXTEND) {
+            const int had = held_pages(p, s.len_a[i]);
+            if (j < had || j >= held_pages(p, s.len_b[i])) continue;
+            const int page = s.list[s.rank[i] + j - had];
+            *entry = page;
+            p.ref[page] = 1;
+        }
+        if (OP == OP_FORK && s.a[i] != s.b[i]) {
+            const int r = s.rank[i];
+            if (r >= 0 && shall[x] >= 0 && (j + 1) * T > s.len_b[i]) {  // the last page, not full
+                w.from[r] = shall[x], w.to[r] = s.list[r], w.tokens[r] = s.len_b[i] - j * T;
+                shall[x] = s.list[r];
+            }
+            if (was[x] == shall[x]) continue;  // what beams have in common
+            if (was[x] >= 0) atomicSub(s.more + was[x], 1);
+            if (shall[x] >= 0) *entry = shall[x], atomicAdd(s.more + shall[x], 1);
+        }
+    }
+    for (int i = tid; i < n; i += threads) p.len[s.a[i]] = s.len_b[i];
+    if (OP == OP_FORK) {
+        if (tid == 0) w.head[H_PAIRS] = need;
+        __syncthreads();
+        add_more();
+    }
+}
+
+// ---------------------------------------------------------------------------
 // the tokens of the pairs that a plan has left: an item is one plane of one pair
 // ---------------------------------------------------------------------------
 constexpr int kMoveThreads = 256, kMoveUnroll = 4;
 
 __global__ void __launch_bounds__(kMoveThreads) k_pages_move(PagesArgs p) {
     pdl_wait();
+    pdl_trigger();
     const Work w(p);
     const int pairs = __ldcg(w.head + H_PAIRS), planes = 2 * p.n_layer;
     const int unit = p.head_dim / 8;  // 16-byte units of a token of one head
@@ -431,8 +690,17 @@ __global__ void __launch_bounds__(kWriteWarps * 32) k_pages_write(PagesArgs p, i
                                                                   const uint4 *__restrict__ k, const uint4 *__restrict__ v,
                                                                   long long k_stride, long long v_stride, int n_tokens) {
     pdl_wait();
+    pdl_trigger();
     const int t = blockIdx.x * kWriteWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (t >= n_tokens) return;
+    const int unit = p.head_dim / 8, n_units = p.n_kv_head * unit;
+    const uint4 *ks = k + t * k_stride, *vs = v + t * v_stride;
+    // the data is on its way while its place is looked up
+    constexpr int U = 4;
+    uint4 kd[U], vd[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+        if (lane + 32 * i < n_units) kd[i] = __ldg(ks + lane + 32 * i), vd[i] = __ldg(vs + lane + 32 * i);
     if (t == 0 && lane == 0 && (start[0] != 0 || start[n] != n_tokens)) atomicOr(p.status, W4J_PAGES_BAD_START);
     // the last i with start[i] <= t, 32 places at a time
     int lo = 0, hi = n;
@@ -451,29 +719,39 @@ __global__ void __launch_bounds__(kWriteWarps * 32) k_pages_write(PagesArgs p, i
         if (lane == 0) atomicOr(p.status, row_ok ? W4J_PAGES_BAD_START : W4J_PAGES_BAD_ROW);
         return;
     }
-    const int j = (int)(pos / p.page_tokens), tok = (int)(pos % p.page_tokens);
+    const int j = (int)pos / p.page_tokens, tok = (int)pos - j * p.page_tokens;
     const int page = __ldcg(p.table + (size_t)r * p.width + j);
     if (page < 0 || page >= p.n_pages) {
         if (lane == 0) atomicOr(p.status, W4J_PAGES_BAD_PAGE);
         return;
     }
-    const int unit = p.head_dim / 8, n_units = p.n_kv_head * unit;
     const size_t page_units = (size_t)n_units * p.page_tokens;
-    uint4 *pool = reinterpret_cast<uint4 *>(p.pool);
-    uint4 *kd = pool + ((size_t)(2 * layer) * p.n_pages + page) * page_units + (size_t)tok * unit;
-    uint4 *vd = kd + (size_t)p.n_pages * page_units;
-    const uint4 *ks = k + t * k_stride, *vs = v + t * v_stride;
+    uint4 *kp = reinterpret_cast<uint4 *>(p.pool) + ((size_t)(2 * layer) * p.n_pages + page) * page_units + (size_t)tok * unit;
+    uint4 *vp = kp + (size_t)p.n_pages * page_units;
     const int whole = p.page_tokens * unit;
-    for (int u = lane; u < n_units; u += 32) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int u = lane + 32 * i, at = u / unit * whole + u % unit;
+        if (u < n_units) kp[at] = kd[i], vp[at] = vd[i];
+    }
+    for (int u = lane + 32 * U; u < n_units; u += 32) {
         const int at = u / unit * whole + u % unit;
-        kd[at] = ks[u];
-        vd[at] = vs[u];
+        kp[at] = __ldg(ks + u);
+        vp[at] = __ldg(vs + u);
     }
 }
 
-int plan_blocks(const PagesArgs &p, long long entries) {
-    // one block answers sooner while its passes are short (a cluster barrier costs more than a block's)
-    return entries <= 4096 && p.n_pages <= 8192 && p.n_rows <= 4096 ? 1 : kPlanCluster;
+// The threads of the one block that takes a call of n rows; 0 where it is too much for one.
+int small_threads(const PagesArgs &p, int n) {
+    const long long steps = (long long)n * ((p.width + 31) / 32), warps = (steps + kEntries - 1) / kEntries,
+                    by_pages = (p.n_pages + 32 * kRefs - 1) / (32 * kRefs), need = warps > by_pages ? warps : by_pages;
+    if (need > kSmallThreads / 32 || small_bytes(p, n) > 160 * 1024) return 0;
+    return 32 * (int)(need < 4 ? 4 : need);
+}
+
+template <PagesOp OP>
+cudaError_t launch_small(const PagesArgs &p, const int *a, const int *b, int *live, int n, int threads, cudaStream_t s) {
+    return launch_after<k_pages_small<OP>>(1, threads, small_bytes(p, n), s, 1, p, a, b, live, n);
 }
 
 int move_blocks(const PagesArgs &p, long long pairs) {
@@ -490,32 +768,36 @@ size_t pages_work_bytes(const PagesArgs &p) {
 }
 
 cudaError_t launch_pages_fork(const PagesArgs &p, const int *dst, const int *src, int n, cudaStream_t s) {
-    const int nb = plan_blocks(p, (long long)n * p.width);
-    cudaError_t e = launch_after(k_pages_fork, nb, kPlanThreads, 0, s, nb, p, dst, src, n);
+    const int t = small_threads(p, n);
+    const cudaError_t e = t ? launch_small<OP_FORK>(p, dst, src, nullptr, n, t, s)
+                            : launch_after<k_pages_fork>(kPlanCluster, kPlanThreads, 0, s, kPlanCluster, p, dst, src, n);
     if (e != cudaSuccess) return e;
-    return launch_after(k_pages_move, move_blocks(p, n), kMoveThreads, 0, s, 1, p);
+    return launch_after<k_pages_move>(move_blocks(p, n), kMoveThreads, 0, s, 1, p);
 }
 
 cudaError_t launch_pages_extend(const PagesArgs &p, const int *rows, const int *start, int n, cudaStream_t s) {
-    const int nb = plan_blocks(p, (long long)n * p.width);
-    return launch_after(k_pages_extend, nb, kPlanThreads, 0, s, nb, p, rows, start, n);
+    const int t = small_threads(p, n);
+    return t ? launch_small<OP_EXTEND>(p, rows, start, nullptr, n, t, s)
+             : launch_after<k_pages_extend>(kPlanCluster, kPlanThreads, 0, s, kPlanCluster, p, rows, start, n);
 }
 
 cudaError_t launch_pages_free(const PagesArgs &p, const int *rows, int n, cudaStream_t s) {
-    const int nb = plan_blocks(p, (long long)n * p.width);
-    return launch_after(k_pages_free, nb, kPlanThreads, 0, s, nb, p, rows, n);
+    const int t = small_threads(p, n);
+    return t ? launch_small<OP_FREE>(p, rows, nullptr, nullptr, n, t, s)
+             : launch_after<k_pages_free>(kPlanCluster, kPlanThreads, 0, s, kPlanCluster, p, rows, n);
 }
 
 cudaError_t launch_pages_compact(const PagesArgs &p, int *live, cudaStream_t s) {
-    const int nb = plan_blocks(p, (long long)p.n_rows * p.width);
-    cudaError_t e = launch_after(k_pages_compact, nb, kPlanThreads, 0, s, nb, p, live);
+    const int t = small_threads(p, p.n_rows);
+    const cudaError_t e = t ? launch_small<OP_COMPACT>(p, nullptr, nullptr, live, p.n_rows, t, s)
+                            : launch_after<k_pages_compact>(kPlanCluster, kPlanThreads, 0, s, kPlanCluster, p, live);
     if (e != cudaSuccess) return e;
-    return launch_after(k_pages_move, move_blocks(p, p.n_pages / 2), kMoveThreads, 0, s, 1, p);
+    return launch_after<k_pages_move>(move_blocks(p, p.n_pages / 2), kMoveThreads, 0, s, 1, p);
 }
 
 cudaError_t launch_pages_write(const PagesArgs &p, int layer, const int *rows, const int *start, int n, const void *k,
                                const void *v, long long k_stride, long long v_stride, int n_tokens, cudaStream_t s) {
-    return launch_after(k_pages_write, (n_tokens + kWriteWarps - 1) / kWriteWarps, kWriteWarps * 32, 0, s, 1, p, layer, rows,
+    return launch_after<k_pages_write>((n_tokens + kWriteWarps - 1) / kWriteWarps, kWriteWarps * 32, 0, s, 1, p, layer, rows,
                         start, n, reinterpret_cast<const uint4 *>(k), reinterpret_cast<const uint4 *>(v), k_stride / 8,
                         v_stride / 8, n_tokens);
 }

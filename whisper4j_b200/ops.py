@@ -252,6 +252,7 @@ class Int8Linear:
         self._bias = None if bias is None else _vector(bias, self.n, self._index, "bias")
         self.weight, self.scale, self.bias = weight, scale, bias
         self._weight, self._k16, self._lib = weight.data_ptr(), k16, _lib.lib()
+        self._work_bytes = {}  # scratch of a call, by its rows
 
     @classmethod
     def from_float(cls, weight, bias=None):
@@ -278,7 +279,9 @@ class Int8Linear:
         if not m:
             return out
         g, b = _norm(ln, k, index)
-        n_bytes = self._lib.w4j_op_linear_i8_layer_workspace(m, k)
+        n_bytes = self._work_bytes.get(m)
+        if n_bytes is None:
+            n_bytes = self._work_bytes[m] = self._lib.w4j_op_linear_i8_layer_workspace(m, k)
         work = torch.empty(n_bytes, dtype=torch.int8, device=x.device) if n_bytes else None
         check(self._lib.w4j_op_linear_i8_layer(index, x.data_ptr(), _TYPES[x.dtype], ldx, g, b, m, k, self._weight, self._k16,
                                                self._scale, self.n, self._bias, code, out.data_ptr(), _TYPES[out.dtype], ldy,
