@@ -331,7 +331,7 @@ int w4j_op_logits_argmax_noalloc(int device, const float *x, int M, int d, const
  *           are neither read nor written
  *   len     [n_rows] tokens of each row
  *   status  [1] what calls could not do, W4J_PAGES_* bits, added up until the caller clears it
- *   work    w4j_op_pages_workspace() bytes of scratch that this cache's calls share
+ *   work    w4j_op_pages_workspace's bytes of scratch that this cache's calls share
  *
  * A new cache is ref, len and status set to zero.  A last page that is not full belongs to one row alone:
  * every call here keeps that so, and a caller that builds tables of its own has to.
@@ -360,8 +360,8 @@ typedef struct w4j_pages {
     size_t work_bytes;
 } w4j_pages;
 
-/* Bytes of scratch (16-byte aligned) that a cache of these sizes needs; 0 where the sizes are refused. */
-size_t w4j_op_pages_workspace(const w4j_pages *cache);
+/* Bytes of scratch (16-byte aligned) that a cache of these sizes needs (its pointers are not looked at). */
+int w4j_op_pages_workspace(const w4j_pages *cache, size_t *bytes);
 
 /* Row rows[i] grows by start[i + 1] - start[i] tokens (start: n + 1 ascending numbers from 0), whose keys
  * and values w4j_op_pages_write brings layer by layer. */
@@ -405,7 +405,7 @@ int w4j_op_pages_compact(const w4j_pages *cache, int32_t *n_live, void *stream);
  *           elements apart (multiples of 8, 16-byte aligned); query head h reads key/value head h / (n_head / n_kv_head)
  *   shared[g] may be at most max_shared, and at most len - n_query + 1 (or 0) of each of its rows.  max_shared and
  *           max_own (an upper bound of len - shared over the rows) size the launch; only max_shared is a limit
- *   work    w4j_op_attn_shared_workspace() bytes, 16-byte aligned, for this call alone until it has run
+ *   work    w4j_op_attn_shared_workspace's bytes, 16-byte aligned, for this call alone until it has run
  *
  * Scores, the softmax and all sums are held in 32 bits; the softmax's weights are rounded to the cache's
  * type before they meet the values.  A sequence whose row, group or shared length is bad, or whose table names a
@@ -426,8 +426,8 @@ typedef struct w4j_attn_shared {
     size_t work_bytes;
 } w4j_attn_shared;
 
-/* Bytes of scratch a call of these sizes needs (pointers and strides are not looked at); 0 where they are refused. */
-size_t w4j_op_attn_shared_workspace(const w4j_attn_shared *args);
+/* Bytes of scratch a call of these sizes needs, 0 for a few short rows (pointers and strides are not looked at). */
+int w4j_op_attn_shared_workspace(const w4j_attn_shared *args, size_t *bytes);
 int w4j_op_attn_shared(const w4j_attn_shared *args, void *stream);
 
 /* ---------------------------------------------------------------------------
@@ -461,10 +461,10 @@ int w4j_op_linear_i8(int device, const int8_t *x, int64_t ldx, const float *x_sc
 /*
  * The two in one call, x in floats (as w4j_op_quantize_rows) and y as w4j_op_linear_i8 makes it: up to 8 rows that fit
  * 48 KB as integers take one launch.  Behind a LayerNorm its sums may run in another order there, so that a quotient
- * next to a half may fall to its other side.  work: w4j_op_linear_i8_layer_workspace(M, K) bytes (0 for those few rows),
+ * next to a half may fall to its other side.  work: w4j_op_linear_i8_layer_workspace's bytes (0 for those few rows),
  * 16-byte aligned, for this call alone until it has run.
  */
-size_t w4j_op_linear_i8_layer_workspace(int M, int K);
+int w4j_op_linear_i8_layer_workspace(int M, int K, size_t *bytes);
 int w4j_op_linear_i8_layer(int device, const void *x, int x_type, int64_t ldx, const float *ln_g, const float *ln_b, int M,
                            int K, const int8_t *w, int64_t ldw, const float *w_scale, int N, const float *bias,
                            int epilogue, void *y, int y_type, int64_t ldy, void *work, size_t work_bytes, void *stream);

@@ -21,6 +21,13 @@ def refused(rc, text):
     assert text in lib().w4j_last_error().decode()
 
 
+def workspace(fn, *args):
+    n = ctypes.c_size_t(77)
+    rc = fn(*args, ctypes.byref(n))
+    assert rc == W4J_OK or n.value == 0
+    return rc, n.value
+
+
 BAD_CACHES = [(dict(type=GGML_F32), "type"), (dict(head_dim=96), "head_dim"), (dict(page_tokens=0), "page_tokens"),
               (dict(page_tokens=12), "page_tokens"), (dict(page_tokens=1032), "page_tokens"), (dict(n_layer=0), "n_layer"),
               (dict(n_kv_head=-1), "n_kv_head"), (dict(n_pages=0), "n_pages"), (dict(n_pages=(1 << 21) + 1), "n_pages"),
@@ -34,14 +41,15 @@ BAD_POINTERS = [(dict(pool=None), "null"), (dict(ref=None), "null"), (dict(table
 
 @pytest.mark.parametrize("kw,text", BAD_CACHES)
 def test_workspace_refuses_sizes(kw, text):
-    assert lib().w4j_op_pages_workspace(ctypes.byref(cache(**kw))) == 0
-    assert text in lib().w4j_last_error().decode()
+    refused(workspace(lib().w4j_op_pages_workspace, ctypes.byref(cache(**kw)))[0], text)
 
 
 def test_workspace_grows_with_the_cache():
-    small = lib().w4j_op_pages_workspace(ctypes.byref(cache(pool=None, work=None)))
-    assert 0 < small < lib().w4j_op_pages_workspace(ctypes.byref(cache(n_rows=8))) < 1 << 16
-    assert lib().w4j_op_pages_workspace(None) == 0
+    w = lib().w4j_op_pages_workspace
+    small = workspace(w, ctypes.byref(cache(pool=None, work=None)))[1]
+    assert 0 < small < workspace(w, ctypes.byref(cache(n_rows=8)))[1] < 1 << 16
+    refused(workspace(w, None)[0], "null")
+    refused(w(ctypes.byref(cache()), None), "null")
 
 
 @pytest.mark.parametrize("kw,text", BAD_CACHES + BAD_POINTERS)
@@ -82,7 +90,7 @@ def test_write_refusals(layer, k, ks, v, vs, tokens, text):
 
 
 def test_bf16_is_a_cache_type():
-    assert lib().w4j_op_pages_workspace(ctypes.byref(cache(type=GGML_BF16, head_dim=128))) > 0
+    assert workspace(lib().w4j_op_pages_workspace, ctypes.byref(cache(type=GGML_BF16, head_dim=128)))[1] > 0
 
 
 def test_a_device_that_is_not_there():
@@ -125,16 +133,15 @@ def attn(c, **kw):
     (dict(max_shared=81), "max_shared"), (dict(max_own=81), "max_own")])
 def test_attention_refuses_sizes(kw, text):
     a = ctypes.byref(attn(cache(), **kw))
-    assert lib().w4j_op_attn_shared_workspace(a) == 0
-    assert text in lib().w4j_last_error().decode()
+    refused(workspace(lib().w4j_op_attn_shared_workspace, a)[0], text)
     refused(lib().w4j_op_attn_shared(a, None), text)
 
 
 @pytest.mark.parametrize("kw,text", [
     (dict(q=None), "null"), (dict(out=None), "null"), (dict(rows=None), "null"), (dict(group_start=None), "null"),
-    (dict(shared=None), "null"), (dict(work=None), "null"), (dict(q_stride=376), "strides"), (dict(out_stride=388), "strides"),
-    (dict(q=P + 8), "aligned"), (dict(out=P + 2), "aligned"), (dict(work=P + 8), "aligned"), (dict(work_bytes=64), "work"),
-    (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(shared=None), "null"), (dict(work=None, n_seq=100), "work"), (dict(q_stride=376), "strides"), (dict(out_stride=388), "strides"),
+    (dict(q=P + 8), "aligned"), (dict(out=P + 2), "aligned"), (dict(work=P + 8, n_seq=100), "work"),
+    (dict(work_bytes=64, n_seq=100), "work"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(scale=float("inf")), "scale")])
 def test_attention_refuses_arguments(kw, text):
     refused(lib().w4j_op_attn_shared(ctypes.byref(attn(cache(), **kw)), None), text)
@@ -192,6 +199,14 @@ def test_layer_refusals(kw, text):
 
 def test_layer_workspace():
     w = lib().w4j_op_linear_i8_layer_workspace
-    assert w(9, 100) == 9 * (112 + 4) and w(8, 1280) == 0 and w(1, 40000) == 0 and w(8, 7000) == 8 * (7008 + 4)
+    for m, k, n in ((9, 100, 9 * (112 + 4)), (8, 1280, 0), (1, 40000, 0), (8, 7000, 8 * (7008 + 4))):
+        assert workspace(w, m, k) == (W4J_OK, n)
     for m, k in ((0, 1), (1, 0), (1, 131057), ((1 << 24) + 1, 1)):
-        assert w(m, k) == 0 and b"shape" in lib().w4j_last_error()
+        refused(workspace(w, m, k)[0], "shape")
+    refused(w(1, 1, None), "null")
+
+
+def test_a_few_short_rows_need_no_scratch():
+    w = lib().w4j_op_attn_shared_workspace
+    assert workspace(w, ctypes.byref(attn(cache()))) == (W4J_OK, 0)
+    assert workspace(w, ctypes.byref(attn(cache(), n_seq=100)))[1] > 0

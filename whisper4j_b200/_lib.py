@@ -118,16 +118,16 @@ SIGNATURES = {
     "w4j_op_logits_argmax": (_I, [_P, _P, _I, _P, _I, _P, _P, _P, _P, _P]),
     "w4j_op_logits_argmax_noalloc": (_I, [_I, _P, _I, _I, _P, _I, _P, _P, _P, _P, _P]),
     "w4j_test_withhold_logits_copies": (_I, [_I]),
-    "w4j_op_pages_workspace": (_SZ, [_P]),
+    "w4j_op_pages_workspace": (_I, [_P, ctypes.POINTER(_SZ)]),
     "w4j_op_pages_extend": (_I, [_P, _P, _P, _I, _P]),
     "w4j_op_pages_write": (_I, [_P, _I, _P, _P, _I, _P, _I64, _P, _I64, _I, _P]),
     "w4j_op_pages_fork": (_I, [_P, _P, _P, _I, _P]),
     "w4j_op_pages_free": (_I, [_P, _P, _I, _P]),
     "w4j_op_pages_compact": (_I, [_P, _P, _P]),
-    "w4j_op_attn_shared_workspace": (_SZ, [_P]),
+    "w4j_op_attn_shared_workspace": (_I, [_P, ctypes.POINTER(_SZ)]),
     "w4j_op_attn_shared": (_I, [_P, _P]),
     "w4j_op_quantize_rows": (_I, [_I, _P, _I, _I, _I, _I64, _P, _P, _P, _I64, _P, _P]),
-    "w4j_op_linear_i8_layer_workspace": (_SZ, [_I, _I]),
+    "w4j_op_linear_i8_layer_workspace": (_I, [_I, _I, ctypes.POINTER(_SZ)]),
     "w4j_op_linear_i8_layer": (_I, [_I, _P, _I, _I64, _P, _P, _I, _I, _P, _I64, _P, _I, _P, _I, _P, _I, _I64, _P, _SZ, _P]),
     "w4j_op_linear_i8": (_I, [_I, _P, _I64, _P, _I, _I, _P, _I64, _P, _I, _P, _I, _P, _I, _I64, _P]),
 }

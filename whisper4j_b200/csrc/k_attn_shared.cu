@@ -144,9 +144,10 @@ struct WarpTile {
         }
     }
 
-    // Keys [k0, k1) of the row whose table is `table`.  Query 8 n + 2 q + i sees the keys below lim[n][i], all
-    // queries see those below `all`.  sm: the warp's ring, full: a barrier for each stage; box: rows of a TMA box.
-    __device__ __forceinline__ void run(const PagesArgs &p, const int *table, int head, const CUtensorMap *kmap,
+    // Keys [k0, k1) of the row whose table is `table`; boxes below `shared` are found in `first`'s instead.  Query
+    // 8 n + 2 q + i sees the keys below lim[n][i], all queries see those below `all`.  sm: the warp's ring, full: a
+    // barrier for each stage; box: rows of a TMA box.
+    __device__ __forceinline__ void run(const PagesArgs &p, const int *table, const int *first, int shared, int head, const CUtensorMap *kmap,
                                         const CUtensorMap *vmap, unsigned char *sm, uint64_t *full, int box, int k0, int k1,
                                         const int (&lim)[NT][2], int all, float scale_log2, int *bad, int *failed) {
         const int lane = threadIdx.x & 31, g = lane >> 2;
@@ -156,7 +157,8 @@ struct WarpTile {
         int key = start + (lane & 15) * box, j = key / p.page_tokens, tok = key - j * p.page_tokens;
         const int dj = STEP / p.page_tokens, dt = STEP - dj * p.page_tokens;
         const bool mine = (lane & 15) * box < STEP;
-        int page = mine && key < k1 ? __ldg(table + j) : 0;
+        auto page_of = [&]() { return mine && key < k1 ? __ldg((key + box <= shared ? first : table) + j) : 0; };
+        int page = page_of();
         auto issue = [&](int i) {
             const int at = start + i * STEP, boxes = (min(STEP, k1 - at) + box - 1) / box, st = i % kAsStages;
             if (lane == 0) mbar_expect_tx(full + st, 2 * NB * boxes * box * 128);
@@ -170,7 +172,7 @@ struct WarpTile {
             __syncwarp();
             key += STEP, j += dj, tok += dt;
             if (tok >= p.page_tokens) tok -= p.page_tokens, ++j;
-            page = mine && key < k1 ? __ldg(table + j) : 0;  // for the next call
+            page = page_of();  // for the next call
         };
         for (int i = 0; i < kAsStages && i < n_steps; ++i) issue(i);
         // ldmatrix rows: keys as they lie, values transposed
@@ -317,6 +319,28 @@ struct WarpTile {
 // ---------------------------------------------------------------------------
 // items: (group tile, head, split) of the shared keys, then (row, head, tile, split) of the rows' own
 // ---------------------------------------------------------------------------
+// Row, its group's first row, length and shared length of sequence `seq`, 0 or what is wrong with it (then rows 0); the whole warp calls it.
+// first: whether this call also looks at the groups' ends.
+__device__ __forceinline__ int find_row(const AttnSharedArgs &a, int seq, bool first, int &row, int &row0, int &len, int &shared) {
+    const PagesArgs &p = a.p;
+    const int r = __ldg(a.rows + seq);
+    const int gr = warp_find(a.n_group, seq, [&](int i) { return (long long)__ldg(a.group_start + i); });
+    const int lo = __ldg(a.group_start + gr), hi = __ldg(a.group_start + gr + 1), s = __ldg(a.shared + gr);
+    const bool row_ok = r >= 0 && r < p.n_rows;
+    row = row_ok ? r : 0;
+    len = row_ok ? max(0, min(__ldg(p.len + r), p.width * p.page_tokens)) : 0;
+    shared = s;
+    // the shared keys are read through the group's first row: what is wrong there concerns all of them
+    const bool group_ok = lo >= 0 && lo <= seq && seq < hi && hi <= a.n_seq;
+    const int r0 = group_ok ? __ldg(a.rows + lo) : -1;
+    row0 = r0 >= 0 && r0 < p.n_rows ? r0 : 0;
+    const int len0 = r0 >= 0 && r0 < p.n_rows ? __ldg(p.len + r0) : -1;
+    int bad = !group_ok ? W4J_PAGES_BAD_START : !row_ok || len0 < 0 ? W4J_PAGES_BAD_ROW
+              : s < 0 || s > a.max_shared || s > max(0, min(len, len0) - a.n_query + 1) ? W4J_PAGES_BAD_SHARED : 0;
+    if (first && (lo != 0 || __ldg(a.group_start + a.n_group) != a.n_seq)) bad |= W4J_PAGES_BAD_START;
+    return bad;
+}
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_constant__ CUtensorMap kmap,
                                                                const __grid_constant__ CUtensorMap vmap, AttnSharedArgs a,
@@ -367,21 +391,10 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_cons
         head = (int)(item / a.own_tiles / a.own_splits % p.n_kv_head);
         seq0 = (int)(item / a.own_tiles / a.own_splits / p.n_kv_head);
         n_rows = c;
-        const int r = __ldg(a.rows + seq0);
-        const int gr = warp_find(a.n_group, seq0, [&](int i) { return (long long)__ldg(a.group_start + i); });
-        const int lo = __ldg(a.group_start + gr), hi = __ldg(a.group_start + gr + 1), s = __ldg(a.shared + gr);
-        const bool row_ok = r >= 0 && r < p.n_rows;
-        own_len = row_ok ? max(0, min(__ldg(p.len + r), p.width * p.page_tokens)) : 0;
-        table = p.table + (size_t)(row_ok ? r : 0) * p.width;
-        // the shared keys are read through the group's first row: what is wrong there concerns all of them
-        const bool group_ok = lo >= 0 && lo <= seq0 && seq0 < hi && hi <= a.n_seq;
-        const int r0 = group_ok ? __ldg(a.rows + lo) : -1;
-        const int len0 = r0 >= 0 && r0 < p.n_rows ? __ldg(p.len + r0) : -1;
-        bad = !group_ok ? W4J_PAGES_BAD_START : !row_ok || len0 < 0 ? W4J_PAGES_BAD_ROW
-              : s < 0 || s > a.max_shared || s > max(0, min(own_len, len0) - a.n_query + 1) ? W4J_PAGES_BAD_SHARED : 0;
-        if (seq0 + head + split + tile == 0 && (lo != 0 || __ldg(a.group_start + a.n_group) != a.n_seq))
-            bad |= W4J_PAGES_BAD_START;
-        const int from = bad ? 0 : s, n = bad ? 0 : own_len - s;
+        int r, r0, shared;
+        bad = find_row(a, seq0, seq0 + head + split + tile == 0, r, r0, own_len, shared);
+        table = p.table + (size_t)r * p.width;
+        const int from = bad ? 0 : shared, n = bad ? 0 : own_len - shared;
         const int step = ((n + a.own_splits - 1) / a.own_splits + 31) / 32 * 32;
         k0 = from + min(n, split * step), k1 = min(from + n, k0 + step);
         slot = a.shared_splits + split;
@@ -417,7 +430,7 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_cons
     WarpTile<T, D, NT> w;
     int bad_page = 0;
     w.load_q(qr);
-    w.run(p, table, head, &kmap, &vmap, sm + wi * kAsStages * kAsStage, full[wi], box, k0, k1, lim, own_len - a.n_query + 1,
+    w.run(p, table, nullptr, 0, head, &kmap, &vmap, sm + wi * kAsStages * kAsStage, full[wi], box, k0, k1, lim, own_len - a.n_query + 1,
           a.scale_log2, &bad_page, &failed[wi]);
     if (__any_sync(0xffffffffu, bad_page)) bad |= W4J_PAGES_BAD_PAGE;
     __syncwarp();
@@ -428,6 +441,95 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_cons
     }
     w.store(po, pm);
     if (a.tc_tiles) pdl_wait();
+}
+
+// ---------------------------------------------------------------------------
+// a few short rows: a block takes a row, head and tile, its warps share all of the row's keys (the group's among them: read
+// again by every row, from L2) and join their sums in shared memory.  One launch and no scratch; bound by latency.
+// ---------------------------------------------------------------------------
+constexpr int kDirectWarps = 8;
+constexpr size_t kDirectSmem = (size_t)kDirectWarps * kAsStages * kAsStage + 1024;
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_constant__ CUtensorMap kmap,
+                                                                   const __grid_constant__ CUtensorMap vmap, AttnSharedArgs a,
+                                                                   int box) {
+    extern __shared__ unsigned char raw[];
+    __shared__ uint64_t full[kDirectWarps][kAsStages];
+    __shared__ int failed, wrong;
+    __shared__ float2 ml[kDirectWarps][8 * NT];
+    pdl_wait();
+    pdl_trigger();
+    constexpr int R = 8 * NT;
+    const PagesArgs &p = a.p;
+    const int tid = threadIdx.x, wi = tid >> 5, lane = tid & 31, g = lane >> 2, qd = lane & 3;
+    const int c = a.n_query * a.rep;
+    const int tile = blockIdx.x % a.own_tiles, head = blockIdx.x / a.own_tiles % p.n_kv_head, seq = blockIdx.x / a.own_tiles / p.n_kv_head;
+    if (tid == 0) failed = wrong = 0;
+    if (lane == 0) {
+        for (int i = 0; i < kAsStages; ++i) mbar_init(&full[wi][i], 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    int row, row0, len, shared;
+    int bad = find_row(a, seq, blockIdx.x == 0, row, row0, len, shared);
+    const int n = bad ? 0 : len, step = ((n + kDirectWarps - 1) / kDirectWarps + 31) / 32 * 32;
+    const int k0 = min(n, wi * step), k1 = min(n, k0 + step);
+    const T *q = reinterpret_cast<const T *>(a.q);
+    const T *qr[NT];
+    int lim[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = tile * R + 8 * t + g;
+        qr[t] = r < c ? q + ((size_t)seq * a.n_query + r / a.rep) * a.q_stride + (size_t)(head * a.rep + r % a.rep) * D : nullptr;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int x = tile * R + 8 * t + 2 * qd + i;
+            lim[t][i] = x < c ? len - a.n_query + x / a.rep + 1 : 0;
+        }
+    }
+    unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023) +
+                        wi * kAsStages * kAsStage;
+    WarpTile<T, D, NT> w;
+    int bad_page = 0;
+    w.load_q(qr);
+    w.run(p, p.table + (size_t)row * p.width, p.table + (size_t)row0 * p.width, bad ? 0 : shared, head, &kmap, &vmap, sm, full[wi], box, k0, k1, lim, len - a.n_query + 1, a.scale_log2,
+          &bad_page, &failed);
+    if (__any_sync(0xffffffffu, bad_page)) bad |= W4J_PAGES_BAD_PAGE;
+    if (bad && lane == 0) atomicOr(&wrong, bad);
+    __syncwarp();
+    // the warp's o over its ring, [8 NT][D]
+    float *po[NT][2], *pm[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            po[t][i] = reinterpret_cast<float *>(sm) + (8 * t + 2 * qd + i) * D;
+            pm[t][i] = reinterpret_cast<float *>(&ml[wi][8 * t + 2 * qd + i]);
+        }
+    w.store(po, pm);
+    __syncthreads();
+    if (tid == 0 && wrong) atomicOr(p.status, wrong);
+    const bool lost = failed || wrong;
+    const float *o0 = reinterpret_cast<const float *>(sm - wi * kAsStages * kAsStage);
+    for (int x = tid; x < R * D / 2; x += kDirectWarps * 32) {
+        const int r = x / (D / 2), d = 2 * (x % (D / 2)), qi = tile * R + r;
+        if (qi >= c) break;
+        float m = kNone, l = 0.f, u = 0.f, v = 0.f;
+#pragma unroll
+        for (int y = 0; y < kDirectWarps; ++y) m = fmaxf(m, ml[y][r].x);
+#pragma unroll
+        for (int y = 0; y < kDirectWarps; ++y) {
+            const float2 part = ml[y][r];
+            if (part.y == 0.f) continue;
+            const float f = ex2(part.x - m);
+            const float2 o = *reinterpret_cast<const float2 *>(o0 + y * (kAsStages * kAsStage / 4) + r * D + d);
+            l += f * part.y, u += f * o.x, v += f * o.y;
+        }
+        const float inv = lost ? NAN : l == 0.f ? 0.f : 1.f / l;  // a query that sees nothing gets zeros
+        T *out = reinterpret_cast<T *>(a.out) + ((size_t)seq * a.n_query + qi / a.rep) * a.out_stride + (size_t)(head * a.rep + qi % a.rep) * D;
+        *reinterpret_cast<uint32_t *>(out + d) = pack2<T>(u * inv, v * inv);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -825,6 +927,13 @@ cudaError_t launch(const AttnSharedArgs &a, cudaStream_t s) {
         return make_tmap_f16_box(&km, pk, head_rows, D, box) && make_tmap_f16_box(&vm, pv, head_rows, D, box) ? box : 0;
     };
     cudaError_t e;
+    if (a.direct) {
+        const int box = maps(2048 / D);
+        if (!box) return cudaErrorInvalidValue;
+        const unsigned blocks = a.n_seq * p.n_kv_head * a.own_tiles;
+        return a.tile_rows == 8 ? launch_after<k_attn_direct<T, D, 1>>(blocks, kDirectWarps * 32, kDirectSmem, s, 1, km, vm, a, box)
+                                : launch_after<k_attn_direct<T, D, 2>>(blocks, kDirectWarps * 32, kDirectSmem, s, 1, km, vm, a, box);
+    }
     if (a.tc_tiles) {
         const int box = maps(kTcKeys);
         if (!box) return cudaErrorInvalidValue;
@@ -882,6 +991,13 @@ void attn_shared_plan(AttnSharedArgs &a) {
     a.own_splits = own < 1 ? 1 : own;
     a.own_items = (unsigned)a.n_seq * p.n_kv_head * a.own_tiles * a.own_splits;
     a.slots = a.shared_splits + a.own_splits;
+    // a block for each row, head and tile where they are no more than the SMs and no warp gets more than four steps
+    a.direct = 0;
+    const unsigned direct_tiles = (unsigned)((c + (c <= 8 ? 7 : 15)) / (c <= 8 ? 8 : 16));
+    if ((long long)a.n_seq * p.n_kv_head * direct_tiles <= 148 && a.max_shared + a.max_own <= kDirectWarps * 32 * 4) {
+        a.direct = 1, a.slots = 0;
+        a.tile_rows = c <= 8 ? 8 : 16, a.own_tiles = direct_tiles;
+    }
 }
 
 size_t attn_shared_work_bytes(const AttnSharedArgs &a) {

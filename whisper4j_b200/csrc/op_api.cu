@@ -58,9 +58,13 @@ static int pages_call(const w4j_pages *c, const char *who, const void *a, const 
     return W4J_OK;
 }
 
-extern "C" size_t w4j_op_pages_workspace(const w4j_pages *c) {
+extern "C" int w4j_op_pages_workspace(const w4j_pages *c, size_t *bytes) {
     PagesArgs p;
-    return pages_sizes(c, "w4j_op_pages_workspace", &p) < 0 ? 0 : pages_work_bytes(p);
+    if (!bytes) return set_err(W4J_ERR_ARG, "w4j_op_pages_workspace: null argument");
+    *bytes = 0;
+    TRY(pages_sizes(c, "w4j_op_pages_workspace", &p));
+    *bytes = pages_work_bytes(p);
+    return W4J_OK;
 }
 
 extern "C" int w4j_op_pages_extend(const w4j_pages *c, const int32_t *rows, const int32_t *start, int n, void *stream) {
@@ -143,9 +147,13 @@ static int attn_sizes(const w4j_attn_shared *x, const char *who, AttnSharedArgs 
     return W4J_OK;
 }
 
-extern "C" size_t w4j_op_attn_shared_workspace(const w4j_attn_shared *x) {
+extern "C" int w4j_op_attn_shared_workspace(const w4j_attn_shared *x, size_t *bytes) {
     AttnSharedArgs a;
-    return attn_sizes(x, "w4j_op_attn_shared_workspace", &a) < 0 ? 0 : attn_shared_work_bytes(a);
+    if (!bytes) return set_err(W4J_ERR_ARG, "w4j_op_attn_shared_workspace: null argument");
+    *bytes = 0;
+    TRY(attn_sizes(x, "w4j_op_attn_shared_workspace", &a));
+    *bytes = attn_shared_work_bytes(a);
+    return W4J_OK;
 }
 
 extern "C" int w4j_op_attn_shared(const w4j_attn_shared *x, void *stream) {
@@ -153,17 +161,18 @@ extern "C" int w4j_op_attn_shared(const w4j_attn_shared *x, void *stream) {
     AttnSharedArgs a;
     TRY(attn_sizes(x, who, &a));
     TRY(pages_check(x->cache, who, &a.p));
-    if (!x->q || !x->out || !x->rows || !x->group_start || !x->shared || !x->work)
+    if (!x->q || !x->out || !x->rows || !x->group_start || !x->shared)
         return set_err(W4J_ERR_ARG, "%s: null argument", who);
     const int64_t token = (int64_t)x->n_head * a.p.head_dim;
     if (x->q_stride < token || x->out_stride < token || x->q_stride % 8 || x->out_stride % 8)
         return set_err(W4J_ERR_ARG, "%s: strides must be multiples of 8 of at least n_head * head_dim", who);
-    if (!aligned(x->q, 16) || !aligned(x->out, 16) || !aligned(x->work, 16))
-        return set_err(W4J_ERR_ARG, "%s: q, out and work must be 16-byte aligned", who);
+    if (!aligned(x->q, 16) || !aligned(x->out, 16))
+        return set_err(W4J_ERR_ARG, "%s: q and out must be 16-byte aligned", who);
     if (!(x->scale > 0) || x->scale > 3e38f) return set_err(W4J_ERR_ARG, "%s: scale must be positive and finite", who);
-    if (x->work_bytes < attn_shared_work_bytes(a))
-        return set_err(W4J_ERR_ARG, "%s: work has %zu bytes, w4j_op_attn_shared_workspace asks for %zu", who, x->work_bytes,
-                       attn_shared_work_bytes(a));
+    const size_t need = attn_shared_work_bytes(a);
+    if (need && (!x->work || !aligned(x->work, 16) || x->work_bytes < need))
+        return set_err(W4J_ERR_ARG, "%s: work must be 16-byte aligned and hold the %zu bytes that w4j_op_attn_shared_workspace asks for",
+                       who, need);
     a.scale_log2 = x->scale * 1.44269504f;
     a.q = x->q, a.out = x->out, a.q_stride = x->q_stride, a.out_stride = x->out_stride;
     a.rows = x->rows, a.group_start = x->group_start, a.shared = x->shared;
@@ -228,12 +237,13 @@ extern "C" int w4j_op_linear_i8(int device, const int8_t *x, int64_t ldx, const 
     return W4J_OK;
 }
 
-extern "C" size_t w4j_op_linear_i8_layer_workspace(int M, int K) {
-    if (M < 1 || K < 1 || M > 1 << 24 || K > 131056) {
-        set_err(W4J_ERR_ARG, "w4j_op_linear_i8_layer_workspace: bad shape (%d x %d)", M, K);
-        return 0;
-    }
-    return linear_i8_layer_work(M, K);
+extern "C" int w4j_op_linear_i8_layer_workspace(int M, int K, size_t *bytes) {
+    if (!bytes) return set_err(W4J_ERR_ARG, "w4j_op_linear_i8_layer_workspace: null argument");
+    *bytes = 0;
+    if (M < 1 || K < 1 || M > 1 << 24 || K > 131056)
+        return set_err(W4J_ERR_ARG, "w4j_op_linear_i8_layer_workspace: bad shape (%d x %d)", M, K);
+    *bytes = linear_i8_layer_work(M, K);
+    return W4J_OK;
 }
 
 extern "C" int w4j_op_linear_i8_layer(int device, const void *x, int x_type, int64_t ldx, const float *ln_g, const float *ln_b, int M,

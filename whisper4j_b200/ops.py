@@ -86,8 +86,9 @@ class PagedCache:
                             self.page_tokens, pool.shape[1], self.n_rows, table.shape[1], pool.data_ptr(), ref.data_ptr(),
                             table.data_ptr(), length.data_ptr(), self.status.data_ptr())
         self._ref, self._ptr = ctypes.byref(c), ctypes.pointer(c)
-        c.work_bytes = self._lib.w4j_op_pages_workspace(self._ref)
-        _need(c.work_bytes, self._lib.w4j_last_error().decode())
+        n_bytes = ctypes.c_size_t()
+        check(self._lib.w4j_op_pages_workspace(self._ref, ctypes.byref(n_bytes)))
+        c.work_bytes = n_bytes.value
         self._work = torch.empty(c.work_bytes, dtype=torch.uint8, device=self.device)
         c.work = self._work.data_ptr()
 
@@ -153,7 +154,7 @@ class PagedCache:
             raise ValueError(f"q must be (n_seq, n_query, n_head, {self.head_dim}) {self.dtype} on {self.device}, not {_shape(q)}")
         n_seq, n_query, n_head, _ = q.shape
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != self._index:
             raise ValueError(f"out must be like q, not {_shape(out)}")
         if q.numel() == 0:
@@ -164,12 +165,11 @@ class PagedCache:
         a = AttnShared(self._ptr, layer, n_head, n_query, n_seq, n, max_shared, max_own,
                        self.head_dim ** -0.5 if scale is None else scale, q.data_ptr(), out.data_ptr(),
                        self._query_stride(q, "q"), self._query_stride(out, "out"), r, g, sh)
-        ref = ctypes.byref(a)
-        n_bytes = self._lib.w4j_op_attn_shared_workspace(ref)
-        if not n_bytes:
-            raise ValueError(self._lib.w4j_last_error().decode())
-        work = torch.empty(n_bytes, dtype=torch.uint8, device=self.device)
-        a.work, a.work_bytes = work.data_ptr(), n_bytes
+        ref, n_bytes = ctypes.byref(a), ctypes.c_size_t()
+        check(self._lib.w4j_op_attn_shared_workspace(ref, n_bytes))
+        if n_bytes.value:
+            work = torch.empty(n_bytes.value, dtype=torch.uint8, device=self.device)
+            a.work, a.work_bytes = work.data_ptr(), n_bytes.value
         check(self._lib.w4j_op_attn_shared(ref, _raw_stream(self._index)))
         return out
 
@@ -281,7 +281,9 @@ class Int8Linear:
         g, b = _norm(ln, k, index)
         n_bytes = self._work_bytes.get(m)
         if n_bytes is None:
-            n_bytes = self._work_bytes[m] = self._lib.w4j_op_linear_i8_layer_workspace(m, k)
+            size = ctypes.c_size_t()
+            check(self._lib.w4j_op_linear_i8_layer_workspace(m, k, size))
+            n_bytes = self._work_bytes[m] = size.value
         work = torch.empty(n_bytes, dtype=torch.int8, device=x.device) if n_bytes else None
         check(self._lib.w4j_op_linear_i8_layer(index, x.data_ptr(), _TYPES[x.dtype], ldx, g, b, m, k, self._weight, self._k16,
                                                self._scale, self.n, self._bias, code, out.data_ptr(), _TYPES[out.dtype], ldy,
