@@ -175,13 +175,16 @@ struct WarpTile {
             page = page_of();  // for the next call
         };
         for (int i = 0; i < kAsStages && i < n_steps; ++i) issue(i);
-        // ldmatrix rows: keys as they lie, values transposed
+        // ldmatrix rows: keys as they lie, values transposed; offsets of the first 16 keys' units of dimensions 16 t on
         const int kr = lane & 15, kc = lane >> 4, vr = (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;
+        uint32_t k_at[4], v_at[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) k_at[t] = kr * 128 + ((2 * t + kc) ^ (kr & 7)) * 16, v_at[t] = kKeys + vr * 128 + ((2 * t + vc) ^ (vr & 7)) * 16;
         int i = 0;
         for (; i < n_steps; ++i) {
             const int st = i % kAsStages, kb = start + i * STEP;
             if (!__all_sync(0xffffffffu, wait_phase(full + st, (i / kAsStages) & 1, failed))) break;
-            const uint32_t sk = smem_u32(sm + st * kAsStage), sv = sk + kKeys;
+            const uint32_t base = smem_u32(sm + st * kAsStage);
             const bool masked = kb < k0 || kb + STEP > min(k1, all);
             if (kb + STEP > k1) {  // behind the last key there may be anything: zero
                 for (int x = lane; x < (kb + STEP - k1) * 8 * NB; x += 32)
@@ -197,7 +200,7 @@ struct WarpTile {
 #pragma unroll
                 for (int t = 0; t < D / 16; ++t) {
                     uint32_t a[4];
-                    ldsm4(a, sk + t / 4 * kBlock + (16 * h + kr) * 128 + (((2 * t + kc) & 7) ^ (kr & 7)) * 16);
+                    ldsm4(a, base + k_at[t & 3] + t / 4 * kBlock + h * 2048);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma<T>(s[n][h], a, qf[n][t][0], qf[n][t][1]);
                 }
@@ -248,20 +251,27 @@ struct WarpTile {
                     for (int t = 0; t < D / 16; ++t)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[n][t][e] *= c[n][e & 1];
-            const bool hidden = kb + STEP > all && hides(sm + st * kAsStage + kKeys);
+            if (kb + STEP > all && hides(sm + st * kAsStage + kKeys)) {
 #pragma unroll
-            for (int h = 0; h < H; ++h)
+                for (int h = 0; h < H; ++h)
 #pragma unroll
-                for (int t = 0; t < D / 16; ++t) {
-                    uint32_t a[4];
-                    ldsm4_t(a, sv + t / 4 * kBlock + (16 * h + vr) * 128 + (((2 * t + vc) & 7) ^ (vr & 7)) * 16);
+                    for (int t = 0; t < D / 16; ++t) {
+                        uint32_t a[4];
+                        ldsm4_t(a, base + v_at[t & 3] + t / 4 * kBlock + h * 2048);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        if (hidden)
-                            add_hidden(o[n][t], a, pf[n][h], lim[n], kb + 16 * h);
-                        else
-                            mma<T>(o[n][t], a, pf[n][h][0], pf[n][h][1]);
-                }
+                        for (int n = 0; n < NT; ++n) add_hidden(o[n][t], a, pf[n][h], lim[n], kb + 16 * h);
+                    }
+            } else {
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int t = 0; t < D / 16; ++t) {
+                        uint32_t a[4];
+                        ldsm4_t(a, base + v_at[t & 3] + t / 4 * kBlock + h * 2048);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma<T>(o[n][t], a, pf[n][h][0], pf[n][h][1]);
+                    }
+            }
             __syncwarp();
             if (i + kAsStages < n_steps) issue(i + kAsStages);
         }
@@ -395,8 +405,9 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_cons
         bad = find_row(a, seq0, seq0 + head + split + tile == 0, r, r0, own_len, shared);
         table = p.table + (size_t)r * p.width;
         const int from = bad ? 0 : shared, n = bad ? 0 : own_len - shared;
-        const int step = ((n + a.own_splits - 1) / a.own_splits + 31) / 32 * 32;
-        k0 = from + min(n, split * step), k1 = min(from + n, k0 + step);
+        // pieces of one size whatever the row's length (a long row's would be the last to end), the last one to the end
+        const int step = ((a.max_own + a.own_splits - 1) / a.own_splits + 31) / 32 * 32;
+        k0 = from + min(n, split * step), k1 = split + 1 == (int)a.own_splits ? from + n : min(from + n, k0 + step);
         slot = a.shared_splits + split;
     }
     // query r of the tile: (sequence, query token, head)
@@ -987,8 +998,8 @@ void attn_shared_plan(AttnSharedArgs &a) {
     }
     a.shared_items = a.shared_tiles * a.shared_splits * p.n_kv_head;
     a.own_tiles = (unsigned)((c + a.tile_rows - 1) / a.tile_rows);
-    const int own = a.max_own > 0 ? splits((long long)a.n_seq * p.n_kv_head * a.own_tiles, a.max_own) : 1;
-    a.own_splits = own < 1 ? 1 : own;
+    const int own = a.max_own > 0 ? splits((long long)a.n_seq * p.n_kv_head * a.own_tiles, a.max_own) : 1, pieces = (a.max_own + 255) / 256;
+    a.own_splits = own > pieces ? own : pieces < 1 ? 1 : pieces;
     a.own_items = (unsigned)a.n_seq * p.n_kv_head * a.own_tiles * a.own_splits;
     a.slots = a.shared_splits + a.own_splits;
     // a block for each row, head and tile where they are no more than the SMs and no warp gets more than four steps
