@@ -286,22 +286,32 @@ __device__ __forceinline__ uint32_t peer_address(const void *p, int rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
     return at;
 }
-__device__ __forceinline__ int peer_load(uint32_t at) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    return v;
+__device__ __forceinline__ void peer_store(uint32_t at, int v) {
+    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
-__device__ __forceinline__ int peer_word(const int *p, int rank) { return peer_load(peer_address(p, rank)); }
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                   "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+                   "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+                   "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(at)
+                 : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
 
 constexpr int kMmThreads = 256, kMmTile = 128, kMmK = 128;  // 128 channels x NT tokens, 128 bytes of k a stage
 
-__host__ __device__ constexpr int mm_stages(int NT) { return 6; }
+__host__ __device__ constexpr int mm_stages(int NT) { return NT <= 64 ? 6 : 4; }
 __host__ __device__ constexpr int mm_stage_bytes(int NT) { return (kMmTile + NT) * kMmK; }
-__host__ __device__ constexpr size_t mm_smem(int NT) { return (size_t)mm_stages(NT) * mm_stage_bytes(NT) + 1024; }
+// the ring, then the sums that the blocks of a cluster hand one another
+__host__ __device__ constexpr size_t mm_smem(int NT) { return (size_t)mm_stages(NT) * mm_stage_bytes(NT) + NT * kMmTile * 4 + 1024; }
 
 // A cluster of blocks owns 128 channels x NT tokens; block q of the cluster multiplies a share of k.  The
 // channels are the MMA's 128 rows (TMEM lanes), so that a warp's store of one token's column is one contiguous run
-// of y, and a lane keeps its channel's scale and bias in registers.
+// of y, and a lane keeps its channel's scale and bias in registers.  With k split, token j belongs to block j % ks: every
+// block stores its sums straight into the owner's shared memory, and after one cluster barrier the owner adds them up.
 template <int NT, typename T, int EPI>
 __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant__ CUtensorMap wmap,
                                                           const __grid_constant__ CUtensorMap xmap, LinearI8Args a, int ks,
@@ -311,7 +321,7 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
     unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t full[S], empty[S], done;
     __shared__ uint32_t slot;
-    __shared__ int failed, issued;
+    __shared__ int failed, issued, lost[8];
     __shared__ float xs[NT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int q = blockIdx.x % ks, tile = blockIdx.x / ks;
@@ -323,6 +333,7 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
         fence_mbar_init();
         failed = issued = 0;
     }
+    if (ks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this block is there
     pdl_wait();  // before the tensor memory: a kernel that waits must not hold what the one before it may need
     pdl_trigger();
     if (warp == 1) tmem_alloc(&slot, kCols), tmem_relinquish();
@@ -357,21 +368,17 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
     mbar_wait(&done, 0, &failed);
     tc_fence_after();
     __syncthreads();
-    // warps w and w + 4 share lanes 32 (w % 4) .. + 31 and take every other run of 16 tokens
+    // warps w and w + 4 share lanes 32 (w % 4) .. + 31 and take every other run of tokens
     const int ch = (warp & 3) * 32 + lane, n = n0 + ch;
     const bool in = n < a.N;
-    const float ws = in ? __ldg(a.ws + n) : 0.f, b = in && a.bias ? __ldg(a.bias + n) : 0.f;
-    T *y = reinterpret_cast<T *>(a.y) + n;
-    int *part = reinterpret_cast<int *>(sm);  // [NT][128], over the stages
-    for (int j0 = (warp >> 2) * 16; j0 < NT; j0 += 32) {
-        float f[16];
-        __syncwarp();
-        tmem_ld16(tmem + ((uint32_t)(warp & 3) << 21) + j0, f);
-        if (ks > 1) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) part[(j0 + j) * kMmTile + ch] = __float_as_int(f[j]);
-        } else {
-            float v[16];
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
+    if (ks == 1) {
+        const float ws = in ? __ldg(a.ws + n) : 0.f, b = in && a.bias ? __ldg(a.bias + n) : 0.f;
+        T *y = reinterpret_cast<T *>(a.y) + n;
+        for (int j0 = (warp >> 2) * 16; j0 < NT; j0 += 32) {
+            float f[16], v[16];
+            __syncwarp();
+            tmem_ld16(lanes + j0, f);
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = output<EPI>(__float_as_int(f[j]), xs[j0 + j], ws, b);
             T *at = y + (long long)(m0 + j0) * a.ldy;
@@ -387,38 +394,64 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
             for (int j = 0; j < 16; ++j)
                 if (in && m0 + j0 + j < a.M) at[j * a.ldy] = from_f32<T>(failed ? NAN : v[j]);
         }
-    }
-    tc_fence_before();
-    if (ks > 1) {  // token j of the tile is added up by block j % ks
-        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        int lost = 0;
-        for (int r = 0; r < ks; ++r) lost |= peer_word(&failed, r);
-        const int c = tid & 127, nn = n0 + c, last = min(NT, a.M - m0);
-        const bool mine = nn < a.N;
-        const float sc = mine ? __ldg(a.ws + nn) : 0.f, bi = mine && a.bias ? __ldg(a.bias + nn) : 0.f;
-        for (int j0 = q + (tid >> 7) * ks; j0 < last; j0 += 8 * ks) {  // four tokens at a time
-            int acc[4] = {};
-            T old[4] = {};
-            for (int r = 0; r < ks; ++r) {
-                const uint32_t at = peer_address(part + c, r);
+        tc_fence_before();
+    } else {
+        constexpr int R = NT < 32 ? NT : 32;
+        const int shift = __popc(ks - 1), tk = NT >> shift;  // ks is a power of two
+        int *sums = reinterpret_cast<int *>(sm + S * kStage);  // [ks][tk][128]
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every block is there
+        uint32_t owner[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (j0 + 2 * i * ks < last) acc[i] += peer_load(at + (j0 + 2 * i * ks) * kMmTile * 4);
+        for (int r = 0; r < 8; ++r) owner[r] = peer_address(sums + q * tk * kMmTile + ch, r & (ks - 1));
+        for (int j0 = (warp >> 2) * R; j0 < NT; j0 += 2 * R) {
+            __syncwarp();
+            if (NT < 32) {
+                float f[16];
+                tmem_ld16(lanes + j0, f);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) peer_store(owner[j & 7] + ((j0 + j) >> shift) * kMmTile * 4, __float_as_int(f[j]));
+            } else {
+                uint32_t f[32];
+                tmem_ld32(lanes + j0, f);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) peer_store(owner[j & 7] + ((j0 + j) >> shift) * kMmTile * 4, (int)f[j]);
             }
-            T *at = reinterpret_cast<T *>(a.y) + (long long)(m0 + j0) * a.ldy + nn;
-            if (EPI == 2)
+        }
+        if (tid < ks) peer_store(peer_address(lost + q, tid), failed);
+        tc_fence_before();
+        // what does not depend on the sums, while they are on their way: a thread takes four channels of a token
+        constexpr int I = NT * kMmTile / 4 / 2 / kMmThreads < 1 ? 1 : NT * kMmTile / 4 / 2 / kMmThreads;  // at most, with ks = 2
+        const int c4 = (tid & 31) * 4, nn = n0 + c4;
+        float sc[4], bi[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (mine && j0 + 2 * i * ks < last) old[i] = at[2 * i * ks * a.ldy];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (mine && j0 + 2 * i * ks < last) {
-                    float v = output<EPI>(acc[i], xs[j0 + 2 * i * ks], sc, bi);
-                    if (EPI == 2) v += to_f32<T>(old[i]);
-                    at[2 * i * ks * a.ldy] = from_f32<T>(lost ? NAN : v);
-                }
+        for (int e = 0; e < 4; ++e) {
+            sc[e] = nn + e < a.N ? __ldg(a.ws + nn + e) : 0.f;
+            bi[e] = nn + e < a.N && a.bias ? __ldg(a.bias + nn + e) : 0.f;
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        int any = 0;
+        for (int r = 0; r < ks; ++r) any |= lost[r];
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const int t = (tid >> 5) + i * (kMmThreads / 32), j = t * ks + q;  // token t of this block's
+            if (t >= tk || m0 + j >= a.M) break;
+            int4 acc = make_int4(0, 0, 0, 0);
+            for (int r = 0; r < ks; ++r) {
+                const int4 x = *reinterpret_cast<const int4 *>(sums + (r * tk + t) * kMmTile + c4);
+                acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+            }
+            const int sum[4] = {acc.x, acc.y, acc.z, acc.w};
+            T *at = reinterpret_cast<T *>(a.y) + (long long)(m0 + j) * a.ldy + nn;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = output<EPI>(sum[e], any ? NAN : xs[j], sc[e], bi[e]);
+                if (EPI == 2 && nn + e < a.N) v[e] += to_f32<T>(at[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (nn + e < a.N) at[e] = from_f32<T>(v[e]);
+        }
     }
     __syncthreads();
     if (failed && tid == 0) drain_ring(full, S, issued);
@@ -623,18 +656,6 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void pair_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                   "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-                   "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-                   "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-                 : "r"(at)
-                 : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
 // TMA: outputs leave as boxes of 32 channels x 32 tokens through shared memory (ymap; not with a residual)
 template <typename T, int EPI, bool TMA>
 __global__ void __launch_bounds__(kPrThreads, 1) k_linear_i8_pair(const __grid_constant__ CUtensorMap wmap,
