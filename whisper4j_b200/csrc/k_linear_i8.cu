@@ -83,22 +83,24 @@ struct Step {
     float s, inv, up;
     bool tiny;
 };
-// Four of them, packed.  Adding 1.5 x 2^23 rounds to the whole number and leaves it in the low byte; only where that lies
-// at or beyond a half (one in some hundred thousand) the exact rule is asked.
-__device__ __forceinline__ uint32_t nearest4(const float *x, const Step &p) {
+// Four of them, packed.  Adding 1.5 x 2^23 rounds to the whole number and leaves it in the low byte; `close` where x / s
+// lies at or beyond a half from one of them (one in some hundred thousand): there the exact rule has to be asked.
+__device__ __forceinline__ uint32_t round4(const float *x, const Step &p, bool &close) {
     const float h = 0.5f * p.s;
     uint32_t t[4];
-    bool close = p.tiny;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float y = fmaf(x[i], p.inv, 12582912.f);
         t[i] = __float_as_uint(y);
         close |= fabsf(fmaf(12582912.f - y, p.s, x[i])) >= h;
     }
-    if (close)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = (uint32_t)nearest(x[i] * p.up, p.s * p.up, p.inv);
     return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint32_t nearest4(const float *x, const Step &p) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= (uint32_t)(nearest(x[i] * p.up, p.s * p.up, p.inv) & 0xff) << (8 * i);
+    return w;
 }
 
 // C: steps held in registers, 0: any rows, read again in every pass (C > 0: K, x, ldx and a LayerNorm's vectors are whole
@@ -174,14 +176,21 @@ __global__ void __launch_bounds__(WARP ? 128 : kQMax) k_quantize_rows(QuantizeAr
     const bool any = good && s > 0.f;
     if (tid == 0) a.scale[row] = good ? s : __int_as_float(0x7fffffff);
     int8_t *q = a.q + (long long)row * a.ldq;
+    bool close = p.tiny;
     pass([&](int k, float(&e)[V]) {
         if (a.ln_g && !C) norm(k, e);
 #pragma unroll
         for (int i = 0; i < V; i += 4) {
-            const uint32_t w = any ? nearest4(e + i, p) : 0;  // (zeros behind K: x is 0 there)
-            *reinterpret_cast<uint32_t *>(q + k + i) = w;
+            const uint32_t w = round4(e + i, p, close);
+            *reinterpret_cast<uint32_t *>(q + k + i) = any ? w : 0;  // (zeros behind K: x is 0 there)
         }
     });
+    if (close && any)  // one branch for all of the thread's elements
+        pass([&](int k, float(&e)[V]) {
+            if (a.ln_g && !C) norm(k, e);
+#pragma unroll
+            for (int i = 0; i < V; i += 4) *reinterpret_cast<uint32_t *>(q + k + i) = nearest4(e + i, p);
+        });
     // the rest up to a multiple of 16 is zero: a product may read it
     const int done = (K + V - 1) / V * V, end = (K + 15) / 16 * 16;
     if (tid * 4 < end - done) *reinterpret_cast<uint32_t *>(q + done + tid * 4) = 0;
