@@ -118,12 +118,16 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
                  : "memory");
 }
 
-constexpr int kAsWarps = 4, kAsStages = 2, kAsStage = 8192;  // bytes of a stage: its keys, then their values
-constexpr size_t kAsSmem = (size_t)kAsWarps * kAsStages * kAsStage + 1024;
+// A block is one warp: rows differ in length, and a block of four kept its shared memory until the last had ended (64
+// streams x 5 beams: 61.2 us with four, 59.9 with two, 55.4 with one).
+constexpr int kAsWarps = 1, kAsStages = 2;
+constexpr int as_step(int D) { return 2048 / D; }             // keys of a stage
+constexpr int as_stage(int D) { return as_step(D) * D * 4; }  // its bytes: the keys, then their values
+constexpr size_t as_smem(int D, int warps) { return (size_t)warps * kAsStages * as_stage(D) + 1024; }
 
 template <typename T, int D, int NT>
 struct WarpTile {
-    static constexpr int NB = D / 64, STEP = 32 / NB, H = STEP / 16, kBlock = STEP * 128, kKeys = NB * kBlock;
+    static constexpr int NB = D / 64, STEP = as_step(D), H = STEP / 16, kBlock = STEP * 128, kKeys = NB * kBlock, kAsStage = as_stage(D);
     uint32_t qf[NT][D / 16][2];
     float o[NT][D / 16][4];  // dimension 16 t + g + 8 (e >> 1), query 8 n + 2 q + (e & 1)
     float m[NT][2], l[NT][2];
@@ -351,8 +355,9 @@ __device__ __forceinline__ int find_row(const AttnSharedArgs &a, int seq, bool f
     return bad;
 }
 
+// (12 of these blocks' rings fit an SM: registers for as many, and for 16 where that costs nothing)
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(kAsWarps * 32, NT == 1 ? 16 : 12) k_attn_shared(const __grid_constant__ CUtensorMap kmap,
                                                                const __grid_constant__ CUtensorMap vmap, AttnSharedArgs a,
                                                                int box) {
     extern __shared__ unsigned char raw[];
@@ -441,7 +446,7 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_cons
     WarpTile<T, D, NT> w;
     int bad_page = 0;
     w.load_q(qr);
-    w.run(p, table, nullptr, 0, head, &kmap, &vmap, sm + wi * kAsStages * kAsStage, full[wi], box, k0, k1, lim, own_len - a.n_query + 1,
+    w.run(p, table, nullptr, 0, head, &kmap, &vmap, sm + wi * kAsStages * as_stage(D), full[wi], box, k0, k1, lim, own_len - a.n_query + 1,
           a.scale_log2, &bad_page, &failed[wi]);
     if (__any_sync(0xffffffffu, bad_page)) bad |= W4J_PAGES_BAD_PAGE;
     __syncwarp();
@@ -459,7 +464,6 @@ __global__ void __launch_bounds__(kAsWarps * 32) k_attn_shared(const __grid_cons
 // again by every row, from L2) and join their sums in shared memory.  One launch and no scratch; bound by latency.
 // ---------------------------------------------------------------------------
 constexpr int kDirectWarps = 8;
-constexpr size_t kDirectSmem = (size_t)kDirectWarps * kAsStages * kAsStage + 1024;
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_constant__ CUtensorMap kmap,
@@ -500,7 +504,7 @@ __global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_
         }
     }
     unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023) +
-                        wi * kAsStages * kAsStage;
+                        wi * kAsStages * as_stage(D);
     WarpTile<T, D, NT> w;
     int bad_page = 0;
     w.load_q(qr);
@@ -522,7 +526,7 @@ __global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_
     __syncthreads();
     if (tid == 0 && wrong) atomicOr(p.status, wrong);
     const bool lost = failed || wrong;
-    const float *o0 = reinterpret_cast<const float *>(sm - wi * kAsStages * kAsStage);
+    const float *o0 = reinterpret_cast<const float *>(sm - wi * kAsStages * as_stage(D));
     for (int x = tid; x < R * D / 2; x += kDirectWarps * 32) {
         const int r = x / (D / 2), d = 2 * (x % (D / 2)), qi = tile * R + r;
         if (qi >= c) break;
@@ -534,7 +538,7 @@ __global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_
             const float2 part = ml[y][r];
             if (part.y == 0.f) continue;
             const float f = ex2(part.x - m);
-            const float2 o = *reinterpret_cast<const float2 *>(o0 + y * (kAsStages * kAsStage / 4) + r * D + d);
+            const float2 o = *reinterpret_cast<const float2 *>(o0 + y * (kAsStages * as_stage(D) / 4) + r * D + d);
             l += f * part.y, u += f * o.x, v += f * o.y;
         }
         const float inv = lost ? NAN : l == 0.f ? 0.f : 1.f / l;  // a query that sees nothing gets zeros
@@ -939,11 +943,11 @@ cudaError_t launch(const AttnSharedArgs &a, cudaStream_t s) {
     };
     cudaError_t e;
     if (a.direct) {
-        const int box = maps(2048 / D);
+        const int box = maps(as_step(D));
         if (!box) return cudaErrorInvalidValue;
         const unsigned blocks = a.n_seq * p.n_kv_head * a.own_tiles;
-        return a.tile_rows == 8 ? launch_after<k_attn_direct<T, D, 1>>(blocks, kDirectWarps * 32, kDirectSmem, s, 1, km, vm, a, box)
-                                : launch_after<k_attn_direct<T, D, 2>>(blocks, kDirectWarps * 32, kDirectSmem, s, 1, km, vm, a, box);
+        return a.tile_rows == 8 ? launch_after<k_attn_direct<T, D, 1>>(blocks, kDirectWarps * 32, as_smem(D, kDirectWarps), s, 1, km, vm, a, box)
+                                : launch_after<k_attn_direct<T, D, 2>>(blocks, kDirectWarps * 32, as_smem(D, kDirectWarps), s, 1, km, vm, a, box);
     }
     if (a.tc_tiles) {
         const int box = maps(kTcKeys);
@@ -952,13 +956,13 @@ cudaError_t launch(const AttnSharedArgs &a, cudaStream_t s) {
                          a, box);
         if (e != cudaSuccess) return e;
     }
-    const int box = maps(2048 / D);
+    const int box = maps(as_step(D));
     if (!box) return cudaErrorInvalidValue;
     const unsigned blocks = (a.shared_items + a.own_items + kAsWarps - 1) / kAsWarps;
     if (a.tile_rows == 8) {
-        e = launch_after<k_attn_shared<T, D, 1>>(blocks, kAsWarps * 32, kAsSmem, s, 1, km, vm, a, box);
+        e = launch_after<k_attn_shared<T, D, 1>>(blocks, kAsWarps * 32, as_smem(D, kAsWarps), s, 1, km, vm, a, box);
     } else {
-        e = launch_after<k_attn_shared<T, D, 2>>(blocks, kAsWarps * 32, kAsSmem, s, 1, km, vm, a, box);
+        e = launch_after<k_attn_shared<T, D, 2>>(blocks, kAsWarps * 32, as_smem(D, kAsWarps), s, 1, km, vm, a, box);
     }
     if (e != cudaSuccess) return e;
     return launch_after<k_attn_shared_join<T, D>>((unsigned)((rows + 7) / 8), 256, 0, s, 1, a);
