@@ -436,7 +436,8 @@ int w4j_op_attn_shared(const w4j_attn_shared *args, void *stream);
  * ------------------------------------------------------------------------- */
 
 /*
- * q = round(x / s), s = max |x| / 127 for each of M rows of K elements (ldx elements apart, of type
+ * q = round(x / s), s = max |x| (1 / 127), 1 / 127 as a 32-bit float and the product rounded to one, for each of M rows
+ * of K elements (ldx elements apart, of type
  * x_type: F32, F16 or BF16), optionally behind a LayerNorm (ln_g and ln_b, K floats each, or both NULL).  The
  * quotient is rounded as if exact, ties to even, and kept within +-127.  q has rows ldq bytes apart (a multiple of 16 of at least
  * K, 16-byte aligned); columns K up to the next multiple of 16 get zeros.  A row of zeros gets scale 0, a row with

@@ -22,9 +22,7 @@ E = 2.0 ** -24
 def quantised(x):
     """(q, scale) of float32-valued rows, in 64 bits."""
     x = x.double()
-    s = (x.abs().amax(1) / 127).float()
-    # a scale below 32 bits' normal range is rounded as a 32-bit division rounds
-    s = torch.from_numpy((x.abs().amax(1).float().cpu().numpy() / np.float32(127)).astype(np.float32)).to(x.device) if x.numel() else s
+    s = torch.from_numpy(x.abs().amax(1).float().cpu().numpy() * np.float32(1 / 127)).to(x.device)
     q = torch.where(s[:, None] > 0, x / s.double()[:, None], 0).round().clamp(-127, 127)
     return q.to(torch.int8), s
 

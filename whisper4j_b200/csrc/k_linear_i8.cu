@@ -1,7 +1,7 @@
 // k_linear_i8.cu — a Linear layer in 8-bit integers: rows quantised by their largest magnitude, the product in
 // exact 32-bit integers on the 5th-generation tensor cores, one scale for each row and each output channel.
 //
-//   s_m = max_k |x_mk| / 127,  q_mk = round(x_mk / s_m),  y_mn = act(s_m t_n sum_k q_mk w_nk + b_n)
+//   s_m = max_k |x_mk| (1 / 127),  q_mk = round(x_mk / s_m),  y_mn = act(s_m t_n sum_k q_mk w_nk + b_n)
 #include <cuda_bf16.h>
 #include <cudaTypedefs.h>
 
@@ -66,6 +66,10 @@ __device__ __forceinline__ U row_reduce(U v, U *sm, Op op) {
     for (int w = 1; w < (int)blockDim.x / 32; ++w) v = op(v, sm[w]);
     return v;
 }
+
+// A scale is the largest magnitude times this 32-bit number (where it is a multiple of 127 half steps of a 16-bit type,
+// many quotients are near ties: everybody who quantises the same rows has to round it alike).
+constexpr float kPerStep = 1.f / 127.f;
 
 // The whole number nearest to x / s, ties to even, by the exact quotient: r from the rounded reciprocal is at most
 // one off, and x - r s, exact in one FMA wherever it matters, says on which side of a half x / s lies.  Within
@@ -170,7 +174,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kQMax) k_quantize_rows(QuantizeAr
     });
     bits = row_reduce<WARP>(bits, reinterpret_cast<uint32_t *>(sm), [](uint32_t p, uint32_t q) { return max(p, q); });
     const bool good = bits < 0x7f800000u;
-    const float s = __fdiv_rn(__uint_as_float(bits), 127.f);
+    const float s = __fmul_rn(__uint_as_float(bits), kPerStep);
     Step p;
     p.s = s, p.tiny = s < 1e-30f, p.up = p.tiny ? 18446744073709551616.f : 1.f, p.inv = __fdiv_rn(1.f, s * p.up);
     const bool any = good && s > 0.f;
@@ -580,7 +584,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_layer(LinearI8Args
     bits = reduce(bits, [](uint32_t p, uint32_t q) { return max(p, q); });
     const bool good = bits < 0x7f800000u;
     Step p;
-    p.s = __fdiv_rn(__uint_as_float(bits), 127.f);
+    p.s = __fmul_rn(__uint_as_float(bits), kPerStep);
     p.tiny = p.s < 1e-30f, p.up = p.tiny ? 18446744073709551616.f : 1.f, p.inv = __fdiv_rn(1.f, p.s * p.up);
     if (row < rows) {
         if (t == 0) sxs[row] = good ? p.s : __int_as_float(0x7fffffff);

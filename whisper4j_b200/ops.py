@@ -219,7 +219,7 @@ def _norm(ln, k, index):
 
 def quantize_rows(x, ln=None):
     """x (M, K) -> (q, scale): q (M, K rounded up to 16) int8 = round(LayerNorm?(x) / scale), zeros behind K, and
-    scale (M,) = max |row| / 127.  ``ln`` is (gamma, beta)."""
+    scale (M,) = max |row| * (1 / 127) in 32 bits.  ``ln`` is (gamma, beta)."""
     m, k, ld = _matrix(x, "x")
     q = torch.empty(m, (k + 15) // 16 * 16, dtype=torch.int8, device=x.device)
     scale = torch.empty(m, dtype=torch.float32, device=x.device)
