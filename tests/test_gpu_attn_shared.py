@@ -229,6 +229,11 @@ def test_bad_sequences_are_marked(n):
     s = fresh()
     s["start"][2] = n + 1  # the last sequence is in no group
     bad(s, "ascend", [n + 1])
+    s = fresh()
+    s["start"][1] = n + 5  # groups that do not ascend
+    attend(s)
+    with pytest.raises(IllegalStateError, match="ascend"):
+        s["cache"].check()
 
 
 def test_captured_and_replayed():

@@ -174,7 +174,7 @@ def linear(device=0, x=P, ldx=112, xs=P, m=2, k=100, w=P, ldw=112, ws=P, n=30, b
 @pytest.mark.parametrize("kw,text", [
     (dict(x=None), "null"), (dict(xs=None), "null"), (dict(w=None), "null"), (dict(ws=None), "null"), (dict(y=None), "null"),
     (dict(y_type=8), "y_type"), (dict(m=0), "shape"), (dict(n=0, ldy=0), "shape"), (dict(k=0), "shape"), (dict(m=(1 << 24) + 1), "shape"),
-    (dict(k=131057, ldx=131072, ldw=131072), "131056"), (dict(ldx=96), "rows"), (dict(ldw=104), "rows"), (dict(x=P + 8), "aligned"),
+    (dict(m=1 << 20, n=1 << 20, ldy=1 << 20), "2^38"), (dict(k=131057, ldx=131072, ldw=131072), "131056"), (dict(ldx=96), "rows"), (dict(ldw=104), "rows"), (dict(x=P + 8), "aligned"),
     (dict(w=P + 4), "aligned"), (dict(ldy=29), "ldy"), (dict(y=P + 2), "aligned"), (dict(epilogue=3), "epilogue"),
     (dict(epilogue=-1), "epilogue")])
 def test_linear_refusals(kw, text):
@@ -210,3 +210,15 @@ def test_a_few_short_rows_need_no_scratch():
     w = lib().w4j_op_attn_shared_workspace
     assert workspace(w, ctypes.byref(attn(cache()))) == (W4J_OK, 0)
     assert workspace(w, ctypes.byref(attn(cache(), n_seq=100)))[1] > 0
+
+
+def test_scratch_stays_in_proportion():
+    """However long the rows may be, their pieces are not many times more than the device takes at once."""
+    w = lib().w4j_op_attn_shared_workspace
+    c = cache(page_tokens=1024, table_width=1 << 20, n_pages=1000)
+    one = workspace(w, ctypes.byref(attn(c, n_seq=1, max_shared=0, max_own=1 << 30)))[1]
+    many = workspace(w, ctypes.byref(attn(c, n_seq=60000, max_shared=0, max_own=1 << 30)))[1]
+    assert 0 < one < 64 << 20
+    assert 0 < many <= 60000 * 6 * 66 * 4
+    both = workspace(w, ctypes.byref(attn(c, n_seq=2, max_shared=1 << 30, max_own=1 << 30)))[1]
+    assert 0 < both < 256 << 20

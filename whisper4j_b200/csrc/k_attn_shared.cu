@@ -334,7 +334,7 @@ struct WarpTile {
 // items: (group tile, head, split) of the shared keys, then (row, head, tile, split) of the rows' own
 // ---------------------------------------------------------------------------
 // Row, its group's first row, length and shared length of sequence `seq`, 0 or what is wrong with it (then rows 0); the whole warp calls it.
-// first: whether this call also looks at the groups' ends.
+// first: whether this call also looks at all of the groups.
 __device__ __forceinline__ int find_row(const AttnSharedArgs &a, int seq, bool first, int &row, int &row0, int &len, int &shared) {
     const PagesArgs &p = a.p;
     const int r = __ldg(a.rows + seq);
@@ -351,7 +351,11 @@ __device__ __forceinline__ int find_row(const AttnSharedArgs &a, int seq, bool f
     const int len0 = r0 >= 0 && r0 < p.n_rows ? __ldg(p.len + r0) : -1;
     int bad = !group_ok ? W4J_PAGES_BAD_START : !row_ok || len0 < 0 ? W4J_PAGES_BAD_ROW
               : s < 0 || s > a.max_shared || s > max(0, min(len, len0) - a.n_query + 1) ? W4J_PAGES_BAD_SHARED : 0;
-    if (first && (lo != 0 || __ldg(a.group_start + a.n_group) != a.n_seq)) bad |= W4J_PAGES_BAD_START;
+    if (first) {  // the groups as a whole
+        bool out = __ldg(a.group_start) != 0 || __ldg(a.group_start + a.n_group) != a.n_seq;
+        for (int i = threadIdx.x & 31; i < a.n_group; i += 32) out |= __ldg(a.group_start + i) > __ldg(a.group_start + i + 1);
+        if (__any_sync(0xffffffffu, out)) bad |= W4J_PAGES_BAD_START;
+    }
     return bad;
 }
 
@@ -1002,14 +1006,16 @@ void attn_shared_plan(AttnSharedArgs &a) {
     }
     a.shared_items = a.shared_tiles * a.shared_splits * p.n_kv_head;
     a.own_tiles = (unsigned)((c + a.tile_rows - 1) / a.tile_rows);
-    const int own = a.max_own > 0 ? splits((long long)a.n_seq * p.n_kv_head * a.own_tiles, a.max_own) : 1, pieces = (a.max_own + 255) / 256;
-    a.own_splits = own > pieces ? own : pieces < 1 ? 1 : pieces;
+    // pieces of 256 keys, as long as they are not many times more than the device takes at once
+    const long long own_items = (long long)a.n_seq * p.n_kv_head * a.own_tiles, most = 6 * want / own_items;
+    const int own = a.max_own > 0 ? splits(own_items, a.max_own) : 1, pieces = (a.max_own + 255) / 256, some = most < pieces ? (int)most : pieces;
+    a.own_splits = own > some ? own : some < 1 ? 1 : some;
     a.own_items = (unsigned)a.n_seq * p.n_kv_head * a.own_tiles * a.own_splits;
     a.slots = a.shared_splits + a.own_splits;
     // a block for each row, head and tile where they are no more than the SMs and no warp gets more than four steps
     a.direct = 0;
     const unsigned direct_tiles = (unsigned)((c + (c <= 8 ? 7 : 15)) / (c <= 8 ? 8 : 16));
-    if ((long long)a.n_seq * p.n_kv_head * direct_tiles <= 148 && a.max_shared + a.max_own <= kDirectWarps * 32 * 4) {
+    if ((long long)a.n_seq * p.n_kv_head * direct_tiles <= 148 && (long long)a.max_shared + a.max_own <= kDirectWarps * 32 * 4) {
         a.direct = 1, a.slots = 0;
         a.tile_rows = c <= 8 ? 8 : 16, a.own_tiles = direct_tiles;
     }

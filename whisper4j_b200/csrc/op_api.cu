@@ -199,6 +199,7 @@ static int check_product(const char *who, int M, int K, const int8_t *w, int64_t
                          int64_t ldy) {
     if (!float_type(y_type)) return set_err(W4J_ERR_ARG, "%s: y_type must be F32 (0), F16 (1) or BF16 (30), not %d", who, y_type);
     if (M < 1 || N < 1 || K < 1 || M > 1 << 24 || N > 1 << 24) return set_err(W4J_ERR_ARG, "%s: bad shape (%d x %d x %d)", who, M, K, N);
+    if ((int64_t)M * N > (int64_t)1 << 38) return set_err(W4J_ERR_ARG, "%s: M * N must be at most 2^38", who);
     if (K > 131056) return set_err(W4J_ERR_ARG, "%s: K = %d: sums of more than 131056 products may leave 32 bits", who, K);
     if (ldw < K || ldw % 16 || !aligned(w, 16))
         return set_err(W4J_ERR_ARG, "%s: w must be 16-byte aligned with rows a multiple of 16 bytes of at least K apart", who);
