@@ -460,8 +460,8 @@ int w4j_op_linear_i8(int device, const int8_t *x, int64_t ldx, const float *x_sc
                      int64_t ldy, void *stream);
 
 /*
- * The two in one call, x in floats (as w4j_op_quantize_rows) and y as w4j_op_linear_i8 makes it: up to 8 rows that fit
- * 48 KB as integers take one launch.  Behind a LayerNorm its sums may run in another order there, so that a quotient
+ * The two in one call, x in floats (as w4j_op_quantize_rows) and y as w4j_op_linear_i8 makes it: up to 4 rows that fit
+ * 1536 bytes as integers take one launch.  Behind a LayerNorm its sums may run in another order there, so that a quotient
  * next to a half may fall to its other side.  work: w4j_op_linear_i8_layer_workspace's bytes (0 for those few rows),
  * 16-byte aligned, for this call alone until it has run.
  */

@@ -199,7 +199,7 @@ def test_layer_refusals(kw, text):
 
 def test_layer_workspace():
     w = lib().w4j_op_linear_i8_layer_workspace
-    for m, k, n in ((9, 100, 9 * (112 + 4)), (8, 1280, 0), (1, 40000, 0), (8, 7000, 8 * (7008 + 4))):
+    for m, k, n in ((9, 100, 9 * (112 + 4)), (1, 1280, 0), (4, 380, 0), (2, 1280, 2 * 1284), (1, 40000, 40004), (5, 100, 5 * (112 + 4)), (8, 7000, 8 * (7008 + 4))):
         assert workspace(w, m, k) == (W4J_OK, n)
     for m, k in ((0, 1), (1, 0), (1, 131057), ((1 << 24) + 1, 1)):
         refused(workspace(w, m, k)[0], "shape")

@@ -34,8 +34,10 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 
 // ---------------------------------------------------------------------------
 // rows to 8 bits: a warp per row where there are many rows, else a block, 16 bytes per thread and step, held in
-// registers between the passes (sum, squares, largest magnitude, quotients) where the row fits.  Bound by HBM for
-// many rows and by the latency of its reductions for few.
+// registers between the passes (sum, squares, largest magnitude, quotients) where the row fits.  12000 rows of 1280
+// 32-bit numbers behind a LayerNorm take 24 us, 3.2 TB/s: bound by the passes' instructions and their latency at 24 warps
+// an SM, half of what HBM would give.  Packed arithmetic, or the warp's next row fetched ahead at more registers, took as
+// long or longer.  Few rows are bound by the latency of the reductions (320 rows of 5120: 3 to 5 us).
 // ---------------------------------------------------------------------------
 constexpr int kQMax = 1024;
 
@@ -201,7 +203,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kQMax) k_quantize_rows(QuantizeAr
 }
 
 // A warp per row from 8 rows for every SM's scheduler on, where a row fits its registers (12000 rows of 1280 with a
-// LayerNorm: 51 us with a block per row, @WARP@ with a warp); fewer rows get as many threads as they have units.
+// LayerNorm: 51 us with a block per row, 24 with a warp); fewer rows get as many threads as they have units.
 template <typename T>
 cudaError_t quantize(const QuantizeArgs &a, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
@@ -324,7 +326,9 @@ __host__ __device__ constexpr size_t mm_smem(int NT) { return (size_t)mm_stages(
 // A cluster of blocks owns 128 channels x NT tokens; block q of the cluster multiplies a share of k.  The
 // channels are the MMA's 128 rows (TMEM lanes), so that a warp's store of one token's column is one contiguous run
 // of y, and a lane keeps its channel's scale and bias in registers.  With k split, token j belongs to block j % ks: every
-// block stores its sums straight into the owner's shared memory, and after one cluster barrier the owner adds them up.
+// block stores its sums straight into the owner's shared memory, and after one cluster barrier the owner adds them up
+// (fetching them from their makers instead took 15.7 us rather than 13.8 for 320 rows x 5120 x 1280 channels with their
+// quantisation).  That product is bound by its operands' way from L2 (39 MB, 5 us), the exchange and the start.
 template <int NT, typename T, int EPI>
 __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant__ CUtensorMap wmap,
                                                           const __grid_constant__ CUtensorMap xmap, LinearI8Args a, int ks,
@@ -474,6 +478,7 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
 // ---------------------------------------------------------------------------
 // a few rows: a warp per channel, 16 bytes of its weights per lane and step against MT rows (dp4a), the next steps' weights
 // on their way.  Bound by the latency of one trip to HBM and by its launch; no tensor memory, barriers or cluster.
+// (One row x 1280 x 3840 channels: 4.5 us, on the tensor cores 7.6.)
 // ---------------------------------------------------------------------------
 constexpr int kFewWarps = 8;
 
@@ -512,9 +517,12 @@ __global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_few(LinearI8Args a
     }
 }
 
-// The whole layer for a few rows in one launch: every block quantises the rows for itself (8, 4, 2 or 1 warps to a row)
-// into shared memory while the first 2 KB of its channels' weights are on their way.
-constexpr size_t kLayerSmem = 48 * 1024;
+// The whole layer for a few rows in one launch: every block quantises the rows for itself (8, 4 or 2 warps to a row)
+// into shared memory while the first 2 KB of its channels' weights are on their way.  One row x 1280 x 3840 channels
+// takes 3.8 us in a graph, 1.3 TB/s of weights, where the two launches took 6.
+// Longer rows or more of them are quantised once instead, by a launch of their own (in a graph, 1280 x 3840: 2 rows 7.1 us
+// against 4.6, 4 rows 17 against 5.6; 5120 x 1280: 1 row 9.3 against 6.2); below, a launch saved is 2.5 us of the host's.
+constexpr size_t kLayerSmem = 1536;
 
 __device__ __forceinline__ float load1(const void *x, int type, long long i) {
     return type == W4J_GGML_F32 ? __ldg(static_cast<const float *>(x) + i)
@@ -630,7 +638,9 @@ __global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_layer(LinearI8Args
 // many rows: a pair of SMs owns 256 channels x 256 tokens at a time (tcgen05.mma with cta_group::2), each with 128 of the
 // channels and half of the tokens in its shared memory, so that a tile's operands cross from L2 once: 64 bytes a cycle
 // and SM at the integer MMAs' 8192 products, where a single SM's 128 x 256 tile would want 96.  Persistent: two
-// accumulators in tensor memory, and sixteen warps turn one into outputs while the next tile's products run.
+// accumulators in tensor memory, and sixteen warps turn one into outputs while the next tile's products run (12000 rows x
+// 1280 x 5120 with GELU: 83 us with eight warps, 70 with sixteen; 111 when the outputs were stored one by one).  2.3
+// POP/s, the integer pipe 56 % active: bound by the operands' way from L2, 616 MB at 9 TB/s.
 // ---------------------------------------------------------------------------
 constexpr int kPrWarps = 16, kPrThreads = 64 + 32 * kPrWarps, kPrTokens = 1024 / kPrWarps, kPrStage = 2 * kMmTile * kMmK;
 constexpr int pr_stages(int bytes) { return bytes == 4 ? 4 : 5; }
@@ -897,17 +907,23 @@ cudaError_t product_pair(const LinearI8Args &a, cudaStream_t s) {
 
 constexpr int kFewRows = 8;
 
+// Which kernel takes a product, times in a graph: the warps' one pass over the weights where it is short (K = 1280: 2 rows
+// 3.3 us against 4.4, 4 rows 4.5 against 4.4; K = 384: 4 rows 2.3 against 3.4; K = 5120: 1 row 3.6 against 4.7, 2 rows 5.4
+// against 4.7); the pair where single blocks of 128 x 128 would need a second turn of the SMs (K = 1280, N = 5120: 320 rows
+// 9.8 us against 8.1, 512 rows 9.8 against 15.2; K = 5120, N = 1280: 1500 rows 18.1 against 17.1, 2048 rows 18.3 against 31.9).
 template <typename T, int EPI>
 cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
     const unsigned few = (a.N + kFewWarps - 1) / kFewWarps;
     if (a.M == 1) return launch_after<k_linear_i8_few<1, T, EPI>>(few, kFewWarps * 32, 0, s, 1, a);
-    if (a.M <= 4) return launch_after<k_linear_i8_few<4, T, EPI>>(few, kFewWarps * 32, 0, s, 1, a);
-    if (a.M <= kFewRows) return launch_after<k_linear_i8_few<8, T, EPI>>(few, kFewWarps * 32, 0, s, 1, a);
+    if (a.M <= kFewRows && a.M * (long long)a.K < 5120) {
+        if (a.M <= 4) return launch_after<k_linear_i8_few<4, T, EPI>>(few, kFewWarps * 32, 0, s, 1, a);
+        return launch_after<k_linear_i8_few<8, T, EPI>>(few, kFewWarps * 32, 0, s, 1, a);
+    }
     if (a.M <= 16) return product<16, T, EPI>(a, s);
     if (a.M <= 32) return product<32, T, EPI>(a, s);
     if (a.M <= 64) return product<64, T, EPI>(a, s);
-    const long long tiles = (long long)((a.N + 255) / 256) * ((a.M + 255) / 256);
-    if (a.M > 128 && tiles >= 48) return product_pair<T, EPI>(a, s);
+    const long long tiles = ((a.N + 127LL) / 128) * ((a.M + 127LL) / 128);
+    if (a.M > 128 && tiles > 148) return product_pair<T, EPI>(a, s);
     return product<128, T, EPI>(a, s);
 }
 
@@ -917,8 +933,7 @@ cudaError_t layer(const LinearI8Args &a, const QuantizeArgs &q, cudaStream_t s) 
     const size_t smem = (size_t)a.M * ((a.K + 15) / 16 * 16);
     if (a.M == 1) return launch_after<k_linear_i8_layer<1, T, EPI>>(blocks, kFewWarps * 32, smem, s, 1, a, q);
     if (a.M == 2) return launch_after<k_linear_i8_layer<2, T, EPI>>(blocks, kFewWarps * 32, smem, s, 1, a, q);
-    if (a.M <= 4) return launch_after<k_linear_i8_layer<4, T, EPI>>(blocks, kFewWarps * 32, smem, s, 1, a, q);
-    return launch_after<k_linear_i8_layer<8, T, EPI>>(blocks, kFewWarps * 32, smem, s, 1, a, q);
+    return launch_after<k_linear_i8_layer<4, T, EPI>>(blocks, kFewWarps * 32, smem, s, 1, a, q);
 }
 
 template <typename T>
@@ -945,7 +960,7 @@ cudaError_t launch_linear_i8(const LinearI8Args &a, cudaStream_t s) {
 
 size_t linear_i8_layer_work(int M, int K) {
     const size_t k16 = ((size_t)K + 15) / 16 * 16;
-    return M <= kFewRows && M * k16 <= kLayerSmem ? 0 : M * (k16 + 4);
+    return M <= 4 && M * k16 <= kLayerSmem ? 0 : M * (k16 + 4);
 }
 
 cudaError_t launch_linear_i8_layer(LinearI8Args a, QuantizeArgs q, void *work, cudaStream_t s) {
