@@ -129,6 +129,17 @@ def test_against_64_bits(shape, dim, dtype):
     verify(s, attend(s))
 
 
+# few rows and long ones: a row's keys are shared out over the blocks of a cluster, whose size these change
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,heads,nq", [(1, 1, 1), (3, 8, 1), (4, 8, 1), (5, 8, 1), (9, 8, 1), (13, 8, 1), (5, 4, 11)])
+def test_few_long_rows(n, heads, nq, dim):
+    shared = 0 if n == 1 else 701
+    lens = [[3017, 2100, 701, 0, 1, 640, 513][i % 7] if i else 3017 for i in range(n)]
+    lens = [max(x, shared) if x > 1 else x for x in lens]
+    s = make([1] * n, [shared if x > shared else 0 for x in lens], lens, nq=nq, heads=heads, kv=heads, dim=dim, page=24)
+    verify(s, attend(s))
+
+
 @pytest.mark.parametrize("page", [8, 24, 64, 136, 1024])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_page_sizes(page, dim):
@@ -234,6 +245,14 @@ def test_bad_sequences_are_marked(n):
     attend(s)
     with pytest.raises(IllegalStateError, match="ascend"):
         s["cache"].check()
+
+
+def test_a_bad_page_late_in_a_long_row():
+    """Read by one of the blocks that share the row's keys: all of the row's results are marked."""
+    s = make([1, 1], [0, 0], [2000, 2000], heads=8, kv=8)
+    clean = attend(s)
+    s["cache"].table[int(s["rows"][0]), 120] = 1 << 20
+    assert torch.equal(bad(s, "table entry", [0])[1], clean[1])
 
 
 def test_captured_and_replayed():

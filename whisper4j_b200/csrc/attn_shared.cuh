@@ -14,7 +14,7 @@ struct AttnSharedArgs {
     const int *rows, *group_start, *shared;
     float *part_o, *part_ml;         // [query token][head][slot][head_dim], [..][slot][2] (maximum in base 2, sum)
     // the split of the work (attn_shared_plan)
-    int direct;                      // all by k_attn_direct, no scratch
+    int direct;                      // all by k_attn_direct on clusters of so many blocks, no scratch (0: not)
     int tile_rows;                   // query rows of a warp's tile, 8 or 16
     unsigned tc_tiles;               // shared keys by k_attn_shared_tc, in tiles of 128 rows (0: warp tiles)
     unsigned shared_tiles, shared_splits, own_tiles, own_splits, slots;

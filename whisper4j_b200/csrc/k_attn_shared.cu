@@ -98,7 +98,9 @@ __device__ __forceinline__ bool wait_phase(uint64_t *bar, unsigned parity, int *
 // dimensions and its 8 columns the few queries; P goes from one fragment layout to the other by an 8 x 8
 // transposition.  Each warp has a ring of its own: a stage holds STEP keys and their values, brought page by page
 // as TMA boxes (128-byte swizzle, read back by ldmatrix), so that a stage is in flight while another is worked on
-// without holding registers, and no warp waits for another.  Bound by HBM.
+// without holding registers, and no warp waits for another.  Bound by HBM and, where rows are short, by the look-ups
+// that each begins with: 256 rows x 20 heads of 64, 257 tokens each on average, 61 us, 5.5 TB/s (112 us with fragments
+// loaded straight into registers); 64 x 5 rows of 111 tokens behind 227 shared ones 55 us, 4.6 TB/s.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     uint32_t r;
@@ -464,10 +466,24 @@ __global__ void __launch_bounds__(kAsWarps * 32, NT == 1 ? 16 : 12) k_attn_share
 }
 
 // ---------------------------------------------------------------------------
-// a few short rows: a block takes a row, head and tile, its warps share all of the row's keys (the group's among them: read
-// again by every row, from L2) and join their sums in shared memory.  One launch and no scratch; bound by latency.
+// a few rows: a block, or for longer rows a cluster of blocks, takes a row, head and tile; its warps share all of the row's
+// keys (the group's among them: read again by every row, from L2) and join their sums in shared memory, the blocks' over
+// the cluster's.  One launch and no scratch; bound by latency (5 rows x 8 heads x 284 tokens: 4.8 us in a graph, 8.4 with
+// parts and a join; x 1500 tokens 7.8 and 11.1).
 // ---------------------------------------------------------------------------
-constexpr int kDirectWarps = 8;
+constexpr int kDirectWarps = 8, kDirectMost = 8;  // warps of a block, blocks of a cluster
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// What block `rank` of the cluster has at this place of its shared memory.
+__device__ __forceinline__ float2 ld_cluster(const float2 *p, int rank) {
+    uint32_t at;
+    float2 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_constant__ CUtensorMap kmap,
@@ -476,14 +492,15 @@ __global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_
     extern __shared__ unsigned char raw[];
     __shared__ uint64_t full[kDirectWarps][kAsStages];
     __shared__ int failed, wrong;
-    __shared__ float2 ml[kDirectWarps][8 * NT];
+    __shared__ float2 ml[kDirectWarps][8 * NT], block_ml[8 * NT];
     pdl_wait();
     pdl_trigger();
     constexpr int R = 8 * NT;
     const PagesArgs &p = a.p;
     const int tid = threadIdx.x, wi = tid >> 5, lane = tid & 31, g = lane >> 2, qd = lane & 3;
     const int c = a.n_query * a.rep;
-    const int tile = blockIdx.x % a.own_tiles, head = blockIdx.x / a.own_tiles % p.n_kv_head, seq = blockIdx.x / a.own_tiles / p.n_kv_head;
+    const int rank = blockIdx.x % a.direct, item = blockIdx.x / a.direct;
+    const int tile = item % a.own_tiles, head = item / a.own_tiles % p.n_kv_head, seq = item / a.own_tiles / p.n_kv_head;
     if (tid == 0) failed = wrong = 0;
     if (lane == 0) {
         for (int i = 0; i < kAsStages; ++i) mbar_init(&full[wi][i], 1);
@@ -492,8 +509,8 @@ __global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_
     __syncthreads();
     int row, row0, len, shared;
     int bad = find_row(a, seq, blockIdx.x == 0, row, row0, len, shared);
-    const int n = bad ? 0 : len, step = ((n + kDirectWarps - 1) / kDirectWarps + 31) / 32 * 32;
-    const int k0 = min(n, wi * step), k1 = min(n, k0 + step);
+    const int n = bad ? 0 : len, warps = a.direct * kDirectWarps, step = ((n + warps - 1) / warps + 31) / 32 * 32;
+    const int k0 = min((long long)n, (long long)(rank * kDirectWarps + wi) * step), k1 = min(n, k0 + step);
     const T *q = reinterpret_cast<const T *>(a.q);
     const T *qr[NT];
     int lim[NT][2];
@@ -530,10 +547,16 @@ __global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_
     __syncthreads();
     if (tid == 0 && wrong) atomicOr(p.status, wrong);
     const bool lost = failed || wrong;
-    const float *o0 = reinterpret_cast<const float *>(sm - wi * kAsStages * as_stage(D));
+    float *o0 = reinterpret_cast<float *>(sm - wi * kAsStages * as_stage(D));
+    auto put = [&](int r, int d, float l, float u, float v) {
+        const int qi = tile * R + r;
+        if (qi >= c) return;
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // a query that sees nothing gets zeros
+        T *out = reinterpret_cast<T *>(a.out) + ((size_t)seq * a.n_query + qi / a.rep) * a.out_stride + (size_t)(head * a.rep + qi % a.rep) * D;
+        *reinterpret_cast<uint32_t *>(out + d) = pack2<T>(u * inv, v * inv);
+    };
     for (int x = tid; x < R * D / 2; x += kDirectWarps * 32) {
-        const int r = x / (D / 2), d = 2 * (x % (D / 2)), qi = tile * R + r;
-        if (qi >= c) break;
+        const int r = x / (D / 2), d = 2 * (x % (D / 2));
         float m = kNone, l = 0.f, u = 0.f, v = 0.f;
 #pragma unroll
         for (int y = 0; y < kDirectWarps; ++y) m = fmaxf(m, ml[y][r].x);
@@ -545,10 +568,37 @@ __global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_
             const float2 o = *reinterpret_cast<const float2 *>(o0 + y * (kAsStages * as_stage(D) / 4) + r * D + d);
             l += f * part.y, u += f * o.x, v += f * o.y;
         }
-        const float inv = lost ? NAN : l == 0.f ? 0.f : 1.f / l;  // a query that sees nothing gets zeros
-        T *out = reinterpret_cast<T *>(a.out) + ((size_t)seq * a.n_query + qi / a.rep) * a.out_stride + (size_t)(head * a.rep + qi % a.rep) * D;
-        *reinterpret_cast<uint32_t *>(out + d) = pack2<T>(u * inv, v * inv);
+        if (lost) m = 0.f, l = NAN;
+        if (a.direct == 1) {
+            put(r, d, l, u, v);
+            continue;
+        }
+        // over the first warp's, whose two numbers of this place no other thread reads
+        *reinterpret_cast<float2 *>(o0 + r * D + d) = make_float2(u, v);
+        if (d == 0) block_ml[r] = make_float2(m, l);
     }
+    if (a.direct == 1) return;
+    cluster_sync();
+    for (int x = rank * kDirectWarps * 32 + tid; x < R * D / 2; x += a.direct * kDirectWarps * 32) {
+        const int r = x / (D / 2), d = 2 * (x % (D / 2));
+        float2 part[kDirectMost], o[kDirectMost];
+        float m = kNone, l = 0.f, u = 0.f, v = 0.f;
+#pragma unroll
+        for (int y = 0; y < kDirectMost; ++y) {
+            const int from = min(y, a.direct - 1);
+            part[y] = y < a.direct ? ld_cluster(block_ml + r, from) : make_float2(kNone, 0.f);
+            o[y] = ld_cluster(reinterpret_cast<const float2 *>(o0 + r * D + d), from);
+            m = fmaxf(m, part[y].x);
+        }
+#pragma unroll
+        for (int y = 0; y < kDirectMost; ++y) {
+            if (part[y].y == 0.f) continue;
+            const float f = ex2(part[y].x - m);
+            l += f * part[y].y, u += f * o[y].x, v += f * o[y].y;
+        }
+        put(r, d, l, u, v);
+    }
+    cluster_sync();  // the others have read this block's
 }
 
 // ---------------------------------------------------------------------------
@@ -562,7 +612,8 @@ __global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_
 // operand as it lies in the pages (MN-major).
 //
 // 128 x 128 exponentials take the 16 a cycle of an SM's special function units 1024 cycles, the MMAs of a tile 512 (head
-// 64) or 1024 (head 128); a tile takes 1850 to 2100, bound by the round from S over P to the S that comes after the
+// 64) or 1024 (head 128); a tile takes 1850 to 2500 (4 x 256 rows x 16381 keys x 8 heads of 128: 86 us, 0.8 PFLOP/s),
+// bound by the round from S over P to the S that comes after the
 // next (softmax 1500, P V and Q K^T 600 to 900 with their hand-overs).  Moving 4 to 16 of every 32 exponentials to a
 // polynomial on the FMA pipes made that round longer (142 -> 143 .. 150 us on 4 x 256 rows x 16381 keys x 8 heads of
 // 128) and was not kept.
@@ -893,7 +944,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
     if (warp == 9) tc_fence_after(), tmem_dealloc(tmem, 512);
 }
 
-// The parts of one query joined, a warp per query and head, lane i dimensions i D / 32 on.
+// The parts of one query joined, a warp per query and head, lane i dimensions i D / 32 on.  Bound by latency: 5 us for
+// 5120 queries of 5 parts, most of it beside the kernel before it.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_attn_shared_join(AttnSharedArgs a) {
     pdl_wait();
@@ -915,13 +967,14 @@ __global__ void __launch_bounds__(256) k_attn_shared_join(AttnSharedArgs a) {
     }
     constexpr int N = D / 32;
     float acc[N] = {}, l = 0.f;
+#pragma unroll 8
     for (int i = 0; i < a.slots; ++i) {
         const float2 v = __ldg(ml + i);
-        if (v.y == 0.f) continue;
-        const float f = ex2(v.x - mx);
+        const bool none = v.y == 0.f;  // then its place holds nothing
+        const float f = none ? 0.f : ex2(v.x - mx);
         l += f * v.y;
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] += f * po[(size_t)i * D + lane * N + e];
+        for (int e = 0; e < N; ++e) acc[e] = fmaf(f, none ? 0.f : po[(size_t)i * D + lane * N + e], acc[e]);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a query that sees nothing gets zeros
     uint32_t w[N / 2];
@@ -949,9 +1002,10 @@ cudaError_t launch(const AttnSharedArgs &a, cudaStream_t s) {
     if (a.direct) {
         const int box = maps(as_step(D));
         if (!box) return cudaErrorInvalidValue;
-        const unsigned blocks = a.n_seq * p.n_kv_head * a.own_tiles;
-        return a.tile_rows == 8 ? launch_after<k_attn_direct<T, D, 1>>(blocks, kDirectWarps * 32, as_smem(D, kDirectWarps), s, 1, km, vm, a, box)
-                                : launch_after<k_attn_direct<T, D, 2>>(blocks, kDirectWarps * 32, as_smem(D, kDirectWarps), s, 1, km, vm, a, box);
+        const unsigned blocks = a.n_seq * p.n_kv_head * a.own_tiles * a.direct;
+        const size_t smem = as_smem(D, kDirectWarps);
+        return a.tile_rows == 8 ? launch_after<k_attn_direct<T, D, 1>>(blocks, kDirectWarps * 32, smem, s, a.direct, km, vm, a, box)
+                                : launch_after<k_attn_direct<T, D, 2>>(blocks, kDirectWarps * 32, smem, s, a.direct, km, vm, a, box);
     }
     if (a.tc_tiles) {
         const int box = maps(kTcKeys);
@@ -974,18 +1028,24 @@ cudaError_t launch(const AttnSharedArgs &a, cudaStream_t s) {
 
 }  // namespace
 
-// From so many query rows of a group on, the tensor cores' tiles of 128 rows take the shared keys.
-constexpr int kTcRows = 32;
+// From so many query rows of a group on, the tensor cores' tiles of 128 rows take the shared keys (64 groups and heads x
+// 4096 keys, in a graph: head 64, 16 rows 30.3 us against the warps' 25.8, 24 rows 31.3 against 34.2; head 128, 8 rows 35.9
+// against 36.1, 16 rows 37.6 against 49).
+constexpr int tc_rows(int D) { return D == 64 ? 24 : 16; }
 
 void attn_shared_plan(AttnSharedArgs &a) {
     const PagesArgs &p = a.p;
     const long long c = a.n_query * a.rep, want = 148 * 16;  // warps in flight on the device
     auto splits = [&](long long items, int keys) {
-        const long long n = (want + items - 1) / items, most = (keys + 63) / 64;
+        // a step costs a warp 0.85 us, a part its row's join 0.18 us: no more parts than where both are
+        // equal, nor of fewer than 64 keys
+        const long long n = (want + items - 1) / items, steps = (keys + as_step(p.head_dim) - 1) / as_step(p.head_dim);
+        long long most = 1;
+        while (most * 64 < keys && most * most < 5 * steps) ++most;
         return (int)(n < most ? n : most);
     };
     // tiles of 16 query rows where a row's own part or, on the warps, a group has more than 8
-    const bool tc = a.max_shared > 0 && a.n_seq * c / a.n_group >= kTcRows;
+    const bool tc = a.max_shared > 0 && a.n_seq * c / a.n_group >= tc_rows(p.head_dim);
     a.tile_rows = c <= 8 && (tc || a.max_shared == 0 || a.n_seq * c / a.n_group <= 8) ? 8 : 16;
     a.tc_tiles = a.shared_tiles = a.shared_splits = 0;
     if (a.max_shared > 0) {
@@ -1012,11 +1072,19 @@ void attn_shared_plan(AttnSharedArgs &a) {
     a.own_splits = own > some ? own : some < 1 ? 1 : some;
     a.own_items = (unsigned)a.n_seq * p.n_kv_head * a.own_tiles * a.own_splits;
     a.slots = a.shared_splits + a.own_splits;
-    // a block for each row, head and tile where they are no more than the SMs and no warp gets more than four steps
+    // A row, head and tile to a block, or to a cluster of as many as find room at once (clusters of 7 or 5 fill the SMs'
+    // groups badly), up to 16 steps a warp, on clusters of eight 32.  One row x 8 heads x 64, in a graph: 300 tokens 5.1 us
+    // on a block, 5.8 on eight, 8.7 with parts and a join; 1500 tokens 9.7, 5.8, 10.3; 24000 tokens 82, 15.4, 26.8.  16 rows,
+    // one block each: 1500 tokens 10.2 against 12.6, 6000 tokens 24.5 against 18.
     a.direct = 0;
     const unsigned direct_tiles = (unsigned)((c + (c <= 8 ? 7 : 15)) / (c <= 8 ? 8 : 16));
-    if ((long long)a.n_seq * p.n_kv_head * direct_tiles <= 148 && (long long)a.max_shared + a.max_own <= kDirectWarps * 32 * 4) {
-        a.direct = 1, a.slots = 0;
+    const long long items = (long long)a.n_seq * p.n_kv_head * direct_tiles, keys = (long long)a.max_shared + a.max_own;
+    int blocks = items <= 148 ? 1 : 0;
+    if (keys > 512)
+        for (const int n : {2, 3, 4, 6, 8})
+            if (items * n <= (n == 2 ? 148 : 128)) blocks = n;
+    if (keys <= (long long)blocks * kDirectWarps * (blocks < 8 ? 16 : 32) * as_step(p.head_dim)) {
+        a.direct = blocks, a.slots = 0;
         a.tile_rows = c <= 8 ? 8 : 16, a.own_tiles = direct_tiles;
     }
 }
