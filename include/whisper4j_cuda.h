@@ -426,7 +426,7 @@ typedef struct w4j_attn_shared {
     size_t work_bytes;
 } w4j_attn_shared;
 
-/* Bytes of scratch a call of these sizes needs, 0 for a few short rows (pointers and strides are not looked at). */
+/* Bytes of scratch a call of these sizes needs, 0 for a few rows that are not very long (pointers and strides are not looked at). */
 int w4j_op_attn_shared_workspace(const w4j_attn_shared *args, size_t *bytes);
 int w4j_op_attn_shared(const w4j_attn_shared *args, void *stream);
 
