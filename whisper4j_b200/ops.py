@@ -91,6 +91,7 @@ class PagedCache:
         c.work_bytes = n_bytes.value
         self._work = torch.empty(c.work_bytes, dtype=torch.uint8, device=self.device)
         c.work = self._work.data_ptr()
+        self._attend_work = None, 0  # sizes of the last attend and its scratch
 
     def _ints(self, t, name, n=None):
         """Address and length of a contiguous int32 vector on the cache's device."""
@@ -165,11 +166,16 @@ class PagedCache:
         a = AttnShared(self._ptr, layer, n_head, n_query, n_seq, n, max_shared, max_own,
                        self.head_dim ** -0.5 if scale is None else scale, q.data_ptr(), out.data_ptr(),
                        self._query_stride(q, "q"), self._query_stride(out, "out"), r, g, sh)
-        ref, n_bytes = ctypes.byref(a), ctypes.c_size_t()
-        check(self._lib.w4j_op_attn_shared_workspace(ref, n_bytes))
-        if n_bytes.value:
-            work = torch.empty(n_bytes.value, dtype=torch.uint8, device=self.device)
-            a.work, a.work_bytes = work.data_ptr(), n_bytes.value
+        ref, sizes = ctypes.byref(a), (n_head, n_query, n_seq, n, max_shared, max_own)
+        last, n_bytes = self._attend_work
+        if sizes != last:
+            size = ctypes.c_size_t()
+            check(self._lib.w4j_op_attn_shared_workspace(ref, size))
+            n_bytes = size.value
+            self._attend_work = sizes, n_bytes
+        if n_bytes:
+            work = torch.empty(n_bytes, dtype=torch.uint8, device=self.device)
+            a.work, a.work_bytes = work.data_ptr(), n_bytes
         check(self._lib.w4j_op_attn_shared(ref, _raw_stream(self._index)))
         return out
 
