@@ -179,6 +179,32 @@ def test_calls_that_cannot_be_done_change_nothing(n_rows):
         refused(c, m, "page", call)
 
 
+@pytest.mark.parametrize("n", [40, 100, 1000])
+def test_forks_of_many_rows_that_cannot_be_done(n):
+    """A fault in any one row, late or early, leaves all rows as they were."""
+    c, m = new_cache(n_layer=1, n_kv=1, n_rows=2 * n, n_pages=4 * n, max_tokens=64)
+    grow(c, m, list(range(n)), [30 + i % 3 for i in range(n)])  # 2 pages each; 32 is whole, 30 and 31 are not
+    dst, src = list(range(n, 2 * n)), list(range(n))
+    for at in (0, n // 2, n - 1):
+        for value in (2 * n, -2):
+            refused(c, m, "out of range", lambda: c.fork(ints(dst), ints(src[:at] + [value] + src[at + 1:])))
+        refused(c, m, "out of range", lambda: c.fork(ints(dst[:at] + [2 * n] + dst[at + 1:]), ints(src)))
+        old = int(m.table[at, 1])
+        c.table[at, 1] = m.table[at, 1] = 4 * n
+        refused(c, m, "page", lambda: c.fork(ints(dst), ints(src)))
+        c.table[at, 1] = m.table[at, 1] = old
+    refused(c, m, "twice", lambda: c.fork(ints(dst[:-1] + dst[:1]), ints(src)))
+    c.fork(ints(dst), ints(src))  # a row of its own for each: full pages shared, the last one stays with the source
+    m.fork(dst, src)
+    grow(c, m, dst, [1] * n)
+    same(c, m)
+    grow(c, m, [0], [20])  # n - 2 pages are left, and n rows want one
+    refused(c, m, "free pages", lambda: c.fork(ints(dst), ints([0] * n)))
+    c.fork(ints(dst[2:]), ints([0] * (n - 2)))
+    m.fork(dst[2:], [0] * (n - 2))
+    same(c, m)
+
+
 def test_write_leaves_out_what_has_no_place():
     c, m = new_cache()
     grow(c, m, [0, 1], [3, 4])

@@ -11,7 +11,8 @@
 // the free list by prefix sums over slices of `ref`.  The tokens are moved by a second kernel on all SMs
 // from a list of (source, destination, tokens) that the first one leaves.  The first is bound by the
 // latency of its dependent passes over L2, the second by HBM.  A call whose lists fit one block's registers and
-// shared memory takes one block that reads everything once (k_pages_small): three passes instead of five.
+// shared memory takes one block that reads everything once (k_pages_small), a fork of more rows a cluster of such blocks:
+// three passes instead of five.
 //
 // Every call is all or nothing: the cluster checks all rows, lengths and the number of free pages before
 // its first write, and a call that cannot be done raises a bit of `status` and changes nothing else.
@@ -431,7 +432,7 @@ struct SmallRows {  // of the n rows of a call, and of all rows
 size_t small_bytes(const PagesArgs &p, int n) { return 4 * (5 * (size_t)n + 2 * (size_t)p.n_rows + 2 * (size_t)p.n_pages); }
 
 // a, b: dst and src (fork), rows and start (extend), rows (free), n_live (compact: the call's rows are all of them)
-template <PagesOp OP>
+template <PagesOp OP, bool MANY>
 __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, const int *__restrict__ a, const int *__restrict__ b,
                                                                int *live_out, int n) {
     extern __shared__ int dyn[];
@@ -440,7 +441,8 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
     const SmallRows s(dyn, n, p.n_rows, p.n_pages);
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, T = p.page_tokens, W = p.width;
     // step x of a warp: 32 entries (runs of 32 in each row) of row i from j0 on
-    const int runs = (W + 31) / 32, steps = n * runs, warps = threads / 32;
+    const int blocks = MANY ? cluster_size() : 1, block = MANY ? cluster_rank() : 0;
+    const int runs = (W + 31) / 32, steps = n * runs, warps = blocks * (threads / 32), first = block * (threads / 32) + tid / 32;
     auto row_of = [&](int step, int &j) {
         const int i = runs == 1 ? step : step / runs;
         j = (step - i * runs) * 32 + lane;
@@ -464,8 +466,10 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
         for (int i = tid; i < p.n_rows; i += threads) s.mark[i] = -1, s.owner[i] = 0x7fffffff;
         for (int i = tid; i < p.n_pages; i += threads) s.more[i] = 0;
     }
-    if (tid == 0) bad = OP == OP_EXTEND && b[0] != 0 ? W4J_PAGES_BAD_START : 0, w.head[H_PAIRS] = 0;
+    if (tid == 0) bad = OP == OP_EXTEND && b[0] != 0 ? W4J_PAGES_BAD_START : 0;
+    if (tid == 0 && block == 0) w.head[H_PAIRS] = 0;
     __syncthreads();
+    if (MANY) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this block's `bad` is there
     for (int i = tid; i < n; i += threads) {
         const int r = OP == OP_COMPACT ? i : s.a[i];
         if (r < 0 || r >= p.n_rows || (OP != OP_COMPACT && atomicExch(s.mark + r, i) != -1)) {
@@ -495,7 +499,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
 #pragma unroll
     for (int x = 0; x < kEntries; ++x) {
         was[x] = shall[x] = -1;
-        const int step = tid / 32 + x * warps;
+        const int step = first + x * warps;
         if (OP == OP_EXTEND || step >= steps) continue;
         int j;
         const int i = row_of(step, j), r = OP == OP_COMPACT ? i : s.a[i];
@@ -506,7 +510,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
         bool out = false;
 #pragma unroll
         for (int x = 0; x < kEntries; ++x) {
-            const int step = tid / 32 + x * warps;
+            const int step = first + x * warps;
             if (step >= steps) continue;
             int j;
             const int i = row_of(step, j);
@@ -520,7 +524,11 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
 #pragma unroll
         for (int i = 0; i < kRefs; ++i) {
             const int page = tid * kRefs + i;
-            if (page < p.n_pages && s.more[page]) p.ref[page] = ref[i] + s.more[page];
+            if (page >= p.n_pages || !s.more[page]) continue;
+            if (MANY)
+                atomicAdd(p.ref + page, s.more[page]);
+            else
+                p.ref[page] = ref[i] + s.more[page];
         }
     };
     if (OP == OP_FREE) {
@@ -576,7 +584,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
         for (int x = 0; x < kEntries; ++x)
             if (was[x] >= live) {
                 int j;
-                const int i = row_of(tid / 32 + x * warps, j);
+                const int i = row_of(first + x * warps, j);
                 p.table[(size_t)i * W + j] = w.stage[was[x]];
             }
         if (tid == 0) {
@@ -608,13 +616,22 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
         if (ref[i] <= 0 && at < need) s.list[at++] = tid * kRefs + i;
     if (need > free_pages && tid == 0) atomicOr(&bad, W4J_PAGES_FULL);
     __syncthreads();
+    if (MANY) {  // what one has found holds for all; and all have read what follows writes
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (tid < blocks && bad) {
+            uint32_t at;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&bad)), "r"(tid));
+            asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(at), "r"(bad) : "memory");
+        }
+        cluster_barrier();
+    }
     if (bad) {
-        if (tid == 0) atomicOr(p.status, bad);
+        if (tid == 0 && block == 0) atomicOr(p.status, bad);
         return;
     }
 #pragma unroll
     for (int x = 0; x < kEntries; ++x) {
-        const int step = tid / 32 + x * warps;
+        const int step = first + x * warps;
         if (step >= steps) break;
         int j;
         const int i = row_of(step, j);
@@ -638,9 +655,10 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
             if (shall[x] >= 0) *entry = shall[x], atomicAdd(s.more + shall[x], 1);
         }
     }
-    for (int i = tid; i < n; i += threads) p.len[s.a[i]] = s.len_b[i];
+    if (block == 0)
+        for (int i = tid; i < n; i += threads) p.len[s.a[i]] = s.len_b[i];
     if (OP == OP_FORK) {
-        if (tid == 0) w.head[H_PAIRS] = need;
+        if (tid == 0 && block == 0) w.head[H_PAIRS] = need;
         __syncthreads();
         add_more();
     }
@@ -752,9 +770,25 @@ int small_threads(const PagesArgs &p, int n) {
     return 32 * (int)(need < 4 ? 4 : need);
 }
 
+// A fork of more rows: the same by a cluster, whose blocks all plan for all rows and pages and share the tables'
+// entries out.  One block's time is its instructions (4 layers of large-v3-turbo, with the move: 5 rows 8.1 us on one, 8.7
+// on eight, 40 rows 12.0 and 10.0, 320 rows 19.4 and 14.7; 640 rows 23.4 where k_pages_fork took 37.4).
+constexpr int kForkBlocks = 8, kForkSteps = 6;
+int fork_threads(const PagesArgs &p, int n, int &blocks) {
+    const long long steps = (long long)n * ((p.width + 31) / 32), by_pages = (p.n_pages + 32 * kRefs - 1) / (32 * kRefs);
+    blocks = 1;
+    if (steps < 32) return small_threads(p, n);
+    if (by_pages > kSmallThreads / 32 || small_bytes(p, n) > 160 * 1024 || steps > kForkBlocks * kSmallThreads / 32 * kEntries) return 0;
+    blocks = kForkBlocks;
+    const long long share = (steps + kForkBlocks * kForkSteps - 1) / (kForkBlocks * kForkSteps), need = share > by_pages ? share : by_pages;
+    return 32 * (int)(need < 4 ? 4 : need > kSmallThreads / 32 ? kSmallThreads / 32 : need);
+}
+
 template <PagesOp OP>
-cudaError_t launch_small(const PagesArgs &p, const int *a, const int *b, int *live, int n, int threads, cudaStream_t s) {
-    return launch_after<k_pages_small<OP>>(1, threads, small_bytes(p, n), s, 1, p, a, b, live, n);
+cudaError_t launch_small(const PagesArgs &p, const int *a, const int *b, int *live, int n, int threads, cudaStream_t s, int blocks = 1) {
+    if (OP == OP_FORK && blocks > 1)
+        return launch_after<k_pages_small<OP, OP == OP_FORK>>(blocks, threads, small_bytes(p, n), s, blocks, p, a, b, live, n);
+    return launch_after<k_pages_small<OP, false>>(1, threads, small_bytes(p, n), s, 1, p, a, b, live, n);
 }
 
 int move_blocks(const PagesArgs &p, long long pairs) {
@@ -771,8 +805,9 @@ size_t pages_work_bytes(const PagesArgs &p) {
 }
 
 cudaError_t launch_pages_fork(const PagesArgs &p, const int *dst, const int *src, int n, cudaStream_t s) {
-    const int t = small_threads(p, n);
-    const cudaError_t e = t ? launch_small<OP_FORK>(p, dst, src, nullptr, n, t, s)
+    int blocks;
+    const int t = fork_threads(p, n, blocks);
+    const cudaError_t e = t ? launch_small<OP_FORK>(p, dst, src, nullptr, n, t, s, blocks)
                             : launch_after<k_pages_fork>(kPlanCluster, kPlanThreads, 0, s, kPlanCluster, p, dst, src, n);
     if (e != cudaSuccess) return e;
     return launch_after<k_pages_move>(move_blocks(p, n), kMoveThreads, 0, s, 1, p);
