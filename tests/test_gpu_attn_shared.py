@@ -247,6 +247,13 @@ def test_bad_sequences_are_marked(n):
         s["cache"].check()
 
 
+@pytest.mark.parametrize("n", [2, 30])
+def test_rows_may_outgrow_max_own(n):
+    s = make([n], [40], [40 + 97 * (i + 1) for i in range(n)], heads=8, kv=8)
+    s["max_own"] = 1
+    verify(s, attend(s))
+
+
 def test_a_bad_page_late_in_a_long_row():
     """Read by one of the blocks that share the row's keys: all of the row's results are marked."""
     s = make([1, 1], [0, 0], [2000, 2000], heads=8, kv=8)

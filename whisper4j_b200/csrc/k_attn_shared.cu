@@ -1041,7 +1041,7 @@ void attn_shared_plan(AttnSharedArgs &a) {
         // equal, nor of fewer than 64 keys
         const long long n = (want + items - 1) / items, steps = (keys + as_step(p.head_dim) - 1) / as_step(p.head_dim);
         long long most = 1;
-        while (most * 64 < keys && most * most < 5 * steps) ++most;
+        while (most < n && most * 64 < keys && most * most < 5 * steps) ++most;
         return (int)(n < most ? n : most);
     };
     // tiles of 16 query rows where a row's own part or, on the warps, a group has more than 8
