@@ -868,16 +868,24 @@ bool tmap_i8(CUtensorMap *m, const int8_t *base, long long rows, int cols, long 
     return tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, cols, ld, kMmK, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+long long mm_tiles(const LinearI8Args &a, int nt) {
+    return (long long)((a.N + kMmTile - 1) / kMmTile) * ((a.M + nt - 1) / nt);
+}
+// k is split while the tiles leave SMs idle and every block keeps two stages of k
+int mm_split(long long tiles, int kb) {
+    int ks = 1;
+    while (ks < 8 && tiles * ks * 2 <= 148 && kb >= 4 * ks) ks *= 2;
+    return ks;
+}
+
 template <int NT, typename T, int EPI>
 cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
     const int k16 = (a.K + 15) / 16 * 16, kb = (a.K + kMmK - 1) / kMmK;
     alignas(64) CUtensorMap wmap, xmap;
     if (!tmap_i8(&wmap, a.w, a.N, k16, a.ldw, kMmTile) || !tmap_i8(&xmap, a.x, a.M, k16, a.ldx, NT))
         return cudaErrorInvalidValue;
-    const long long token_tiles = (a.M + NT - 1) / NT, tiles = (long long)((a.N + kMmTile - 1) / kMmTile) * token_tiles;
-    // k is split while the tiles leave SMs idle and every block keeps two stages of k
-    int ks = 1;
-    while (ks < 8 && tiles * ks * 2 <= 148 && kb >= 4 * ks) ks *= 2;
+    const long long token_tiles = (a.M + NT - 1) / NT, tiles = mm_tiles(a, NT);
+    const int ks = mm_split(tiles, kb);
     return launch_after<k_linear_i8<NT, T, EPI>>((unsigned)(tiles * ks), kMmThreads, mm_smem(NT), s, ks, wmap, xmap, a, ks,
                         (int)token_tiles);
 }
@@ -910,7 +918,10 @@ constexpr int kFewRows = 8;
 // Which kernel takes a product, times in a graph: the warps' one pass over the weights where it is short (K = 1280: 2 rows
 // 3.3 us against 4.4, 4 rows 4.5 against 4.4; K = 384: 4 rows 2.3 against 3.4; K = 5120: 1 row 3.6 against 4.7, 2 rows 5.4
 // against 4.7); the pair where single blocks of 128 x 128 would need a second turn of the SMs (K = 1280, N = 5120: 320 rows
-// 9.8 us against 8.1, 512 rows 9.8 against 15.2; K = 5120, N = 1280: 1500 rows 18.1 against 17.1, 2048 rows 18.3 against 31.9).
+// 9.8 us against 8.1, 512 rows 9.8 against 15.2; K = 5120, N = 1280: 1500 rows 18.1 against 17.1, 2048 rows 18.3 against 31.9);
+// single blocks otherwise, with as many tokens nt as take the least time by what was measured of a block: 2.5 us + 0.02 us
+// a token + (0.27 + 0.0003 nt) us for each 128 of its k + 1 us for a cluster's sums, one block to an SM (77 x 1000 x 701: 6.1 us with nt = 128, 4.1 with 32;
+// 100 x 5120 x 1280: 7.3 with 128, 7.5 with 64, 9.3 with 32).
 template <typename T, int EPI>
 cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
     const unsigned few = (a.N + kFewWarps - 1) / kFewWarps;
@@ -919,11 +930,19 @@ cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
         if (a.M <= 4) return launch_after<k_linear_i8_few<4, T, EPI>>(few, kFewWarps * 32, 0, s, 1, a);
         return launch_after<k_linear_i8_few<8, T, EPI>>(few, kFewWarps * 32, 0, s, 1, a);
     }
-    if (a.M <= 16) return product<16, T, EPI>(a, s);
-    if (a.M <= 32) return product<32, T, EPI>(a, s);
-    if (a.M <= 64) return product<64, T, EPI>(a, s);
-    const long long tiles = ((a.N + 127LL) / 128) * ((a.M + 127LL) / 128);
-    if (a.M > 128 && tiles > 148) return product_pair<T, EPI>(a, s);
+    if (a.M > 128 && mm_tiles(a, 128) > 148) return product_pair<T, EPI>(a, s);
+    const int kb = (a.K + kMmK - 1) / kMmK;
+    int nt = 16;
+    float least = 0.f;
+    for (const int x : {16, 32, 64, 128}) {
+        const long long tiles = mm_tiles(a, x);
+        const int ks = mm_split(tiles, kb), steps = (kb + ks - 1) / ks;
+        const float us = (float)((tiles * ks + 147) / 148) * (2.5f + 0.02f * x + steps * (0.27f + 0.0003f * x) + (ks > 1));
+        if (x == 16 || us < least) least = us, nt = x;
+    }
+    if (nt == 16) return product<16, T, EPI>(a, s);
+    if (nt == 32) return product<32, T, EPI>(a, s);
+    if (nt == 64) return product<64, T, EPI>(a, s);
     return product<128, T, EPI>(a, s);
 }
 
