@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kMmThreads) k_linear_i8(const __grid_constant_
 // ---------------------------------------------------------------------------
 // a few rows: a warp per channel, 16 bytes of its weights per lane and step against MT rows (dp4a), the next steps' weights
 // on their way.  Bound by the latency of one trip to HBM and by its launch; no tensor memory, barriers or cluster.
-// (One row x 1280 x 3840 channels: 4.5 us, on the tensor cores 7.6.)
+// (One row x 1280 x 3840 channels, weights in L2: 2.6 us, on the tensor cores 4.3.)
 // ---------------------------------------------------------------------------
 constexpr int kFewWarps = 8;
 
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_few(LinearI8Args a
 
 // The whole layer for a few rows in one launch: every block quantises the rows for itself (8, 4 or 2 warps to a row)
 // into shared memory while the first 2 KB of its channels' weights are on their way.  One row x 1280 x 3840 channels
-// takes 3.8 us in a graph, 1.3 TB/s of weights, where the two launches took 6.
+// takes 3.8 us in a graph, 1.3 TB/s of weights, where two launches take 4.5.
 // Longer rows or more of them are quantised once instead, by a launch of their own (in a graph, 1280 x 3840: 2 rows 7.1 us
 // against 4.6, 4 rows 17 against 5.6; 5120 x 1280: 1 row 9.3 against 6.2); below, a launch saved is 2.5 us of the host's.
 constexpr size_t kLayerSmem = 1536;
