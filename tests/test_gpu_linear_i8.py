@@ -196,6 +196,7 @@ def test_layer(xtype, ytype):
 @pytest.mark.parametrize("ln", [False, True])
 @pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 8, 9])
 @pytest.mark.parametrize("k,n,xtype", [(1, 3, torch.float32), (384, 1152, torch.float16), (1000, 50, torch.bfloat16),
+                                       (1530, 4737, torch.float16), (768, 129, torch.float16), (511, 40, torch.float16), (380, 9475, torch.bfloat16),
                                        (5120, 129, torch.float32), (6200, 40, torch.float32), (20000, 10, torch.float32)])
 def test_layer_of_a_few_rows(m, k, n, xtype, ln):
     """One launch where the rows are few and short, two where not; behind a LayerNorm against its exact value: a

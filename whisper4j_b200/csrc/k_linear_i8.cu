@@ -518,11 +518,12 @@ __global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_few(LinearI8Args a
 }
 
 // The whole layer for a few rows in one launch: every block quantises the rows for itself (8, 4 or 2 warps to a row)
-// into shared memory while the first 2 KB of its channels' weights are on their way.  One row x 1280 x 3840 channels
-// takes 3.8 us in a graph, 1.3 TB/s of weights, where two launches take 4.5.
+// into shared memory while its first channels' weights are on their way.  One row x 1280 x 3840 channels
+// takes 3.6 us in a graph, 1.3 TB/s of weights, where two launches take 4.5.
 // Longer rows or more of them are quantised once instead, by a launch of their own (in a graph, 1280 x 3840: 2 rows 7.1 us
 // against 4.6, 4 rows 17 against 5.6; 5120 x 1280: 1 row 9.3 against 6.2); below, a launch saved is 2.5 us of the host's.
 constexpr size_t kLayerSmem = 1536;
+constexpr int kLayerBlocks = 4;  // to an SM
 
 __device__ __forceinline__ float load1(const void *x, int type, long long i) {
     return type == W4J_GGML_F32 ? __ldg(static_cast<const float *>(x) + i)
@@ -531,27 +532,28 @@ __device__ __forceinline__ float load1(const void *x, int type, long long i) {
 }
 
 template <int MT, typename T, int EPI>
-__global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_layer(LinearI8Args a, QuantizeArgs in) {
+__global__ void __launch_bounds__(kFewWarps * 32, kLayerBlocks) k_linear_i8_layer(LinearI8Args a, QuantizeArgs in) {
     extern __shared__ __align__(16) int8_t sq[];  // [M][K rounded up to 16]
     __shared__ uint32_t sm[kFewWarps];
     __shared__ float sxs[MT];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = blockIdx.x * kFewWarps + warp;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int K = a.K, units = (K + 15) / 16, k16 = 16 * units;
+    int n = blockIdx.x * kFewWarps + warp;
     const int8_t *w = a.w + (long long)n * a.ldw;
     if (n < a.N)  // into L2 only: the weights may be what the kernel before this one writes
         for (int k = lane * 128; k < K; k += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(w + k));
     pdl_wait();
     pdl_trigger();
-    constexpr int U = 4, E = 8;
+    constexpr int U = (kLayerSmem + 511) / 512;  // 16-byte units of a channel for each lane
     uint4 v[U];
-    auto weights = [&](int u0) {
+    auto weights = [&]() {
 #pragma unroll
         for (int i = 0; i < U; ++i)
-            v[i] = n < a.N && u0 + 32 * i < units ? __ldg(reinterpret_cast<const uint4 *>(w) + u0 + 32 * i) : make_uint4(0, 0, 0, 0);
+            v[i] = n < a.N && lane + 32 * i < units ? __ldg(reinterpret_cast<const uint4 *>(w) + lane + 32 * i) : make_uint4(0, 0, 0, 0);
     };
-    weights(lane);
-    // row `row` by `per` warps; the first E of a thread's elements stay in registers
-    constexpr int per = kFewWarps / MT, nt = 32 * per;
+    weights();
+    // row `row` by `per` warps, E elements of a thread in registers: MT / 2 rows and one more have the longest
+    constexpr int per = kFewWarps / MT, nt = 32 * per, E = (kLayerSmem / (MT / 2 + 1) + nt - 1) / nt;
     const int row = warp / per, t = tid % nt, rows = min(MT, a.M);
     const long long x0 = (long long)min(row, rows - 1) * in.ldx;
     float c[E];
@@ -561,7 +563,6 @@ __global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_layer(LinearI8Args
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (t + e * nt < K) f(t + e * nt, c[e]);
-        for (int k = t + E * nt; k < K; k += nt) f(k, load1(in.x, in.type, x0 + k));
     };
     auto reduce = [&](auto r, auto op) {
         using R = decltype(r);
@@ -607,30 +608,30 @@ __global__ void __launch_bounds__(kFewWarps * 32) k_linear_i8_layer(LinearI8Args
         for (int k = K + t; k < k16; k += nt) q[k] = 0;
     }
     __syncthreads();
-    int acc[MT] = {};
-    for (int u0 = lane;;) {
+    while (n < a.N) {
+        int acc[MT] = {};
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             if (m >= rows) break;
 #pragma unroll
             for (int i = 0; i < U; ++i) {
-                if (u0 + 32 * i >= units) break;
-                const uint4 x = *reinterpret_cast<const uint4 *>(sq + m * k16 + 16 * (u0 + 32 * i));
+                if (lane + 32 * i >= units) break;
+                const uint4 x = *reinterpret_cast<const uint4 *>(sq + m * k16 + 16 * (lane + 32 * i));
                 acc[m] = __dp4a((int)v[i].x, (int)x.x, acc[m]), acc[m] = __dp4a((int)v[i].y, (int)x.y, acc[m]);
                 acc[m] = __dp4a((int)v[i].z, (int)x.z, acc[m]), acc[m] = __dp4a((int)v[i].w, (int)x.w, acc[m]);
             }
         }
-        u0 += 32 * U;
-        if (u0 - lane >= units) break;
-        weights(u0);
-    }
-    if (n >= a.N) return;
-    const float ws = __ldg(a.ws + n), b = a.bias ? __ldg(a.bias + n) : 0.f;
+        const float ws = __ldg(a.ws + n), b = a.bias ? __ldg(a.bias + n) : 0.f;
+        T *y = reinterpret_cast<T *>(a.y) + n;
+        n += gridDim.x * kFewWarps;
+        w = a.w + (long long)n * a.ldw;
+        weights();
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+        for (int m = 0; m < MT; ++m) {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
-        if (m < rows && lane == m) finish<T, EPI>(acc[m], sxs[m], ws, b, reinterpret_cast<T *>(a.y) + (long long)m * a.ldy + n);
+            for (int o = 16; o; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
+            if (m < rows && lane == m) finish<T, EPI>(acc[m], sxs[m], ws, b, y + (long long)m * a.ldy);
+        }
     }
 }
 
@@ -948,7 +949,9 @@ cudaError_t product(const LinearI8Args &a, cudaStream_t s) {
 
 template <typename T, int EPI>
 cudaError_t layer(const LinearI8Args &a, const QuantizeArgs &q, cudaStream_t s) {
-    const unsigned blocks = (a.N + kFewWarps - 1) / kFewWarps;
+    // as many as find room at once: a second turn would wait for the rows a second time (1 x 1280 x 5120 in a graph: 6.9 us
+    // with a block for each eight channels, 4.7 so)
+    const unsigned all = (a.N + kFewWarps - 1) / kFewWarps, most = 148 * kLayerBlocks, blocks = all < most ? all : most;
     const size_t smem = (size_t)a.M * ((a.K + 15) / 16 * 16);
     if (a.M == 1) return launch_after<k_linear_i8_layer<1, T, EPI>>(blocks, kFewWarps * 32, smem, s, 1, a, q);
     if (a.M == 2) return launch_after<k_linear_i8_layer<2, T, EPI>>(blocks, kFewWarps * 32, smem, s, 1, a, q);
