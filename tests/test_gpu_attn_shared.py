@@ -247,10 +247,11 @@ def test_bad_sequences_are_marked(n):
         s["cache"].check()
 
 
-@pytest.mark.parametrize("n", [2, 30])
-def test_rows_may_outgrow_max_own(n):
-    s = make([n], [40], [40 + 97 * (i + 1) for i in range(n)], heads=8, kv=8)
-    s["max_own"] = 1
+@pytest.mark.parametrize("max_own", [0, 1])
+@pytest.mark.parametrize("n,shared", [(2, 40), (30, 40), (30, 0)])
+def test_rows_may_outgrow_max_own(n, shared, max_own):
+    s = make([n], [shared], [40 + 97 * (i + 1) for i in range(n)], heads=8, kv=8)
+    s["max_own"] = max_own
     verify(s, attend(s))
 
 

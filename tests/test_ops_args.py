@@ -210,6 +210,8 @@ def test_a_few_short_rows_need_no_scratch():
     w = lib().w4j_op_attn_shared_workspace
     assert workspace(w, ctypes.byref(attn(cache()))) == (W4J_OK, 0)
     assert workspace(w, ctypes.byref(attn(cache(), n_seq=100)))[1] > 0
+    # rows may outgrow max_own, 0 included: parts need their scratch all the same
+    assert workspace(w, ctypes.byref(attn(cache(), n_seq=200, max_shared=0, max_own=0)))[1] > 0
 
 
 def test_scratch_stays_in_proportion():

@@ -1083,7 +1083,7 @@ void attn_shared_plan(AttnSharedArgs &a) {
     if (keys > 512)
         for (const int n : {2, 3, 4, 6, 8})
             if (items * n <= (n == 2 ? 148 : 128)) blocks = n;
-    if (keys <= (long long)blocks * kDirectWarps * (blocks < 8 ? 16 : 32) * as_step(p.head_dim)) {
+    if (blocks && keys <= (long long)blocks * kDirectWarps * (blocks < 8 ? 16 : 32) * as_step(p.head_dim)) {
         a.direct = blocks, a.slots = 0;
         a.tile_rows = c <= 8 ? 8 : 16, a.own_tiles = direct_tiles;
     }
