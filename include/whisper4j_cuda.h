@@ -331,9 +331,10 @@ int w4j_op_logits_argmax_noalloc(int device, const float *x, int M, int d, const
  *           are neither read nor written
  *   len     [n_rows] tokens of each row
  *   status  [1] what calls could not do, W4J_PAGES_* bits, added up until the caller clears it
- *   work    w4j_op_pages_workspace's bytes of scratch that this cache's calls share
+ *   work    w4j_op_pages_workspace's bytes of scratch that belong to this cache for as long as it lives and that
+ *           all of its calls share, captured ones too: it keeps which rows' last extension was refused
  *
- * A new cache is ref, len and status set to zero.  A last page that is not full belongs to one row alone:
+ * A new cache is ref, len, status and work set to zero.  A last page that is not full belongs to one row alone:
  * every call here keeps that so, and a caller that builds tables of its own has to.
  *
  * The calls are asynchronous on `stream` and change the cache in stream order; calls on one cache that
@@ -370,8 +371,10 @@ int w4j_op_pages_extend(const w4j_pages *cache, const int32_t *rows, const int32
 /* Keys and values of the last start[i + 1] - start[i] tokens of row rows[i], as tokens start[i] ..
  * start[i + 1] - 1 of k and v (n_tokens = start[n] tokens of [n_kv_head][head_dim], k_stride and v_stride
  * elements apart, multiples of 8, both 16-byte aligned: the K and V parts of a fused projection can stay in
- * place).  After w4j_op_pages_extend of the same rows and start.  A token whose row or page is out of range
- * is left out and raises its status bit. */
+ * place).  After w4j_op_pages_extend of the same rows and start.  A row whose last extension was refused takes no
+ * tokens until one succeeds (its length has not grown: theirs would be the places of its last ones): they are left
+ * out and raise that refusal's status bits again.  A token whose row or page is out of range is left out and raises
+ * its status bit. */
 int w4j_op_pages_write(const w4j_pages *cache, int layer, const int32_t *rows, const int32_t *start, int n,
                        const void *k, int64_t k_stride, const void *v, int64_t v_stride, int n_tokens, void *stream);
 

@@ -275,3 +275,67 @@ def test_on_a_stream_of_its_own():
     torch.cuda.current_stream().wait_stream(side)
     m.fork([3], [1])
     same(c, m)
+
+
+def tokens(c, n, seed):
+    g = torch.Generator("cuda").manual_seed(seed)
+    return torch.randn(2, n, c.n_kv_head, c.head_dim, device="cuda", generator=g).to(c.pool.dtype)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("n_rows", [8, 30000])  # planned by one block, and by a cluster
+def test_writes_behind_a_refused_extension_change_nothing(n_rows, captured):
+    """Rows whose last page is full and shared: the tokens of an extension that finds no page would land on it."""
+    c, m = new_cache(n_pages=8, n_rows=n_rows)
+    grow(c, m, [0, 6], [48, 33])  # 3 + 3 pages, 2 free
+    c.fork(ints([1, 2]), ints([0, 0]))
+    m.fork([1, 2], [0, 0])
+    rows, start, kv = ints([0, 1, 2]), ints([0, 1, 2, 3]), tokens(c, 3, 5)
+
+    def step():
+        c.extend(rows, start)
+        for layer in range(c.n_layer):
+            c.write(layer, rows, start, kv[0], kv[1])
+
+    run = step
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        run = graph.replay
+    for _ in range(2):
+        refused(c, m, "free pages", run)  # three rows want a page each
+    refused(c, m, "free pages", lambda: c.write(0, rows, start, kv[0], kv[1]))  # also behind a status that was read
+    grow(c, m, [6], [2])  # another row goes on
+    c.extend(ints([1]), ints([0, 1]))  # and one of the three
+    m.extend([1], [0, 1])
+    more = tokens(c, 1, 6)
+    for layer in range(c.n_layer):
+        c.write(layer, ints([1]), ints([0, 1]), more[0], more[1])
+        m.write(layer, [1], [0, 1], *more.view(torch.int16).cpu().numpy())
+    same(c, m)
+    c.free(ints([6]))
+    m.free([6])
+    run()  # there is room now
+    m.extend([0, 1, 2], [0, 1, 2, 3])
+    for layer in range(c.n_layer):
+        m.write(layer, [0, 1, 2], [0, 1, 2, 3], *kv.view(torch.int16).cpu().numpy())
+    same(c, m)
+
+
+@pytest.mark.parametrize("n_rows", [8, 30000])
+@pytest.mark.parametrize("rows,counts,text", [([0, 1], [1, 65], "outgrow"), ([0, 0], [1, 1], "twice"), ([0, -1], [1, 1], "out of range"),
+                                              ([1, 0], [3, -1], "ascend")])
+def test_writes_behind_any_refusal(n_rows, rows, counts, text):
+    c, m = new_cache(n_rows=n_rows)
+    grow(c, m, [0, 1], [20, 48])
+    start = starts(counts)
+    kv = tokens(c, max(start), 3)
+
+    def step():
+        c.extend(ints(rows), ints(start))
+        c.write(1, ints(rows), ints(start), kv[0], kv[1])
+
+    refused(c, m, text, step)
+    grow(c, m, [0, 1], [2, 3])
+    same(c, m)

@@ -31,12 +31,18 @@ constexpr int kPlanCluster = 8;
 // what a call leaves for its second kernel and for the next pass of its own, in the caller's workspace
 enum { H_PAIRS = 0, H_BAD = 1, H_COUNT = 8, H_MORE = 16, H_SIZE = 32 };  // H_COUNT, H_MORE: one word per block
 
+// What a row's last extension leaves for the writes that follow it: 0, or this number and the bits that refused it.  The
+// row's length has not grown then, and its new tokens' places would be those of its last ones, on pages that other rows may
+// hold too.  (Scratch that nobody has set to zero looks refused once in 2^24.)
+constexpr int kRefused = 0x57346a00, kRefusedBits = 0xff;
+
 struct Work {
-    int *head, *list, *mark, *owner, *rank, *slen, *from, *to, *tokens, *stage;
+    int *head, *refused, *list, *mark, *owner, *rank, *slen, *from, *to, *tokens, *stage;
     __host__ __device__ Work(const PagesArgs &p) {
         const size_t r = p.n_rows, n = p.n_pages, most = r > n ? r : n;
         head = p.work;
-        list = head + H_SIZE;      // free pages, or the holes of a compaction
+        refused = head + H_SIZE;   // of each row, kept from call to call: only extensions write it
+        list = refused + r;        // free pages, or the holes of a compaction
         mark = list + n;           // the call's index of each row, -1 where it has none
         owner = mark + r;          // fork: the first destination that takes a row over
         rank = owner + r;
@@ -148,6 +154,14 @@ __device__ __forceinline__ bool go_on(const PagesArgs &p, const Work &w, int mor
     const int bad = __ldcg(w.head + H_BAD) | more;
     if (bad && gid == 0) atomicOr(p.status, bad);
     return bad == 0;
+}
+
+// The outcome of an extension for the rows it names (threads gid of nt): 0, or the bits that refused it.
+__device__ __forceinline__ void note_outcome(const PagesArgs &p, const Work &w, const int *rows, int n, int bad, int gid, int nt) {
+    for (int i = gid; i < n; i += nt) {
+        const int r = rows[i];
+        if (r >= 0 && r < p.n_rows) w.refused[r] = bad ? kRefused | bad : 0;
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -267,7 +281,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_extend(PagesArgs p, cons
     }
     count_free(p, w, sm);
     cluster_barrier();
-    if (!go_on(p, w, 0, gid)) return;
+    if (!go_on(p, w, 0, gid)) return note_outcome(p, w, rows, n, __ldcg(w.head + H_BAD), gid, nt);
     const int have = all_free(w);
     int need = 0;
     for (int i0 = 0, c = 0; i0 < n; i0 += kPlanThreads, ++c) {
@@ -278,7 +292,9 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_extend(PagesArgs p, cons
         if (i < n && c % cluster_size() == cluster_rank()) w.rank[i] = r;
         need = min(need + total, have + 1);
     }
-    if (!go_on(p, w, need > have ? W4J_PAGES_FULL : 0, gid)) return;
+    const int lack = need > have ? W4J_PAGES_FULL : 0;
+    note_outcome(p, w, rows, n, lack, gid, nt);
+    if (!go_on(p, w, lack, gid)) return;
     list_free(p, w, need, sm);
     cluster_barrier();
     for (int i = gw; i < n; i += nw) {
@@ -625,6 +641,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
         }
         cluster_barrier();
     }
+    if (OP == OP_EXTEND) note_outcome(p, w, s.a, n, bad, tid, threads);
     if (bad) {
         if (tid == 0 && block == 0) atomicOr(p.status, bad);
         return;
@@ -735,6 +752,11 @@ __global__ void __launch_bounds__(kWriteWarps * 32) k_pages_write(PagesArgs p, i
     const int r = rows[lo], s0 = start[lo], s1 = start[lo + 1];
     if (t < s0 || t >= s1) return;  // behind the last sequence, or a start that does not ascend (reported above)
     const bool row_ok = r >= 0 && r < p.n_rows;
+    const int refused = row_ok ? __ldcg(Work(p).refused + r) : 0;
+    if ((refused & ~kRefusedBits) == kRefused) {  // its extension did not take place
+        if (lane == 0) atomicOr(p.status, refused & kRefusedBits);
+        return;
+    }
     const long long pos = row_ok ? (long long)row_len(p, r) - s1 + t : -1;
     if (pos < 0) {
         if (lane == 0) atomicOr(p.status, row_ok ? W4J_PAGES_BAD_START : W4J_PAGES_BAD_ROW);
@@ -801,7 +823,7 @@ int move_blocks(const PagesArgs &p, long long pairs) {
 size_t pages_work_bytes(const PagesArgs &p) {
     const size_t r = p.n_rows, n = p.n_pages, most = r > n ? r : n;
     const size_t stage = r * p.width > n ? r * p.width : n;
-    return 4 * (H_SIZE + n + 4 * r + 3 * most + stage);
+    return 4 * (H_SIZE + n + 5 * r + 3 * most + stage);
 }
 
 cudaError_t launch_pages_fork(const PagesArgs &p, const int *dst, const int *src, int n, cudaStream_t s) {

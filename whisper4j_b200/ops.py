@@ -89,7 +89,7 @@ class PagedCache:
         n_bytes = ctypes.c_size_t()
         check(self._lib.w4j_op_pages_workspace(self._ref, ctypes.byref(n_bytes)))
         c.work_bytes = n_bytes.value
-        self._work = torch.empty(c.work_bytes, dtype=torch.uint8, device=self.device)
+        self._work = torch.zeros(c.work_bytes, dtype=torch.uint8, device=self.device)
         c.work = self._work.data_ptr()
         self._attend_work = None, 0  # sizes of the last attend and its scratch
 
@@ -108,7 +108,8 @@ class PagedCache:
         check(self._lib.w4j_op_pages_extend(self._ref, r, s, n, _raw_stream(self._index)))
 
     def write(self, layer, rows, start, k, v):
-        """Keys and values (n_tokens, n_kv_head, head_dim) of the tokens that ``extend(rows, start)`` made room for."""
+        """Keys and values (n_tokens, n_kv_head, head_dim) of the tokens that ``extend(rows, start)`` made room for.  Where
+        that was refused, nothing is written to its rows."""
         r, n = self._ints(rows, "rows")
         s, _ = self._ints(start, "start", n + 1)
         ks, tokens = self._tokens(k, "k"), k.shape[0]
