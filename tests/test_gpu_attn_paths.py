@@ -1,0 +1,149 @@
+"""The attention kernels that take calls of many rows: 128-row tiles on the tensor cores, warps for the groups of few rows
+and for all own tokens, and the join of their parts.
+
+A few rows that are not very long go another way, in one launch that needs no scratch; every case here asks the library
+for its scratch first, so that a case which that launch would take fails instead of testing nothing.  The tensor cores
+take shared keys from 24 (head 64) or 16 (head 128) query rows of a group and head on: the groups here have 40 and more
+or at most 15.  Values, tolerances and the reference are test_gpu_attn_shared.py's.
+"""
+import ctypes
+
+import pytest
+
+from .test_gpu_attn_shared import BF16, F16, attend, bad, make, verify
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+def by_parts(s):
+    """Asserts that the call is not one for the launch without scratch."""
+    from whisper4j_b200 import _lib
+    c, (n_seq, nq, heads, _) = s["cache"], s["q"].shape
+    a = _lib.AttnShared(ctypes.pointer(c._c), 0, heads, nq, n_seq, s["shared"].numel(), s["max_shared"], s["max_own"], 1.0)
+    n = ctypes.c_size_t()
+    assert _lib.lib().w4j_op_attn_shared_workspace(ctypes.byref(a), ctypes.byref(n)) == 0 and n.value > 0
+    return s
+
+
+# (rows of each group, heads, key/value heads, queries a row): groups on the tensor cores, on warps of 8 and of 16 rows
+TC, TC_GROUPED, WARP8, WARP16 = ([80, 75], 1, 1, 1), ([41, 40], 12, 4, 1), ([5] * 32, 1, 1, 1), ([3] * 52, 5, 1, 1)
+PATHS = dict(tc=TC, tc_grouped=TC_GROUPED, warp8=WARP8, warp16=WARP16)
+
+
+def case(path, shared, own, **kw):
+    """Every group shares about `shared` tokens; the rows' own numbers of tokens run over `own`."""
+    groups, heads, kv, nq = PATHS[path]
+    nq = kw.pop("nq", nq)
+    per = [max(0, shared - 3 * g % 7) for g in range(len(groups))]
+    lens = [per[g] + own[i % len(own)] for g, n in enumerate(groups) for i in range(n)]
+    return by_parts(make(groups, per, lens, nq=nq, heads=heads, kv=kv, **kw))
+
+
+@pytest.mark.parametrize("page", [8, 24, 64, 136, 1024])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("path", PATHS)
+def test_page_sizes(path, dim, page):
+    s = case(path, 5 * min(page, 150) // 2, [1, 9, 30, 2, 70], page=page, dim=dim, dtype=BF16 if page == 24 else F16)
+    verify(s, attend(s))
+
+
+# shared lengths about the borders of boxes and tiles, none at all, and long ones
+@pytest.mark.parametrize("shared", [0, 1, 63, 64, 65, 127, 129, 192, 1100])
+@pytest.mark.parametrize("path,dtype", [(p, t) for p in PATHS for t in (F16, BF16)])
+def test_shared_lengths(path, dtype, shared):
+    s = case(path, shared, [1, 3, 17], page=16, dim=64 if shared % 2 else 128, dtype=dtype)
+    verify(s, attend(s))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("path", PATHS)
+def test_long_own_parts(path, dim):
+    """Own tokens in several pieces, some of which end before they begin."""
+    s = case(path, 100, [700, 1, 300, 257, 512], page=24, dim=dim)
+    verify(s, attend(s))
+
+
+@pytest.mark.parametrize("heads,kv,nq", [(10, 2, 7), (5, 1, 20), (1, 1, 33), (16, 16, 17)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_several_tiles_of_own_queries(dim, heads, kv, nq):
+    groups = [45, 2, 13]
+    shared = [80, 0, 21]
+    lens = [shared[g] + nq + i % 60 for g, n in enumerate(groups) for i in range(n)]
+    s = by_parts(make(groups, shared, lens, nq=nq, heads=heads, kv=kv, dim=dim, page=8))
+    verify(s, attend(s))
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_rows_that_see_little_or_nothing(path):
+    """No token, fewer tokens than queries, and groups that share nothing."""
+    groups, heads, kv, _ = PATHS[path]
+    n = sum(groups)
+    s = by_parts(make(groups, [0] * len(groups), [(0, 1, 2, 9, 0, 40)[i % 6] for i in range(n)], nq=5, heads=heads, kv=kv))
+    verify(s, attend(s))
+
+
+@pytest.mark.parametrize("what", ["nan", "inf", "-inf"])
+@pytest.mark.parametrize("own", [7, 600])
+@pytest.mark.parametrize("path", PATHS)
+def test_later_tokens_may_be_anything(path, own, what):
+    """Tokens that only a row's last two queries see hold NaN or infinities, in a row's one piece or its last of several.
+    (Not bit by bit as without them: where a tile holds such a number its 16-key sums start from zero.)"""
+    groups, heads, kv, _ = PATHS[path]
+    if path.startswith("warp"):
+        groups = [1] * 160  # with four queries each as few rows as before
+    shared = [50] * len(groups)
+    lens = [50 + own + i % 5 for i in range(sum(groups))]
+    s = by_parts(make(groups, shared, lens, nq=4, heads=heads, kv=kv))
+    c, clean = s["cache"], attend(s)
+    verify(s, clean)
+    rows, table = s["rows"].tolist(), c.table.tolist()
+    for i, n in enumerate(lens):
+        p = table[rows[i]][(n - 2) // 16]
+        c.pool[:, p, :, (n - 2) % 16] = float(what)
+    out = attend(s)
+    assert not torch.isfinite(out[:, 2:]).any()
+    verify({**s, "q": s["q"][:, :2], "lens": [n - 2 for n in lens]}, out[:, :2])
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_nan_in_one_row_stays_there(path):
+    s = case(path, 90, [4, 20, 33])
+    clean = attend(s)
+    s["q"][3] = float("nan")
+    out = attend(s)
+    assert torch.isnan(out[3]).all()
+    keep = [i for i in range(len(s["lens"])) if i != 3]
+    assert torch.equal(out[keep], clean[keep])
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_bad_sequences_are_marked(path):
+    def fresh():
+        return case(path, 70, [5, 30, 44])
+    clean = attend(fresh())
+    n = len(clean)
+    s = fresh()
+    first = int(s["start"][1])  # sequences of the first group
+    others = [i for i in range(n) if i != 2]
+    s["rows"][2] = n + 4
+    assert torch.equal(bad(s, "out of range", [2])[others], clean[others])
+    s = fresh()
+    s["cache"].table[int(s["rows"][2]), (s["lens"][2] - 1) // 16] = 1 << 20
+    assert torch.equal(bad(s, "table entry", [2])[others], clean[others])
+    s = fresh()
+    s["shared"][0] = s["max_shared"] + 1
+    assert torch.equal(bad(s, "shared", list(range(first)))[first:], clean[first:])
+    s = fresh()
+    s["cache"].table[int(s["rows"][0]), 1] = -1  # a shared page: the whole group
+    assert torch.equal(bad(s, "table entry", list(range(first)))[first:], clean[first:])
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_in_place_and_repeated(path):
+    s = case(path, 200, [4, 300, 33])
+    first = attend(s)
+    for _ in range(3):
+        assert torch.equal(attend(s), first)
+    assert torch.equal(attend(s, out=s["q"]), first)  # over the queries
