@@ -339,3 +339,25 @@ def test_writes_behind_any_refusal(n_rows, rows, counts, text):
     refused(c, m, text, step)
     grow(c, m, [0, 1], [2, 3])
     same(c, m)
+
+
+@pytest.mark.parametrize("n", [4, 500, 5000])
+def test_writes_whose_start_descends_are_reported(n):
+    """Both ends are right; the rows behind the fault get their tokens, the row that it deals none stays as it was."""
+    c, m = new_cache(n_layer=1, n_kv=1, n_rows=6000, n_pages=6100, max_tokens=32)
+    grow(c, m, list(range(n)), [9] * n)
+    for at in sorted({0, n // 2, n - 3}):
+        start = starts([2] * n)
+        start[at + 1], start[at + 2] = start[at + 2] + 1, start[at + 1] + 1
+        kv = tokens(c, start[-1], 7)
+        c.write(0, ints(list(range(n))), ints(start), kv[0], kv[1])
+        with pytest.raises(IllegalStateError, match="ascend"):
+            c.check()
+        k, v = kv.view(torch.int16).cpu().numpy()
+        others = [x for x in range(n) if not at <= x <= at + 2]
+        for x in others:
+            m.write(0, [x], [0, 2], k[2 * x:2 * x + 2], v[2 * x:2 * x + 2])
+        pool = c.pool.view(torch.int16).cpu().numpy()
+        pages = [m.held(x)[0] for x in others + [at + 1]]
+        np.testing.assert_array_equal(pool[:, pages], m.pool[:, pages])
+        m.pool[:] = pool

@@ -720,8 +720,10 @@ __global__ void __launch_bounds__(kMoveThreads) k_pages_move(PagesArgs p) {
 // write: the keys and values of the last start[i + 1] - start[i] tokens of row rows[i], a warp per token.  Bound by
 // HBM (14368 tokens of 20 heads of 64: 25 us, 5.9 TB/s both ways); few tokens by the four dependent look-ups of their
 // place, which their data does not wait for.
+//
+// Blocks behind the tokens' look whether start ascends, kStartRun places each, so that no token waits for that.
 // ---------------------------------------------------------------------------
-constexpr int kWriteWarps = 8;
+constexpr int kWriteWarps = 8, kStartRun = 4096;
 
 __global__ void __launch_bounds__(kWriteWarps * 32) k_pages_write(PagesArgs p, int layer, const int *__restrict__ rows,
                                                                   const int *__restrict__ start, int n,
@@ -729,6 +731,14 @@ __global__ void __launch_bounds__(kWriteWarps * 32) k_pages_write(PagesArgs p, i
                                                                   long long k_stride, long long v_stride, int n_tokens) {
     pdl_wait();
     pdl_trigger();
+    const int token_blocks = (n_tokens + kWriteWarps - 1) / kWriteWarps;
+    if ((int)blockIdx.x >= token_blocks) {
+        const int i0 = ((int)blockIdx.x - token_blocks) * kStartRun, i1 = min(n, i0 + kStartRun);
+        bool wrong = i0 == 0 && (start[0] != 0 || start[n] != n_tokens);
+        for (int i = i0 + threadIdx.x; i < i1; i += kWriteWarps * 32) wrong |= start[i] > start[i + 1];
+        if (wrong) atomicOr(p.status, W4J_PAGES_BAD_START);
+        return;
+    }
     const int t = blockIdx.x * kWriteWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (t >= n_tokens) return;
     const int unit = p.head_dim / 8, n_units = p.n_kv_head * unit;
@@ -739,7 +749,6 @@ __global__ void __launch_bounds__(kWriteWarps * 32) k_pages_write(PagesArgs p, i
 #pragma unroll
     for (int i = 0; i < U; ++i)
         if (lane + 32 * i < n_units) kd[i] = __ldg(ks + lane + 32 * i), vd[i] = __ldg(vs + lane + 32 * i);
-    if (t == 0 && lane == 0 && (start[0] != 0 || start[n] != n_tokens)) atomicOr(p.status, W4J_PAGES_BAD_START);
     // the last i with start[i] <= t, 32 places at a time
     int lo = 0, hi = n;
     while (hi - lo > 1) {
@@ -750,7 +759,7 @@ __global__ void __launch_bounds__(kWriteWarps * 32) k_pages_write(PagesArgs p, i
         hi = min(hi, lo + step);
     }
     const int r = rows[lo], s0 = start[lo], s1 = start[lo + 1];
-    if (t < s0 || t >= s1) return;  // behind the last sequence, or a start that does not ascend (reported above)
+    if (t < s0 || t >= s1) return;  // behind the last sequence, or a start that does not ascend: the last blocks report both
     const bool row_ok = r >= 0 && r < p.n_rows;
     const int refused = row_ok ? __ldcg(Work(p).refused + r) : 0;
     if ((refused & ~kRefusedBits) == kRefused) {  // its extension did not take place
@@ -857,7 +866,8 @@ cudaError_t launch_pages_compact(const PagesArgs &p, int *live, cudaStream_t s) 
 
 cudaError_t launch_pages_write(const PagesArgs &p, int layer, const int *rows, const int *start, int n, const void *k,
                                const void *v, long long k_stride, long long v_stride, int n_tokens, cudaStream_t s) {
-    return launch_after<k_pages_write>((n_tokens + kWriteWarps - 1) / kWriteWarps, kWriteWarps * 32, 0, s, 1, p, layer, rows,
+    const int blocks = (n_tokens + kWriteWarps - 1) / kWriteWarps + (n + kStartRun - 1) / kStartRun;
+    return launch_after<k_pages_write>(blocks, kWriteWarps * 32, 0, s, 1, p, layer, rows,
                         start, n, reinterpret_cast<const uint4 *>(k), reinterpret_cast<const uint4 *>(v), k_stride / 8,
                         v_stride / 8, n_tokens);
 }
