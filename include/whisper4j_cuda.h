@@ -340,8 +340,8 @@ int w4j_op_logits_argmax_noalloc(int device, const float *x, int M, int d, const
  * The calls are asynchronous on `stream` and change the cache in stream order; calls on one cache that
  * may run at the same time (several streams without an event between them) are the caller's to order, and
  * so are replays of graphs that hold them.  The integer arguments (rows, start, dst, src) are device arrays
- * that must stay as they are until the call has run.  Each call is all or nothing: where a row is out of
- * range or named twice, a length does not fit or the free pages do not suffice, it changes nothing but
+ * that must stay as they are until the call has run.  Each call but a write is all or nothing: where a row is
+ * out of range or named twice, a length does not fit or the free pages do not suffice, it changes nothing but
  * `status`.  New pages are the lowest free ones in the order of the call's rows; pages that a call lets go
  * of are free for the next call.  page_tokens is a multiple of 8 up to 1024, head_dim 64 or 128.
  * ------------------------------------------------------------------------- */
@@ -373,8 +373,9 @@ int w4j_op_pages_extend(const w4j_pages *cache, const int32_t *rows, const int32
  * elements apart, multiples of 8, both 16-byte aligned: the K and V parts of a fused projection can stay in
  * place).  After w4j_op_pages_extend of the same rows and start.  A row whose last extension was refused takes no
  * tokens until one succeeds (its length has not grown: theirs would be the places of its last ones): they are left
- * out and raise that refusal's status bits again.  A token whose row or page is out of range is left out and raises
- * its status bit. */
+ * out and raise that refusal's status bits again.  Tokens whose row or page is out of range, and tokens that start
+ * deals to no row, are left out and raise their status bit.  So are those of a row that is named twice, but for the index
+ * that it has in its last extension's rows. */
 int w4j_op_pages_write(const w4j_pages *cache, int layer, const int32_t *rows, const int32_t *start, int n,
                        const void *k, int64_t k_stride, const void *v, int64_t v_stride, int n_tokens, void *stream);
 

@@ -341,6 +341,32 @@ def test_writes_behind_any_refusal(n_rows, rows, counts, text):
     same(c, m)
 
 
+@pytest.mark.parametrize("n", [3, 40, 700, 5000])
+def test_writes_that_name_a_row_twice(n):
+    """Two tokens would have one place: the row takes those at the index of its last extension, if any."""
+    c, m = new_cache(n_layer=1, n_kv=1, n_rows=6000, n_pages=6100, max_tokens=32)
+    rows, start = list(range(n)), starts([1 + i % 2 for i in range(n)])
+    grow(c, m, rows, [3] * n)
+    kv = tokens(c, start[-1], 7)
+    for move in (0, 1):  # at their extension's indexes, and all of them at others
+        for i, j in ((0, n - 1), (n - 1, 0), (n // 2, n // 2 + 1)):
+            order = rows[move:] + rows[:move]
+            order[j] = order[i]
+            c.write(0, ints(order), ints(start), kv[0], kv[1])
+            k, v = kv.view(torch.int16).cpu().numpy()
+            for x in range(n):
+                if order.count(order[x]) == 1 or x == order[x]:
+                    m.write(0, [order[x]], [0, start[x + 1] - start[x]], k[start[x]:start[x + 1]], v[start[x]:start[x + 1]])
+            with pytest.raises(IllegalStateError, match="twice"):
+                c.check()
+            same(c, m)
+            kv += 1
+    order = rows[1:] + rows[:1]
+    c.write(0, ints(order), ints(start), kv[0], kv[1])
+    m.write(0, order, start, *kv.view(torch.int16).cpu().numpy())
+    same(c, m)
+
+
 @pytest.mark.parametrize("n", [4, 500, 5000])
 def test_writes_whose_start_descends_are_reported(n):
     """Both ends are right; the rows behind the fault get their tokens, the row that it deals none stays as it was."""

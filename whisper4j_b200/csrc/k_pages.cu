@@ -14,8 +14,9 @@
 // shared memory takes one block that reads everything once (k_pages_small), a fork of more rows a cluster of such blocks:
 // three passes instead of five.
 //
-// Every call is all or nothing: the cluster checks all rows, lengths and the number of free pages before
-// its first write, and a call that cannot be done raises a bit of `status` and changes nothing else.
+// Every call but a write is all or nothing: the cluster checks all rows, lengths and the number of free pages before
+// its first write, and a call that cannot be done raises a bit of `status` and changes nothing else.  A write leaves out
+// the tokens that have no place.
 #include "host_api.cuh"
 #include "pages.cuh"
 #include "w4j_internal.cuh"
@@ -31,18 +32,18 @@ constexpr int kPlanCluster = 8;
 // what a call leaves for its second kernel and for the next pass of its own, in the caller's workspace
 enum { H_PAIRS = 0, H_BAD = 1, H_COUNT = 8, H_MORE = 16, H_SIZE = 32 };  // H_COUNT, H_MORE: one word per block
 
-// What a row's last extension leaves for the writes that follow it: 0, or this number and the bits that refused it.  The
-// row's length has not grown then, and its new tokens' places would be those of its last ones, on pages that other rows may
-// hold too.  (Scratch that nobody has set to zero looks refused once in 2^24.)
+// What a row's last extension leaves for the writes that follow it: the row's index in its list, or this number and the bits
+// that refused it.  The row's length has not grown then, and its new tokens' places would be those of its last ones, on
+// pages that other rows may hold too.  (Scratch that nobody has set to zero looks refused once in 2^24.)
 constexpr int kRefused = 0x57346a00, kRefusedBits = 0xff;
 
 struct Work {
-    int *head, *refused, *list, *mark, *owner, *rank, *slen, *from, *to, *tokens, *stage;
+    int *head, *outcome, *list, *mark, *owner, *rank, *slen, *from, *to, *tokens, *stage;
     __host__ __device__ Work(const PagesArgs &p) {
         const size_t r = p.n_rows, n = p.n_pages, most = r > n ? r : n;
         head = p.work;
-        refused = head + H_SIZE;   // of each row, kept from call to call: only extensions write it
-        list = refused + r;        // free pages, or the holes of a compaction
+        outcome = head + H_SIZE;   // of each row's last extension, kept from call to call: nothing else writes it
+        list = outcome + r;        // free pages, or the holes of a compaction
         mark = list + n;           // the call's index of each row, -1 where it has none
         owner = mark + r;          // fork: the first destination that takes a row over
         rank = owner + r;
@@ -156,11 +157,11 @@ __device__ __forceinline__ bool go_on(const PagesArgs &p, const Work &w, int mor
     return bad == 0;
 }
 
-// The outcome of an extension for the rows it names (threads gid of nt): 0, or the bits that refused it.
+// The outcome of an extension for the rows it names (threads gid of nt), `bad` the bits that refused it.
 __device__ __forceinline__ void note_outcome(const PagesArgs &p, const Work &w, const int *rows, int n, int bad, int gid, int nt) {
     for (int i = gid; i < n; i += nt) {
         const int r = rows[i];
-        if (r >= 0 && r < p.n_rows) w.refused[r] = bad ? kRefused | bad : 0;
+        if (r >= 0 && r < p.n_rows) w.outcome[r] = bad ? kRefused | bad : i;
     }
 }
 
@@ -721,9 +722,27 @@ __global__ void __launch_bounds__(kMoveThreads) k_pages_move(PagesArgs p) {
 // HBM (14368 tokens of 20 heads of 64: 25 us, 5.9 TB/s both ways); few tokens by the four dependent look-ups of their
 // place, which their data does not wait for.
 //
+// A row named twice would have two tokens at one place, in no fixed order.  Its last extension knew it by one index, so at
+// most one of its places in this call's list is that one, and writes; a row at any other index is looked up among all rows
+// of the call.  (Looking all of them up took 4.4 us instead of 3.0 for 64 rows of one token, marking them in a launch
+// before this one 5.4.)
+//
 // Blocks behind the tokens' look whether start ascends, kStartRun places each, so that no token waits for that.
 // ---------------------------------------------------------------------------
 constexpr int kWriteWarps = 8, kStartRun = 4096;
+
+__device__ __forceinline__ bool named_twice(const int *rows, int n, int r) {
+    constexpr int L = 2;  // (more would cost the kernel registers)
+    int named = 0;
+    for (int i0 = threadIdx.x & 31; i0 < n; i0 += 32 * L) {
+        int other[L];
+#pragma unroll
+        for (int x = 0; x < L; ++x) other[x] = i0 + 32 * x < n ? rows[i0 + 32 * x] : -1;
+#pragma unroll
+        for (int x = 0; x < L; ++x) named += other[x] == r;
+    }
+    return __reduce_add_sync(0xffffffffu, named) > 1;
+}
 
 __global__ void __launch_bounds__(kWriteWarps * 32) k_pages_write(PagesArgs p, int layer, const int *__restrict__ rows,
                                                                   const int *__restrict__ start, int n,
@@ -761,12 +780,16 @@ __global__ void __launch_bounds__(kWriteWarps * 32) k_pages_write(PagesArgs p, i
     const int r = rows[lo], s0 = start[lo], s1 = start[lo + 1];
     if (t < s0 || t >= s1) return;  // behind the last sequence, or a start that does not ascend: the last blocks report both
     const bool row_ok = r >= 0 && r < p.n_rows;
-    const int refused = row_ok ? __ldcg(Work(p).refused + r) : 0;
-    if ((refused & ~kRefusedBits) == kRefused) {  // its extension did not take place
-        if (lane == 0) atomicOr(p.status, refused & kRefusedBits);
+    const int outcome = row_ok ? __ldcg(Work(p).outcome + r) : lo, have = row_ok ? row_len(p, r) : 0;
+    if ((outcome & ~kRefusedBits) == kRefused) {  // its extension did not take place
+        if (lane == 0) atomicOr(p.status, outcome & kRefusedBits);
         return;
     }
-    const long long pos = row_ok ? (long long)row_len(p, r) - s1 + t : -1;
+    if (outcome != lo && named_twice(rows, n, r)) {
+        if (lane == 0) atomicOr(p.status, W4J_PAGES_BAD_ROW);
+        return;
+    }
+    const long long pos = row_ok ? (long long)have - s1 + t : -1;
     if (pos < 0) {
         if (lane == 0) atomicOr(p.status, row_ok ? W4J_PAGES_BAD_START : W4J_PAGES_BAD_ROW);
         return;
