@@ -349,7 +349,7 @@ int w4j_op_logits_argmax_noalloc(int device, const float *x, int M, int d, const
 #define W4J_PAGES_FULL 2      /* too few free pages */
 #define W4J_PAGES_TOO_LONG 4  /* a row would outgrow its table */
 #define W4J_PAGES_BAD_START 8 /* start does not begin at 0, does not ascend or does not fit the row lengths */
-#define W4J_PAGES_BAD_PAGE 16 /* a table entry out of range, or one whose page nobody holds */
+#define W4J_PAGES_BAD_PAGE 16 /* a table entry out of range, or in fork, free and compact one whose page nobody holds */
 
 typedef struct w4j_pages {
     int32_t device;

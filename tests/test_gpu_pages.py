@@ -387,3 +387,19 @@ def test_writes_whose_start_descends_are_reported(n):
         pages = [m.held(x)[0] for x in others + [at + 1]]
         np.testing.assert_array_equal(pool[:, pages], m.pool[:, pages])
         m.pool[:] = pool
+
+
+@pytest.mark.parametrize("n_rows", [8, 400, 30000])  # one block, a cluster of blocks for a fork, the cluster's passes
+def test_rows_whose_pages_nobody_holds(n_rows):
+    """Such a page would be dealt out while the row reads it, or its count fall below none."""
+    c, m = new_cache(n_rows=n_rows, n_layer=1, n_kv=1, n_pages=900)
+    grow(c, m, [0, 1], [70, 20])
+    many = list(range(2, min(n_rows, 102)))
+    page = int(m.table[0, 2])
+    c.ref[page] = m.ref[page] = 0
+    for call in (lambda: c.free(ints([1, 0])), lambda: c.fork(ints([2]), ints([0])), lambda: c.fork(ints([0]), ints([1])),
+                 lambda: c.fork(ints(many), ints([1] * (len(many) - 1) + [0])), lambda: c.compact()):
+        refused(c, m, "page", call)
+    c.free(ints([1]))  # a row that has all of its pages
+    m.free([1])
+    same(c, m)

@@ -107,6 +107,11 @@ __device__ __forceinline__ void mark_rows(const PagesArgs &p, const Work &w, con
     }
 }
 
+// A table entry that names no page that somebody holds.
+__device__ __forceinline__ bool no_page(const PagesArgs &p, int page) {
+    return page < 0 || page >= p.n_pages || __ldcg(p.ref + page) <= 0;
+}
+
 // The block's slice of the pages.
 __device__ __forceinline__ void page_slice(const PagesArgs &p, int &lo, int &hi) {
     const int per = (p.n_pages + cluster_size() - 1) / cluster_size();
@@ -193,7 +198,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(PagesArgs p, const 
         if (lane == 0) w.slen[i] = len;
         for (int j = lane; j < np; j += 32) {
             const int page = __ldcg(p.table + (size_t)s * p.width + j);
-            if (page < 0 || page >= p.n_pages) atomicOr(w.head + H_BAD, W4J_PAGES_BAD_PAGE);
+            if (no_page(p, page)) atomicOr(w.head + H_BAD, W4J_PAGES_BAD_PAGE);
             w.stage[(size_t)i * p.width + j] = page;
         }
     }
@@ -203,7 +208,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(PagesArgs p, const 
         const int np = held_pages(p, row_len(p, d));
         for (int j = lane; j < np; j += 32) {
             const int page = __ldcg(p.table + (size_t)d * p.width + j);
-            if (page < 0 || page >= p.n_pages) atomicOr(w.head + H_BAD, W4J_PAGES_BAD_PAGE);
+            if (no_page(p, page)) atomicOr(w.head + H_BAD, W4J_PAGES_BAD_PAGE);
         }
     }
     count_free(p, w, sm);
@@ -324,7 +329,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_free(PagesArgs p, const 
         const int np = held_pages(p, row_len(p, r));
         for (int j = lane; j < np; j += 32) {
             const int page = __ldcg(p.table + (size_t)r * p.width + j);
-            if (page < 0 || page >= p.n_pages) atomicOr(w.head + H_BAD, W4J_PAGES_BAD_PAGE);
+            if (no_page(p, page)) atomicOr(w.head + H_BAD, W4J_PAGES_BAD_PAGE);
         }
     }
     cluster_barrier();
@@ -353,7 +358,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_compact(PagesArgs p, int
         const int np = held_pages(p, row_len(p, r));
         for (int j = lane; j < np; j += 32) {
             const int page = __ldcg(p.table + (size_t)r * p.width + j);
-            if (page < 0 || page >= p.n_pages || __ldcg(p.ref + page) <= 0) atomicOr(w.head + H_BAD, W4J_PAGES_BAD_PAGE);
+            if (no_page(p, page)) atomicOr(w.head + H_BAD, W4J_PAGES_BAD_PAGE);
         }
     }
     cluster_barrier();
@@ -414,7 +419,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_compact(PagesArgs p, int
 // for eight cycles (a beam reorder of 5 rows: 8.4 us with 1024 threads, 7.4 with as many as it needs).
 // ---------------------------------------------------------------------------
 enum PagesOp { OP_FORK, OP_EXTEND, OP_FREE, OP_COMPACT };
-constexpr int kSmallThreads = 1024, kRefs = 8, kEntries = 12;
+constexpr int kSmallThreads = 1024, kRefs = 8 /* the bits of a byte */, kEntries = 12;
 
 // Exclusive prefix sum over the block's threads.
 __device__ __forceinline__ int small_scan(int v, int *sm, int &total) {
@@ -454,6 +459,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
                                                                int *live_out, int n) {
     extern __shared__ int dyn[];
     __shared__ int sm[32], bad;
+    __shared__ unsigned char held[kSmallThreads];  // bit i of byte t: somebody holds page t kRefs + i
     const Work w(p);
     const SmallRows s(dyn, n, p.n_rows, p.n_pages);
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, T = p.page_tokens, W = p.width;
@@ -474,6 +480,12 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
     } else {
 #pragma unroll
         for (int i = 0; i < kRefs; ++i) ref[i] = tid * kRefs + i < p.n_pages ? p.ref[tid * kRefs + i] : 1;
+    }
+    if (OP != OP_EXTEND) {
+        int bits = 0;
+#pragma unroll
+        for (int i = 0; i < kRefs; ++i) bits |= (ref[i] > 0) << i;
+        held[tid] = (unsigned char)bits;
     }
     if (OP != OP_COMPACT) {
         for (int i = tid; i < n; i += threads) {
@@ -525,6 +537,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
     }
     if (OP != OP_EXTEND) {
         bool out = false;
+        auto no_page = [&](int page) { return page < 0 || page >= p.n_pages || !(held[page / kRefs] >> page % kRefs & 1); };
 #pragma unroll
         for (int x = 0; x < kEntries; ++x) {
             const int step = first + x * warps;
@@ -532,8 +545,8 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
             int j;
             const int i = row_of(step, j);
             const bool in_a = j * T < s.len_a[i], in_b = OP == OP_FORK && j * T < s.len_b[i];
-            if (in_a && (was[x] < 0 || was[x] >= p.n_pages)) out = true, was[x] = -1;
-            if (in_b && (shall[x] < 0 || shall[x] >= p.n_pages)) out = true, shall[x] = -1;
+            if (in_a && no_page(was[x])) out = true, was[x] = -1;
+            if (in_b && no_page(shall[x])) out = true, shall[x] = -1;
         }
         if (out) atomicOr(&bad, W4J_PAGES_BAD_PAGE);
     }
@@ -569,9 +582,6 @@ __global__ void __launch_bounds__(kSmallThreads) k_pages_small(PagesArgs p, cons
     const int free_before = small_scan(mine, sm, free_pages);
     if (OP == OP_COMPACT) {
         const int live = p.n_pages - free_pages;
-#pragma unroll
-        for (int x = 0; x < kEntries; ++x)  // an entry whose page nobody holds
-            if (was[x] >= 0 && __ldcg(p.ref + was[x]) <= 0) atomicOr(&bad, W4J_PAGES_BAD_PAGE);
         __syncthreads();
         if (bad) {
             if (tid == 0) atomicOr(p.status, bad);
