@@ -10,6 +10,8 @@ import ctypes
 
 import pytest
 
+from whisper4j_b200._lib import IllegalStateError
+
 from .test_gpu_attn_shared import BF16, F16, attend, bad, make, verify
 
 pytestmark = pytest.mark.gpu
@@ -138,6 +140,43 @@ def test_bad_sequences_are_marked(path):
     s = fresh()
     s["cache"].table[int(s["rows"][0]), 1] = -1  # a shared page: the whole group
     assert torch.equal(bad(s, "table entry", list(range(first)))[first:], clean[first:])
+
+
+@pytest.mark.parametrize("heads,kv,nq,n", [(4, 2, 1, 6), (8, 2, 3, 6), (4, 2, 1, 60), (8, 2, 3, 60)])  # without and with scratch
+def test_groups_that_are_wrong_as_a_whole(heads, kv, nq, n):
+    """Sequences that are in no group are NaN in all heads; those whose group is right are as ever."""
+    def fresh():
+        groups = [n, n // 2, n, n // 3]
+        return make(groups, [40, 17, 0, 33], [45 + i % 9 for i in range(sum(groups))], nq=nq, heads=heads, kv=kv)
+
+    def wrong(change, lost, same):
+        s = fresh()
+        change(s["start"])
+        out = attend(s)
+        with pytest.raises(IllegalStateError, match="ascend"):
+            s["cache"].check()
+        assert torch.isnan(out[lost]).all() and torch.equal(out[same], clean[same])
+
+    clean = attend(fresh())
+    total, g1, g2, g3 = len(clean), n, n + n // 2, 2 * n + n // 2
+    if n == 60:
+        by_parts(fresh())
+
+    def last_early(start):
+        start[4] -= 1
+    wrong(last_early, [total - 1], list(range(total - 1)))
+
+    def first_late(start):
+        start[0] = 1
+    wrong(first_late, [0], list(range(g1, total)))
+
+    def descends(start):  # the third group starts behind the fourth
+        start[2] = g3 + 1
+    wrong(descends, [], list(range(g2)) + list(range(g3, total)))
+
+    def outside(start):  # the third group ends, and the fourth begins, behind the last sequence
+        start[3] = total + 5
+    wrong(outside, list(range(g2, total)), list(range(g2)))
 
 
 @pytest.mark.parametrize("path", PATHS)

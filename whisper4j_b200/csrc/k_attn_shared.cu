@@ -332,11 +332,28 @@ struct WarpTile {
     }
 };
 
+// Whether sequences first .. last are of group gr, found as warp_find does.  Groups that do not ascend may lay claim to the
+// same sequences: a tile of shared keys leaves those of another group alone.  (What warp_find finds does not fall as the
+// sequence grows: where the first and the last one's is gr, so is that of all between.)
+__device__ __forceinline__ bool of_group(const AttnSharedArgs &a, int first, int last, int gr) {
+    int lo = 0, hi = a.n_group;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + (threadIdx.x & 31) * step;
+        const int start = at < hi ? __ldg(a.group_start + at) : 0x7fffffff;
+        const unsigned m0 = __ballot_sync(0xffffffffu, start <= first), m1 = __ballot_sync(0xffffffffu, start <= last);
+        if (__clz(m0 | 1) != __clz(m1 | 1)) return false;
+        lo += (31 - __clz(m0 | 1)) * step;
+        hi = min(hi, lo + step);
+    }
+    return lo == gr;
+}
+
 // ---------------------------------------------------------------------------
 // items: (group tile, head, split) of the shared keys, then (row, head, tile, split) of the rows' own
 // ---------------------------------------------------------------------------
 // Row, its group's first row, length and shared length of sequence `seq`, 0 or what is wrong with it (then rows 0); the whole warp calls it.
-// first: whether this call also looks at all of the groups.
+// first: whether this call also looks at all of the groups, and reports what is wrong with them.  A sequence is of the group
+// where warp_find finds it; where that is right, it gets its results whatever is wrong with others.
 __device__ __forceinline__ int find_row(const AttnSharedArgs &a, int seq, bool first, int &row, int &row0, int &len, int &shared) {
     const PagesArgs &p = a.p;
     const int r = __ldg(a.rows + seq);
@@ -356,7 +373,7 @@ __device__ __forceinline__ int find_row(const AttnSharedArgs &a, int seq, bool f
     if (first) {  // the groups as a whole
         bool out = __ldg(a.group_start) != 0 || __ldg(a.group_start + a.n_group) != a.n_seq;
         for (int i = threadIdx.x & 31; i < a.n_group; i += 32) out |= __ldg(a.group_start + i) > __ldg(a.group_start + i + 1);
-        if (__any_sync(0xffffffffu, out)) bad |= W4J_PAGES_BAD_START;
+        if (out) atomicOr(p.status, W4J_PAGES_BAD_START);
     }
     return bad;
 }
@@ -381,6 +398,7 @@ __global__ void __launch_bounds__(kAsWarps * 32, NT == 1 ? 16 : 12) k_attn_share
     const T *q = reinterpret_cast<const T *>(a.q);
     unsigned item = blockIdx.x * kAsWarps + (threadIdx.x >> 5);
     int seq0, n_rows, head, split, tile, slot, k0, k1, own_len, bad = 0;
+    unsigned mine = 0xffffffffu;  // the tile's rows
     const int *table;
     if (item < a.shared_items) {
         tile = (int)(item % a.shared_tiles);
@@ -395,6 +413,11 @@ __global__ void __launch_bounds__(kAsWarps * 32, NT == 1 ? 16 : 12) k_attn_share
         n_rows = (seq1 - seq0) * c;
         const int r = __ldg(a.rows + seq0), s = min(__ldg(a.shared + gr), a.max_shared);
         if (tile < 0 || tile * R >= n_rows || r < 0 || r >= p.n_rows) return;
+        if (!of_group(a, seq0 + tile * R / c, seq0 + min(n_rows - 1, tile * R + R - 1) / c, gr)) {
+            mine = 0;
+            for (int x = 0; x < R; ++x)
+                if (tile * R + x < n_rows && of_group(a, seq0 + (tile * R + x) / c, seq0 + (tile * R + x) / c, gr)) mine |= 1u << x;
+        }
         table = p.table + (size_t)r * p.width;
         const int len = max(0, min(min(s, __ldg(p.len + r)), p.width * p.page_tokens));
         const int step = ((len + a.shared_splits - 1) / a.shared_splits + 31) / 32 * 32;
@@ -429,12 +452,12 @@ __global__ void __launch_bounds__(kAsWarps * 32, NT == 1 ? 16 : 12) k_attn_share
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int r = tile * R + 8 * n + g;
-        qr[n] = r < n_rows ? q + token_of(r) * a.q_stride + (size_t)(head * a.rep + r % a.rep) * D : nullptr;
+        qr[n] = r < n_rows && mine >> (8 * n + g) & 1 ? q + token_of(r) * a.q_stride + (size_t)(head * a.rep + r % a.rep) * D : nullptr;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int x = tile * R + 8 * n + 2 * qd + i;
             po[n][i] = pm[n][i] = nullptr, lim[n][i] = 0;
-            if (x >= n_rows) continue;
+            if (x >= n_rows || !(mine >> (8 * n + 2 * qd + i) & 1)) continue;
             lim[n][i] = own_len - a.n_query + x % c / a.rep + 1;
             const size_t part = (token_of(x) * a.n_head + head * a.rep + x % a.rep) * a.slots + slot;
             po[n][i] = a.part_o + part * D;
@@ -714,9 +737,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
     const int t0 = min(all, split * per), n = min(all, t0 + per) - t0;
     // the row of this thread: (sequence, query token, head)
     const int r = tile * 128 + (tid & 127);
+    bool mine = r < n_rows && tid < 256;
+    if (!of_group(a, seq0 + tile * 128 / c, seq0 + min(n_rows - 1, tile * 128 + 127) / c, gr))
+        for (int x = 0; x < 32; ++x) {
+            const int seq = seq0 + (r - lane + x) / c;
+            const bool of = of_group(a, seq, seq, gr);
+            if (lane == x && !of) mine = false;
+        }
     size_t part = 0;
     const T *qr = nullptr;
-    if (r < n_rows && tid < 256) {
+    if (mine) {
         const size_t token = (size_t)(seq0 + r / c) * a.n_query + r % c / a.rep;
         const int h = head * a.rep + r % a.rep;
         qr = reinterpret_cast<const T *>(a.q) + token * a.q_stride + (size_t)h * D;
