@@ -269,3 +269,41 @@ def test_refusals():
                 lambda: ops.Int8Linear(layer.weight, layer.scale[:5]), lambda: layer(x.T.contiguous().T)):
         with pytest.raises(ValueError):
             bad()
+
+
+def gelu_of(v, m, ytype, quantised=True):
+    """GELU of the biases v as each of m rows has them, by a product whose sums are 0."""
+    from whisper4j_b200 import _lib, ops
+    from whisper4j_b200._lib import check, lib
+    n = len(v)
+    b = torch.tensor(v, dtype=torch.float32, device="cuda")
+    w, ws = torch.ones(n, 16, dtype=torch.int8, device="cuda"), torch.ones(n, device="cuda")
+    y = torch.full((m, n), 5.0, dtype=ytype, device="cuda")
+    if not quantised:
+        return ops.Int8Linear(w, ws, b)(torch.zeros(m, 16, device="cuda"), epilogue="gelu", out=y)
+    x, xs = torch.zeros(m, 16, dtype=torch.int8, device="cuda"), torch.ones(m, device="cuda")
+    code = {torch.float32: _lib.GGML_F32, torch.float16: _lib.GGML_F16, torch.bfloat16: _lib.GGML_BF16}[ytype]
+    check(lib().w4j_op_linear_i8(0, x.data_ptr(), 16, xs.data_ptr(), m, 16, w.data_ptr(), 16, ws.data_ptr(), n, b.data_ptr(), 1,
+                                 y.data_ptr(), code, n, torch.cuda.current_stream().cuda_stream))
+    return y
+
+
+GELU_ROWS = [(1, False), (3, False), (1, True), (4, True), (8, True), (40, True), (130, True), (1500, True)]  # the kernels
+
+
+@pytest.mark.parametrize("ytype", TYPES)
+@pytest.mark.parametrize("m,quantised", GELU_ROWS)
+def test_gelu_far_from_zero(m, quantised, ytype):
+    """Beyond |v| = 8 GELU is v or, to 1e-18, 0, whatever the number beside it that an epilogue may take along."""
+    far = [-7.6, -7.7, -8.0, -30.0, -100.0, -1e4, -1e19, -1e20, -1e38, 1e-30, 8.0, 100.0, 6e4, 0.0, -0.5, 1.0]
+    v = [far[i % 16] for i in range(480)] + [far[i // 16 % 16] for i in range(480)] + [far[i * 5 % 16] for i in range(480)]
+    y = gelu_of(v, m, ytype, quantised).double()
+    x = torch.tensor(v, dtype=torch.float64, device="cuda").float().double()
+    u = math.sqrt(2 / math.pi) * (x + 0.044715 * x ** 3)
+    want = torch.where(x < -8, 0, x / (1 + torch.exp(-2 * u)))
+    half = 0 if ytype == torch.float32 else torch.finfo(ytype).eps / 2
+    tol = want.abs() * ((8 + 8 * u.abs().clamp(max=50)) * 2 * E + half) + 1e-18 * (x < -7) + torch.finfo(ytype).smallest_normal * torch.finfo(ytype).eps
+    assert ((y - want).abs() <= tol).all()
+    odd = gelu_of([float("nan"), float("inf"), float("-inf"), 2.0] * 400, m, torch.float32, quantised)[:, :4]
+    assert torch.isnan(odd[:, [0, 2]]).all() and (odd[:, 1] == float("inf")).all()  # the formula's -inf x 0 is none
+    assert ((odd[:, 3] - 1.9545976).abs() <= 1e-5).all()

@@ -255,14 +255,17 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// GELU of two numbers in its tanh form, as v / (1 + 2^t) with t = -2 log2(e) u: no cancellation.  t stops at 63 (what is
-// beyond is below 1e-18), so that one reciprocal of the product serves both denominators.
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// GELU of two numbers in its tanh form, as v / (1 + 2^t) with t = -2 log2(e) u: no cancellation, and 0 where 2^t is beyond
+// 32 bits (NaN for -inf, as the formula's -inf x 0).
 __device__ __forceinline__ uint64_t gelu2(uint64_t v) {
     const uint64_t t = mul2(v, fma2(mul2(v, v), both(-0.1029432397f), both(-2.3022081985f)));
-    const uint64_t d = add2(pack(ex2(fminf(lo(t), 63.f)), ex2(fminf(hi(t), 63.f))), both(1.f));
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(lo(d) * hi(d)));
-    return mul2(mul2(v, both(r)), pack(hi(d), lo(d)));
+    const uint64_t d = add2(pack(ex2(lo(t)), ex2(hi(t))), both(1.f));
+    return mul2(v, pack(rcp(lo(d)), rcp(hi(d))));
 }
 __device__ __forceinline__ float gelu(float v) { return lo(gelu2(both(v))); }
 // One output from its integer sum (exact: |sum| <= 2^14 K < 2^31).
