@@ -413,10 +413,11 @@ int w4j_op_pages_compact(const w4j_pages *cache, int32_t *n_live, void *stream);
  *
  * Scores, the softmax and all sums are held in 32 bits; the softmax's weights are rounded to the cache's
  * type before they meet the values.  A sequence whose row, group or shared length is bad, or whose table names a
- * page that is not there, gets NaN, and the cache's status its bit.  Asynchronous on `stream`; results do
- * not depend on the order in which blocks run.
+ * page that is not there, gets NaN, and the cache's status its bit; so do the sequences that a wait inside the
+ * kernels concerns, if it runs out.  Asynchronous on `stream`; results do not depend on the order in which blocks run.
  */
 #define W4J_PAGES_BAD_SHARED 32 /* a shared length over max_shared, or over what a row's queries all see */
+#define W4J_PAGES_TIMEOUT 64    /* a bounded wait inside a kernel ran out */
 
 typedef struct w4j_attn_shared {
     const w4j_pages *cache;
@@ -433,6 +434,12 @@ typedef struct w4j_attn_shared {
 /* Bytes of scratch a call of these sizes needs, 0 for a few rows that are not very long (pointers and strides are not looked at). */
 int w4j_op_attn_shared_workspace(const w4j_attn_shared *args, size_t *bytes);
 int w4j_op_attn_shared(const w4j_attn_shared *args, void *stream);
+
+/*
+ * Test hook: in the next n_calls of w4j_op_attn_shared every wait for keys and values counts on 16 bytes more than
+ * are copied, so that it runs out (a second or two) and the call reports W4J_PAGES_TIMEOUT.  0 turns it off.
+ */
+int w4j_test_attn_shared_waits_run_out(int n_calls);
 
 /* ---------------------------------------------------------------------------
  * A Linear layer in 8-bit integers with a scale for each row of activations and each output channel (the
@@ -457,7 +464,8 @@ int w4j_op_quantize_rows(int device, const void *x, int x_type, int M, int K, in
  * ldx and ldw bytes apart (multiples of 16), 16-byte aligned, columns K up to the next multiple of 16 zero (as
  * w4j_op_quantize_rows leaves them).  K at most 131056.  y: rows ldy elements apart, at least N.  epilogue: 0 =
  * store, 1 = GELU (tanh form in 32 bits; w4j_op_linear looks the same function up by the f16 of its argument),
- * 2 = residual y += ....  y may not overlap the inputs.
+ * 2 = residual y += ....  y may not overlap the inputs.  If a bounded wait inside the kernels runs out, the outputs that
+ * it concerns are NaN (there is no status word to say so).
  */
 int w4j_op_linear_i8(int device, const int8_t *x, int64_t ldx, const float *x_scale, int M, int K, const int8_t *w,
                      int64_t ldw, const float *w_scale, int N, const float *bias, int epilogue, void *y, int y_type,

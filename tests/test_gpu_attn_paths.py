@@ -186,3 +186,26 @@ def test_in_place_and_repeated(path):
     for _ in range(3):
         assert torch.equal(attend(s), first)
     assert torch.equal(attend(s, out=s["q"]), first)  # over the queries
+
+
+@pytest.mark.parametrize("path", ["direct", "cluster", "tc", "warp8", "warp16"])
+def test_waits_that_run_out_are_reported(path):
+    """The hook makes every wait for keys count on more bytes than come; nothing faults, and the next call is as ever."""
+    from whisper4j_b200._lib import check, lib
+    if path == "direct":
+        s = make([2], [20], [30, 41])
+    elif path == "cluster":
+        s = make([1], [0], [3000])
+    else:
+        s = case(path, 70, [5, 30, 44])
+    clean = attend(s)
+    check(lib().w4j_test_attn_shared_waits_run_out(1))
+    try:
+        out = attend(s)
+        with pytest.raises(IllegalStateError, match="ran out"):
+            s["cache"].check()
+    finally:
+        check(lib().w4j_test_attn_shared_waits_run_out(0))
+    assert torch.isnan(out).all()
+    assert torch.equal(attend(s), clean)
+    s["cache"].check()

@@ -224,3 +224,8 @@ def test_scratch_stays_in_proportion():
     assert 0 < many <= 60000 * 6 * 66 * 4
     both = workspace(w, ctypes.byref(attn(c, n_seq=2, max_shared=1 << 30, max_own=1 << 30)))[1]
     assert 0 < both < 256 << 20
+
+
+def test_the_hook_for_waits_refuses_negative_counts():
+    refused(lib().w4j_test_attn_shared_waits_run_out(-1), "n_calls")
+    assert lib().w4j_test_attn_shared_waits_run_out(0) == W4J_OK

@@ -22,6 +22,7 @@ W4J_ERR_CANCELLED = -5
 GGML_F32, GGML_F16, GGML_Q8_0, GGML_BF16 = 0, 1, 8, 30
 
 PAGES_BAD_ROW, PAGES_FULL, PAGES_TOO_LONG, PAGES_BAD_START, PAGES_BAD_PAGE, PAGES_BAD_SHARED = 1, 2, 4, 8, 16, 32
+PAGES_TIMEOUT = 64
 
 
 class W4jError(RuntimeError):
@@ -126,6 +127,7 @@ SIGNATURES = {
     "w4j_op_pages_compact": (_I, [_P, _P, _P]),
     "w4j_op_attn_shared_workspace": (_I, [_P, ctypes.POINTER(_SZ)]),
     "w4j_op_attn_shared": (_I, [_P, _P]),
+    "w4j_test_attn_shared_waits_run_out": (_I, [_I]),
     "w4j_op_quantize_rows": (_I, [_I, _P, _I, _I, _I, _I64, _P, _P, _P, _I64, _P, _P]),
     "w4j_op_linear_i8_layer_workspace": (_I, [_I, _I, ctypes.POINTER(_SZ)]),
     "w4j_op_linear_i8_layer": (_I, [_I, _P, _I, _I64, _P, _P, _I, _I, _P, _I64, _P, _I, _P, _I, _P, _I, _I64, _P, _SZ, _P]),

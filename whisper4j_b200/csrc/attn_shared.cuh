@@ -18,6 +18,7 @@ struct AttnSharedArgs {
     int tile_rows;                   // query rows of a warp's tile, 8 or 16
     unsigned tc_tiles;               // shared keys by k_attn_shared_tc, in tiles of 128 rows (0: warp tiles)
     unsigned shared_tiles, shared_splits, own_tiles, own_splits, slots;
+    unsigned withhold;               // test hook: bytes that every wait for keys or values counts on in vain
     unsigned shared_items, own_items;  // below 2^28: at most 2^24 query rows, and more splits only where there are few
 };
 

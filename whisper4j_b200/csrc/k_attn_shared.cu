@@ -156,7 +156,7 @@ struct WarpTile {
     // barrier for each stage; box: rows of a TMA box.
     __device__ __forceinline__ void run(const PagesArgs &p, const int *table, const int *first, int shared, int head, const CUtensorMap *kmap,
                                         const CUtensorMap *vmap, unsigned char *sm, uint64_t *full, int box, int k0, int k1,
-                                        const int (&lim)[NT][2], int all, float scale_log2, int *bad, int *failed) {
+                                        const int (&lim)[NT][2], int all, float scale_log2, unsigned withhold, int *bad, int *failed) {
         const int lane = threadIdx.x & 31, g = lane >> 2;
         if (k0 >= k1) return;
         const int start = k0 / box * box, n_steps = (k1 - start + STEP - 1) / STEP;  // boxes do not cross pages
@@ -168,7 +168,7 @@ struct WarpTile {
         int page = page_of();
         auto issue = [&](int i) {
             const int at = start + i * STEP, boxes = (min(STEP, k1 - at) + box - 1) / box, st = i % kAsStages;
-            if (lane == 0) mbar_expect_tx(full + st, 2 * NB * boxes * box * 128);
+            if (lane == 0) mbar_expect_tx(full + st, 2 * NB * boxes * box * 128 + withhold);
             if (page < 0 || page >= p.n_pages) *bad = 1, page = 0;
             const int y = (page * p.n_kv_head + head) * p.page_tokens + tok;
             __syncwarp();
@@ -477,13 +477,14 @@ __global__ void __launch_bounds__(kAsWarps * 32, NT == 1 ? 16 : 12) k_attn_share
     int bad_page = 0;
     w.load_q(qr);
     w.run(p, table, nullptr, 0, head, &kmap, &vmap, sm + wi * kAsStages * as_stage(D), full[wi], box, k0, k1, lim, own_len - a.n_query + 1,
-          a.scale_log2, &bad_page, &failed[wi]);
+          a.scale_log2, a.withhold, &bad_page, &failed[wi]);
     if (__any_sync(0xffffffffu, bad_page)) bad |= W4J_PAGES_BAD_PAGE;
     __syncwarp();
-    if (bad || failed[wi]) {
+    if (failed[wi]) bad |= W4J_PAGES_TIMEOUT;
+    if (bad) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) w.m[n][0] = w.m[n][1] = w.l[n][0] = w.l[n][1] = NAN;  // the join hands it on
-        if (lane == 0 && bad) atomicOr(p.status, bad);
+        if (lane == 0) atomicOr(p.status, bad);
     }
     w.store(po, pm);
     if (a.tc_tiles) pdl_wait();
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_
     int bad_page = 0;
     w.load_q(qr);
     w.run(p, p.table + (size_t)row * p.width, p.table + (size_t)row0 * p.width, bad ? 0 : shared, head, &kmap, &vmap, sm, full[wi], box, k0, k1, lim, len - a.n_query + 1, a.scale_log2,
-          &bad_page, &failed);
+          a.withhold, &bad_page, &failed);
     if (__any_sync(0xffffffffu, bad_page)) bad |= W4J_PAGES_BAD_PAGE;
     if (bad && lane == 0) atomicOr(&wrong, bad);
     __syncwarp();
@@ -569,8 +570,8 @@ __global__ void __launch_bounds__(kDirectWarps * 32) k_attn_direct(const __grid_
         }
     w.store(po, pm);
     __syncthreads();
-    if (tid == 0 && wrong) atomicOr(p.status, wrong);
     const bool lost = failed || wrong;
+    if (tid == 0 && lost) atomicOr(p.status, wrong | (failed ? W4J_PAGES_TIMEOUT : 0));
     float *o0 = reinterpret_cast<float *>(sm - wi * kAsStages * as_stage(D));
     auto put = [&](int r, int d, float l, float u, float v) {
         const int qi = tile * R + r;
@@ -790,7 +791,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
                 key += kTcKeys;
                 page = page_of();  // for the next tile
                 if (!__all_sync(0xffffffffu, i < NS || wait_phase(empty + st, (i / NS - 1) & 1, &failed))) break;
-                if (lane == 0) mbar_expect_tx(full + st, boxes * box * 128 * NB);
+                if (lane == 0) mbar_expect_tx(full + st, boxes * box * 128 * NB + a.withhold);
                 __syncwarp();
                 if (lane < boxes)
                     for (int b = 0; b < NB; ++b)
@@ -954,7 +955,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
             l = l * f0 + l1[row] * f1;
             m = top;
             if (qr) a.part_ml[part * 2] = lost ? NAN : m, a.part_ml[part * 2 + 1] = lost ? NAN : l;
-            if (tid == 0 && *(volatile int *)&bad_page) atomicOr(p.status, W4J_PAGES_BAD_PAGE);
+            if (tid == 0 && lost)
+                atomicOr(p.status, (*(volatile int *)&bad_page ? W4J_PAGES_BAD_PAGE : 0) | (*(volatile int *)&failed ? W4J_PAGES_TIMEOUT : 0));
 #pragma unroll 1
             for (int x = 0; x < D; x += 32) {
                 uint32_t o[32];

@@ -156,6 +156,15 @@ extern "C" int w4j_op_attn_shared_workspace(const w4j_attn_shared *x, size_t *by
     return W4J_OK;
 }
 
+// Test hook (w4j_test_attn_shared_waits_run_out): calls whose waits still run out.
+static std::atomic<int> g_withhold_attn{0};
+
+extern "C" int w4j_test_attn_shared_waits_run_out(int n_calls) {
+    if (n_calls < 0) return set_err(W4J_ERR_ARG, "n_calls must be >= 0");
+    g_withhold_attn.store(n_calls);
+    return W4J_OK;
+}
+
 extern "C" int w4j_op_attn_shared(const w4j_attn_shared *x, void *stream) {
     const char *who = "w4j_op_attn_shared";
     AttnSharedArgs a;
@@ -178,6 +187,10 @@ extern "C" int w4j_op_attn_shared(const w4j_attn_shared *x, void *stream) {
     a.rows = x->rows, a.group_start = x->group_start, a.shared = x->shared;
     a.part_o = static_cast<float *>(x->work);
     a.part_ml = a.part_o + (size_t)a.n_seq * a.n_query * a.n_head * a.slots * a.p.head_dim;
+    int n = g_withhold_attn.load();
+    while (n > 0 && !g_withhold_attn.compare_exchange_weak(n, n - 1)) {
+    }
+    a.withhold = n > 0 ? 16 : 0;
     DeviceGuard g(x->cache->device);
     TRY(g.rc());
     CUDA_TRY(launch_attn_shared(a, x->cache->type == W4J_GGML_BF16, stream_of(stream)));

@@ -28,7 +28,8 @@ _STATUS = {_lib.PAGES_BAD_ROW: "a row is out of range or named twice", _lib.PAGE
            _lib.PAGES_TOO_LONG: "a row would outgrow its table",
            _lib.PAGES_BAD_START: "start does not ascend from 0 or does not fit the rows",
            _lib.PAGES_BAD_PAGE: "a table entry names no held page",
-           _lib.PAGES_BAD_SHARED: "a shared length is over max_shared or over what a row's queries see"}
+           _lib.PAGES_BAD_SHARED: "a shared length is over max_shared or over what a row's queries see",
+           _lib.PAGES_TIMEOUT: "a wait inside a kernel ran out"}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
