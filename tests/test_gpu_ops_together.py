@@ -149,3 +149,56 @@ def test_a_step_in_a_graph_gives_what_it_gives_outside():
         assert torch.equal(a, b)
     for c in caches:
         c.check()
+
+
+def test_gradients_are_refused_and_changes_are_counted():
+    """While autograd records, tensors that require a gradient are refused (the outputs would have none in silence), and a
+    tensor that was kept for a backward pass and then written over makes that pass fail."""
+    from whisper4j_b200 import ops
+
+    c = ops.PagedCache(1, 2, 64, 8, 16, 2, 64)
+    rows, start, group, shared = ints([0]), ints([0, 3]), ints([0, 1]), ints([0])
+    kv = torch.randn(2, 3, 2, 64, device="cuda").half()
+    c.extend(rows, start)
+    c.write(0, rows, start, kv[0], kv[1])
+    q = torch.randn(1, 1, 2, 64, device="cuda").half()
+    x, w = torch.randn(3, 32, device="cuda"), torch.nn.Parameter(torch.randn(16, 32, device="cuda"))
+    bias = torch.nn.Parameter(torch.randn(16, device="cuda"))
+    layer = ops.Int8Linear.from_float(w, bias)
+    norm = (torch.ones(32, device="cuda"), torch.zeros(32, device="cuda"))
+
+    def grad(t):
+        return t.detach().clone().requires_grad_()
+
+    y = torch.zeros(3, 16, device="cuda")
+    calls = (lambda: c.write(0, rows, start, grad(kv[0]), kv[1]), lambda: c.attend(0, grad(q), rows, group, shared, 0, 3),
+             lambda: c.attend(0, q, rows, group, shared, 0, 3, out=grad(q)), lambda: ops.quantize_rows(grad(x)),
+             lambda: layer(grad(x)), lambda: layer(x, ln=(grad(norm[0]), norm[1])), lambda: layer(x, out=grad(y)),
+             lambda: layer(x, epilogue="residual", out=grad(y)))
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    with pytest.raises(ValueError, match="gradient"):
+        ops.PagedCache.from_tensors(grad(c.pool), c.ref, c.table, c.len)
+    layer(x), layer(x, ln=norm)  # the layer's own numbers are none
+    a = torch.ones(3, 16, device="cuda", requires_grad=True)
+    for over in (lambda t: layer(x, out=t), lambda t: layer(x, epilogue="residual", out=t)):
+        kept = torch.zeros(3, 16, device="cuda")
+        product = (a * kept).sum()
+        over(kept)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.backward()
+    kept = q.clone()
+    product = (kept * torch.ones_like(q).requires_grad_()).sum()
+    c.attend(0, q, rows, group, shared, 0, 3, out=kept)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    for call in (lambda: c.write(0, rows, start, kv[0], kv[1]), lambda: c.fork(ints([1]), ints([0])), lambda: c.compact()):
+        product = (c.pool[0] * torch.ones_like(c.pool[0]).requires_grad_()).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.backward()
+    with torch.inference_mode():
+        layer(x, out=torch.empty(3, 16, device="cuda"))

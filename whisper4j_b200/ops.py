@@ -2,7 +2,8 @@
 
 Thin bindings of the ``w4j_op_*`` entry points in include/whisper4j_cuda.h: they check what a tensor knows
 (type, device, layout, shape), hand over the current stream of the tensors' device and allocate outputs and
-scratch with torch's allocator, so calls can be captured into CUDA graphs.  Nothing is synchronised.  A refused
+scratch with torch's allocator, so calls can be captured into CUDA graphs.  Nothing is synchronised.  There are no
+gradients: while they are recorded, a tensor that requires one is refused.  A refused
 argument is a ValueError; what only the device can see (a row named twice, no free page) raises a bit of the
 cache's ``status``, which ``PagedCache.check`` reads.
 
@@ -39,6 +40,16 @@ def _need(ok, what):
         raise ValueError(what)
 
 
+def _no_gradient(name):
+    """Of a tensor that requires a gradient."""
+    if torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, and this operator has none: call it under torch.no_grad()")
+
+
+# autograd has to hear of tensors that a call changes through their addresses
+_changed = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
+
+
 def _shape(t):
     return f"{t.dtype} {tuple(t.shape)} strides {tuple(t.stride())} on {t.device}"
 
@@ -72,11 +83,12 @@ class PagedCache:
               (torch.float16, torch.bfloat16),
               "pool must be a contiguous (2 n_layer, n_pages, n_kv_head, page_tokens, head_dim) float16 or bfloat16 tensor")
         _need(pool.is_cuda, "a paged cache lives on a CUDA device")
+        _need(not pool.requires_grad, "a paged cache holds no gradients")
         self.pool, self.ref, self.table, self.len, self.device = pool, ref, table, length, pool.device
         self.dtype, self._index = pool.dtype, pool.device.index
         self.n_layer, self.n_rows = pool.shape[0] // 2, length.numel()
         self.n_kv_head, self.page_tokens, self.head_dim = pool.shape[2:]
-        self._head_strides = (self.head_dim, 1)
+        self._head_strides, self._pools = (self.head_dim, 1), (pool,)
         for t, shape, name in ((ref, (pool.shape[1],), "ref"), (length, (self.n_rows,), "len"),
                                (table, (self.n_rows, table.shape[-1]), "table")):
             _need(t.shape == shape and t.dtype == _INT32 and t.device == self.device and t.is_contiguous(),
@@ -111,6 +123,8 @@ class PagedCache:
     def write(self, layer, rows, start, k, v):
         """Keys and values (n_tokens, n_kv_head, head_dim) of the tokens that ``extend(rows, start)`` made room for.  Where
         that was refused, nothing is written to its rows."""
+        if k.requires_grad or v.requires_grad:
+            _no_gradient("k or v")
         r, n = self._ints(rows, "rows")
         s, _ = self._ints(start, "start", n + 1)
         ks, tokens = self._tokens(k, "k"), k.shape[0]
@@ -118,6 +132,7 @@ class PagedCache:
         _need(v.shape[0] == tokens, "k and v must have the same tokens")
         check(self._lib.w4j_op_pages_write(self._ref, layer, r, s, n, k.data_ptr(), ks, v.data_ptr(), vs, tokens,
                                            _raw_stream(self._index)))
+        _changed(self._pools)
 
     def _tokens(self, t, name):
         """Elements from one token of k or v to the next."""
@@ -133,6 +148,7 @@ class PagedCache:
         d, n = self._ints(dst, "dst")
         s, _ = self._ints(src, "src", n)
         check(self._lib.w4j_op_pages_fork(self._ref, d, s, n, _raw_stream(self._index)))
+        _changed(self._pools)
 
     def free(self, rows):
         """Empty the rows; pages that nobody else holds become free."""
@@ -143,6 +159,7 @@ class PagedCache:
         """Move the held pages to the front of the pool; returns their number as a (1,) int32 tensor."""
         live = torch.empty(1, dtype=torch.int32, device=self.device)
         check(self._lib.w4j_op_pages_compact(self._ref, live.data_ptr(), _raw_stream(self._index)))
+        _changed(self._pools)
         return live
 
     def attend(self, layer, q, rows, group_start, shared, max_shared, max_own, scale=None, out=None):
@@ -156,6 +173,9 @@ class PagedCache:
         if q.dim() != 4 or q.dtype is not self.dtype or q.get_device() != self._index or q.shape[3] != self.head_dim:
             raise ValueError(f"q must be (n_seq, n_query, n_head, {self.head_dim}) {self.dtype} on {self.device}, not {_shape(q)}")
         n_seq, n_query, n_head, _ = q.shape
+        given = out is not None
+        if q.requires_grad or (given and out.requires_grad):
+            _no_gradient("q or out")
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != self._index:
@@ -179,6 +199,8 @@ class PagedCache:
             work = torch.empty(n_bytes, dtype=torch.uint8, device=self.device)
             a.work, a.work_bytes = work.data_ptr(), n_bytes
         check(self._lib.w4j_op_attn_shared(ref, _raw_stream(self._index)))
+        if given:
+            _changed((out,))
         return out
 
     @staticmethod
@@ -222,6 +244,8 @@ def _matrix(t, name):
 def _norm(ln, k, index):
     if ln is None:
         return None, None
+    if ln[0].requires_grad or ln[1].requires_grad:
+        _no_gradient("gamma or beta")
     return _vector(ln[0], k, index, "gamma"), _vector(ln[1], k, index, "beta")
 
 
@@ -229,6 +253,8 @@ def quantize_rows(x, ln=None):
     """x (M, K) -> (q, scale): q (M, K rounded up to 16) int8 = round(LayerNorm?(x) / scale), zeros behind K, and
     scale (M,) = max |row| * (1 / 127) in 32 bits.  ``ln`` is (gamma, beta)."""
     m, k, ld = _matrix(x, "x")
+    if x.requires_grad:
+        _no_gradient("x")
     q = torch.empty(m, (k + 15) // 16 * 16, dtype=torch.int8, device=x.device)
     scale = torch.empty(m, dtype=torch.float32, device=x.device)
     if m:
@@ -241,7 +267,7 @@ def quantize_rows(x, ln=None):
 
 class Int8Linear:
     """y = activation(LayerNorm?(x) W^T + bias) with x quantised row by row in the call and W (N, K) held as int8
-    ``weight`` with a float32 ``scale`` for each output channel."""
+    ``weight`` with a float32 ``scale`` for each output channel: numbers to compute with, not parameters that learn."""
 
     EPILOGUES = {"store": 0, "gelu": 1, "residual": 2}
 
@@ -256,6 +282,7 @@ class Int8Linear:
             padded = torch.zeros(self.n, k16, dtype=torch.int8, device=weight.device)
             padded[:, :self.k] = weight
             weight = padded
+        scale, bias = scale.detach(), None if bias is None else bias.detach()
         self._scale = _vector(scale, self.n, self._index, "scale")
         self._bias = None if bias is None else _vector(bias, self.n, self._index, "bias")
         self.weight, self.scale, self.bias = weight, scale, bias
@@ -265,7 +292,7 @@ class Int8Linear:
     @classmethod
     def from_float(cls, weight, bias=None):
         """Quantise a float weight (N, K), channel by channel."""
-        q, scale = quantize_rows(weight)
+        q, scale = quantize_rows(weight.detach())
         return cls(q[:, :weight.shape[1]], scale, bias)
 
     def __call__(self, x, ln=None, epilogue="store", out=None, out_dtype=None):
@@ -276,6 +303,9 @@ class Int8Linear:
             raise ValueError(f"x must be (M, {self.k}) on {self.device}, not {_shape(x)}")
         if code is None:
             raise ValueError(f"epilogue must be one of {sorted(self.EPILOGUES)}")
+        given = out is not None
+        if x.requires_grad or (given and out.requires_grad):
+            _no_gradient("x or out")
         if out is None:
             _need(code != 2, "a residual needs the tensor that it is added to: out")
             out = torch.empty(m, self.n, dtype=out_dtype or x.dtype, device=x.device)
@@ -296,4 +326,6 @@ class Int8Linear:
         check(self._lib.w4j_op_linear_i8_layer(index, x.data_ptr(), _TYPES[x.dtype], ldx, g, b, m, k, self._weight, self._k16,
                                                self._scale, self.n, self._bias, code, out.data_ptr(), _TYPES[out.dtype], ldy,
                                                work.data_ptr() if n_bytes else None, n_bytes, _raw_stream(index)))
+        if given:
+            _changed((out,))
         return out
