@@ -229,3 +229,29 @@ def test_scratch_stays_in_proportion():
 def test_the_hook_for_waits_refuses_negative_counts():
     refused(lib().w4j_test_attn_shared_waits_run_out(-1), "n_calls")
     assert lib().w4j_test_attn_shared_waits_run_out(0) == W4J_OK
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_arrays_of_32_bit_numbers_are_aligned(off):
+    """The kernels read them as such; an address between two numbers would be a fault of the device."""
+    L, bad, c = lib(), P + off, ctypes.byref(cache())
+    for name in ("ref", "table", "len", "status"):
+        other = cache(**{name: bad})
+        refused(L.w4j_op_pages_free(ctypes.byref(other), P, 1, None), "aligned")
+        refused(L.w4j_op_pages_compact(ctypes.byref(other), None, None), "aligned")
+        refused(L.w4j_op_attn_shared(ctypes.byref(attn(other)), None), "aligned")
+    for a, b in ((bad, P), (P, bad)):
+        refused(L.w4j_op_pages_extend(c, a, b, 1, None), "aligned")
+        refused(L.w4j_op_pages_write(c, 0, a, b, 1, P, 192, P, 192, 1, None), "aligned")
+        refused(L.w4j_op_pages_fork(c, a, b, 1, None), "aligned")
+    refused(L.w4j_op_pages_free(c, bad, 1, None), "aligned")
+    refused(L.w4j_op_pages_compact(c, bad, None), "aligned")
+    for name in ("rows", "group_start", "shared"):
+        refused(L.w4j_op_attn_shared(ctypes.byref(attn(cache(), **{name: bad})), None), "aligned")
+    for kw in (dict(g=bad, b=P), dict(g=P, b=bad)):
+        refused(quantize(**kw), "aligned")
+        refused(layer(**kw), "aligned")
+    for kw in (dict(ws=bad), dict(bias=bad)):
+        refused(linear(**kw), "aligned")
+        refused(layer(**kw), "aligned")
+    refused(linear(xs=bad), "aligned")

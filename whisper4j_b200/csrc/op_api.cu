@@ -12,6 +12,12 @@ namespace {
 
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// arrays of 32-bit numbers
+template <typename... P>
+bool words(const P *...p) {
+    return (aligned(p, 4) && ...);
+}
+
 cudaStream_t stream_of(void *s) { return reinterpret_cast<cudaStream_t>(s); }
 
 int pages_sizes(const w4j_pages *c, const char *who, PagesArgs *out) {
@@ -43,6 +49,8 @@ int w4j::pages_check(const w4j_pages *c, const char *who, PagesArgs *out) {
         return set_err(W4J_ERR_ARG, "%s: a pointer of the cache is null", who);
     if (!aligned(c->pool, 16) || !aligned(c->work, 16))
         return set_err(W4J_ERR_ARG, "%s: pool and work must be 16-byte aligned", who);
+    if (!words(c->ref, c->table, c->len, c->status))
+        return set_err(W4J_ERR_ARG, "%s: ref, table, len and status must be aligned to their type", who);
     if (c->work_bytes < pages_work_bytes(*out))
         return set_err(W4J_ERR_ARG, "%s: work has %zu bytes, w4j_op_pages_workspace asks for %zu", who, c->work_bytes,
                        pages_work_bytes(*out));
@@ -55,6 +63,7 @@ static int pages_call(const w4j_pages *c, const char *who, const void *a, const 
     if (n < 0 || n > c->n_rows) return set_err(W4J_ERR_ARG, "%s: n = %d rows of a cache of %d", who, n, c->n_rows);
     if (n == 0) return 1;
     if (!a || !b) return set_err(W4J_ERR_ARG, "%s: null argument", who);
+    if (!words(a, b)) return set_err(W4J_ERR_ARG, "%s: lists must be aligned to their type", who);
     return W4J_OK;
 }
 
@@ -120,6 +129,7 @@ extern "C" int w4j_op_pages_free(const w4j_pages *c, const int32_t *rows, int n,
 extern "C" int w4j_op_pages_compact(const w4j_pages *c, int32_t *n_live, void *stream) {
     PagesArgs p;
     TRY(pages_check(c, "w4j_op_pages_compact", &p));
+    if (!words(n_live)) return set_err(W4J_ERR_ARG, "w4j_op_pages_compact: n_live must be aligned to its type");
     DeviceGuard g(c->device);
     TRY(g.rc());
     CUDA_TRY(launch_pages_compact(p, n_live, stream_of(stream)));
@@ -177,6 +187,8 @@ extern "C" int w4j_op_attn_shared(const w4j_attn_shared *x, void *stream) {
         return set_err(W4J_ERR_ARG, "%s: strides must be multiples of 8 of at least n_head * head_dim", who);
     if (!aligned(x->q, 16) || !aligned(x->out, 16))
         return set_err(W4J_ERR_ARG, "%s: q and out must be 16-byte aligned", who);
+    if (!words(x->rows, x->group_start, x->shared))
+        return set_err(W4J_ERR_ARG, "%s: rows, group_start and shared must be aligned to their type", who);
     if (!(x->scale > 0) || x->scale > 3e38f) return set_err(W4J_ERR_ARG, "%s: scale must be positive and finite", who);
     const size_t need = attn_shared_work_bytes(a);
     if (need && (!x->work || !aligned(x->work, 16) || x->work_bytes < need))
@@ -205,11 +217,12 @@ static int check_rows(const char *who, const void *x, int x_type, int M, int K, 
     if (ldx < K) return set_err(W4J_ERR_ARG, "%s: ldx must be at least K", who);
     if (!aligned(x, x_type == W4J_GGML_F32 ? 4 : 2)) return set_err(W4J_ERR_ARG, "%s: x must be aligned to its type", who);
     if ((ln_g == nullptr) != (ln_b == nullptr)) return set_err(W4J_ERR_ARG, "LayerNorm needs both gamma and beta");
+    if (!words(ln_g, ln_b)) return set_err(W4J_ERR_ARG, "%s: gamma and beta must be aligned to their type", who);
     return W4J_OK;
 }
 
-static int check_product(const char *who, int M, int K, const int8_t *w, int64_t ldw, int N, int epilogue, const void *y, int y_type,
-                         int64_t ldy) {
+static int check_product(const char *who, int M, int K, const int8_t *w, int64_t ldw, const float *w_scale, int N, const float *bias,
+                         int epilogue, const void *y, int y_type, int64_t ldy) {
     if (!float_type(y_type)) return set_err(W4J_ERR_ARG, "%s: y_type must be F32 (0), F16 (1) or BF16 (30), not %d", who, y_type);
     if (M < 1 || N < 1 || K < 1 || M > 1 << 24 || N > 1 << 24) return set_err(W4J_ERR_ARG, "%s: bad shape (%d x %d x %d)", who, M, K, N);
     if ((int64_t)M * N > (int64_t)1 << 38) return set_err(W4J_ERR_ARG, "%s: M * N must be at most 2^38", who);
@@ -218,6 +231,7 @@ static int check_product(const char *who, int M, int K, const int8_t *w, int64_t
         return set_err(W4J_ERR_ARG, "%s: w must be 16-byte aligned with rows a multiple of 16 bytes of at least K apart", who);
     if (ldy < N || !aligned(y, y_type == W4J_GGML_F32 ? 4 : 2))
         return set_err(W4J_ERR_ARG, "%s: y must be aligned to its type with ldy at least N", who);
+    if (!words(w_scale, bias)) return set_err(W4J_ERR_ARG, "%s: w_scale and bias must be aligned to their type", who);
     if (epilogue < 0 || epilogue > 2) return set_err(W4J_ERR_ARG, "epilogue must be 0, 1 or 2");
     return W4J_OK;
 }
@@ -229,7 +243,7 @@ extern "C" int w4j_op_quantize_rows(int device, const void *x, int x_type, int M
     TRY(check_rows(who, x, x_type, M, K, ldx, ln_g, ln_b));
     if (ldq < K || ldq % 16 || !aligned(q, 16))
         return set_err(W4J_ERR_ARG, "%s: q must be 16-byte aligned with ldq a multiple of 16 of at least K", who);
-    if (!aligned(scale, 4)) return set_err(W4J_ERR_ARG, "%s: scale must be aligned to its type", who);
+    if (!words(scale)) return set_err(W4J_ERR_ARG, "%s: scale must be aligned to its type", who);
     DeviceGuard g(device);
     TRY(g.rc());
     CUDA_TRY(launch_quantize_rows(QuantizeArgs{x, x_type, M, K, ldx, ln_g, ln_b, q, ldq, scale}, stream_of(stream)));
@@ -241,7 +255,8 @@ extern "C" int w4j_op_linear_i8(int device, const int8_t *x, int64_t ldx, const 
                                 void *y, int y_type, int64_t ldy, void *stream) {
     const char *who = "w4j_op_linear_i8";
     if (!x || !x_scale || !w || !w_scale || !y) return set_err(W4J_ERR_ARG, "%s: null argument", who);
-    TRY(check_product(who, M, K, w, ldw, N, epilogue, y, y_type, ldy));
+    TRY(check_product(who, M, K, w, ldw, w_scale, N, bias, epilogue, y, y_type, ldy));
+    if (!words(x_scale)) return set_err(W4J_ERR_ARG, "%s: x_scale must be aligned to its type", who);
     if (ldx < K || ldx % 16 || !aligned(x, 16))
         return set_err(W4J_ERR_ARG, "%s: x must be 16-byte aligned with rows a multiple of 16 bytes of at least K apart", who);
     DeviceGuard g(device);
@@ -266,7 +281,7 @@ extern "C" int w4j_op_linear_i8_layer(int device, const void *x, int x_type, int
     const char *who = "w4j_op_linear_i8_layer";
     if (!x || !w || !w_scale || !y) return set_err(W4J_ERR_ARG, "%s: null argument", who);
     TRY(check_rows(who, x, x_type, M, K, ldx, ln_g, ln_b));
-    TRY(check_product(who, M, K, w, ldw, N, epilogue, y, y_type, ldy));
+    TRY(check_product(who, M, K, w, ldw, w_scale, N, bias, epilogue, y, y_type, ldy));
     const size_t need = linear_i8_layer_work(M, K);
     if (need && (!work || !aligned(work, 16) || work_bytes < need))
         return set_err(W4J_ERR_ARG, "%s: work must be 16-byte aligned and hold the %zu bytes that w4j_op_linear_i8_layer_workspace asks for",
