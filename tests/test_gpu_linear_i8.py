@@ -307,3 +307,32 @@ def test_gelu_far_from_zero(m, quantised, ytype):
     odd = gelu_of([float("nan"), float("inf"), float("-inf"), 2.0] * 400, m, torch.float32, quantised)[:, :4]
     assert torch.isnan(odd[:, [0, 2]]).all() and (odd[:, 1] == float("inf")).all()  # the formula's -inf x 0 is none
     assert ((odd[:, 3] - 1.9545976).abs() <= 1e-5).all()
+
+
+@pytest.mark.parametrize("epilogue", ["store", "gelu", "residual"])
+@pytest.mark.parametrize("ln", [False, True])
+@pytest.mark.parametrize("m,k", [(1, 1280), (2, 512), (4, 384), (5, 512), (300, 512), (2100, 256)])
+def test_outputs_over_the_inputs(m, k, ln, epilogue):
+    """h = h + W LayerNorm(h) in place, and outputs that lie across their inputs."""
+    from whisper4j_b200 import _lib, ops
+    g = torch.Generator("cuda").manual_seed(m)
+    layer = ops.Int8Linear.from_float(torch.randn(k, k, device="cuda", generator=g) * k ** -0.5, torch.randn(k, device="cuda", generator=g))
+    norm = (1 + 0.1 * torch.randn(k, device="cuda", generator=g), 0.1 * torch.randn(k, device="cuda", generator=g)) if ln else None
+    x = torch.randn(m, k, device="cuda", generator=g)
+    # the rows quantised first, then the product: whole numbers behind a LayerNorm are these
+    q, s = ops.quantize_rows(x, norm)
+    want = x.clone()
+    _lib.check(_lib.lib().w4j_op_linear_i8(0, q.data_ptr(), k, s.data_ptr(), m, k, layer.weight.data_ptr(), k, layer.scale.data_ptr(), k,
+                                           layer.bias.data_ptr(), ops.Int8Linear.EPILOGUES[epilogue], want.data_ptr(), 0, k,
+                                           torch.cuda.current_stream().cuda_stream))
+    for _ in range(5):
+        h = x.clone()
+        assert torch.equal(layer(h, ln=norm, epilogue=epilogue, out=h), want)
+        wide = torch.zeros(m, 2 * k, device="cuda")
+        wide[:, :k] = x
+        if epilogue == "residual":
+            base = wide[:, k // 2:k // 2 + k].clone()
+            out = layer(wide[:, :k], ln=norm, epilogue=epilogue, out=wide[:, k // 2:k // 2 + k])
+            assert ((out - base - (want - x)).abs() <= 4 * E * (out.abs() + want.abs() + x.abs() + base.abs())).all()  # four sums
+        else:
+            assert torch.equal(layer(wide[:, :k], ln=norm, epilogue=epilogue, out=wide[:, k // 2:k // 2 + k]), want)

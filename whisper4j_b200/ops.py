@@ -241,6 +241,14 @@ def _matrix(t, name):
     return m, n, ld
 
 
+def _overlap(a, lda, b, ldb):
+    """Whether the bytes that two matrices span have some in common."""
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    a1 = a0 + ((a.shape[0] - 1) * lda + a.shape[1]) * a.element_size()
+    b1 = b0 + ((b.shape[0] - 1) * ldb + b.shape[1]) * b.element_size()
+    return a0 < b1 and b0 < a1
+
+
 def _norm(ln, k, index):
     if ln is None:
         return None, None
@@ -296,7 +304,8 @@ class Int8Linear:
         return cls(q[:, :weight.shape[1]], scale, bias)
 
     def __call__(self, x, ln=None, epilogue="store", out=None, out_dtype=None):
-        """x (M, K) -> (M, N) of ``out_dtype`` (default: x's), or into ``out``; epilogue "gelu", or "residual": out += ..."""
+        """x (M, K) -> (M, N) of ``out_dtype`` (default: x's), or into ``out``, which may overlap x; epilogue "gelu", or
+        "residual": out += ..."""
         m, k, ldx = _matrix(x, "x")
         index, code = self._index, self.EPILOGUES.get(epilogue)
         if k != self.k or x.get_device() != index:
@@ -323,6 +332,14 @@ class Int8Linear:
             check(self._lib.w4j_op_linear_i8_layer_workspace(m, k, size))
             n_bytes = self._work_bytes[m] = size.value
         work = torch.empty(n_bytes, dtype=torch.int8, device=x.device) if n_bytes else None
+        if given and not n_bytes and _overlap(x, ldx, out, ldy):
+            # one launch would write over rows that some of its blocks have still to read
+            q, scale = quantize_rows(x, ln)
+            check(self._lib.w4j_op_linear_i8(index, q.data_ptr(), self._k16, scale.data_ptr(), m, k, self._weight, self._k16,
+                                             self._scale, self.n, self._bias, code, out.data_ptr(), _TYPES[out.dtype], ldy,
+                                             _raw_stream(index)))
+            _changed((out,))
+            return out
         check(self._lib.w4j_op_linear_i8_layer(index, x.data_ptr(), _TYPES[x.dtype], ldx, g, b, m, k, self._weight, self._k16,
                                                self._scale, self.n, self._bias, code, out.data_ptr(), _TYPES[out.dtype], ldy,
                                                work.data_ptr() if n_bytes else None, n_bytes, _raw_stream(index)))
