@@ -109,6 +109,41 @@ def test_later_tokens_may_be_anything(path, own, what):
     verify({**s, "q": s["q"][:, :2], "lens": [n - 2 for n in lens]}, out[:, :2])
 
 
+@pytest.mark.parametrize("hidden", [64, 128, 192, 320])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("path", list(PATHS) + ["direct"])
+def test_keys_that_score_minus_infinity(path, dtype, hidden):
+    """The first keys score -inf and the others about -200, where no rounding may lose them: their values' mean, for scores
+    that are equal.  (Weights are 1 then, and sums of up to 512 numbers of the type's half step each: 2 u |v| at most.)"""
+    if path == "direct":
+        s = make([2], [400], [410, 403], heads=4, kv=2, dtype=dtype)
+    else:
+        s = case(path, 400, [3, 10], dtype=dtype)
+    c, q = s["cache"], s["q"]
+    page, dim = c.page_tokens, c.head_dim
+    c.pool.nan_to_num_()
+    c.pool[0] = 0
+    q.zero_()
+    q[..., 0], q[..., 1] = 1, 1
+    c.pool[0, ..., 1] = -200  # times scale: -25
+    table, rows, start = c.table.tolist(), s["rows"].tolist(), s["start"].tolist()
+    for i, n in enumerate(s["lens"]):
+        for j in range(hidden // page):
+            c.pool[0, table[rows[i]][j], ..., 0] = float("-inf")
+    out = attend(s, scale=1.0)
+    u = torch.finfo(dtype).eps / 2
+    rep = q.shape[2] // c.n_kv_head
+    for i, n in enumerate(s["lens"]):
+        g = max(x for x in range(len(start) - 1) if start[x] <= i)
+        shared = int(s["shared"][g])
+        pages = [table[rows[start[g]]][j] if (j + 1) * page <= shared else table[rows[i]][j] for j in range(-(-n // page))]
+        v = c.pool[1, pages].transpose(0, 1).reshape(c.n_kv_head, -1, dim)[:, hidden:n].double().repeat_interleave(rep, 0)
+        want, a = v.mean(1), v.abs().mean(1)
+        tol = a * (2 * u + 2 ** -13) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        assert ((out[i, 0].double() - want).abs() <= tol).all(), i
+    c.check()
+
+
 @pytest.mark.parametrize("path", PATHS)
 def test_nan_in_one_row_stays_there(path):
     s = case(path, 90, [4, 20, 33])

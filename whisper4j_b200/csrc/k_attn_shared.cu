@@ -883,10 +883,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
 #pragma unroll
             for (int x = 0; x < 64; x += 2)
                 mx[x / 2 & 3] = max3(mx[x / 2 & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
-            float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * a.scale_log2;
-            if (top == kNone) top = i == 0 ? 0.f : m;
+            const float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * a.scale_log2;
             if (i == 0) {
-                m = top;
+                m = top;  // kNone until a key has scored more than -inf
             } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
                 ok = __all_sync(0xffffffffu, wait_phase(pv_done + (bi ^ 2), ((i - 1) >> 1) & 1, &failed));
                 if (!ok) break;
@@ -904,7 +903,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
                     tmem_store32(o_at + x, o);
                 }
             }
-            const uint64_t base2 = pair(__float_as_uint(-m), __float_as_uint(-m));
+            const float from = m == kNone ? 0.f : -m;
+            const uint64_t base2 = pair(__float_as_uint(from), __float_as_uint(from));
             uint64_t sum[2] = {0, 0};
 #pragma unroll
             for (int x = 0; x < 64; x += 2) {
@@ -950,8 +950,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_shared_tc(const __grid_c
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (w == 0) {
             const bool lost = *(volatile int *)&failed || *(volatile int *)&bad_page;
-            // (a warpgroup without a key has m = 0, l = 0 and O = 0)
-            const float top = l1[row] == 0.f ? m : fmaxf(m, m1[row]), f0 = ex2(m - top), f1 = l1[row] == 0.f ? 0.f : ex2(m1[row] - top);
+            // (a warpgroup whose keys all scored -inf, or without one, has l = 0 and O = 0, and nothing to say about the maximum)
+            const bool none0 = l == 0.f, none1 = l1[row] == 0.f;
+            const float top = none0 ? m1[row] : none1 ? m : fmaxf(m, m1[row]);
+            const float f0 = none0 ? 0.f : ex2(m - top), f1 = none1 ? 0.f : ex2(m1[row] - top);
             l = l * f0 + l1[row] * f1;
             m = top;
             if (qr) a.part_ml[part * 2] = lost ? NAN : m, a.part_ml[part * 2 + 1] = lost ? NAN : l;
