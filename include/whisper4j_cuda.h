@@ -402,8 +402,8 @@ int w4j_op_pages_compact(const w4j_pages *cache, int32_t *n_live, void *stream);
  * same first shared[g] tokens, on the same pages or on copies of them: their keys and values are read
  * once for the whole group, through the table of its first sequence.  Query t (0 <= t < n_query) of a
  * sequence sees the first len - n_query + t + 1 tokens of its row: the last n_query tokens are the queries'
- * own, already written.  A query that sees no token, or none that scores more than -inf, gets zeros.  What lies behind a row's length, and what a
- * query does not see, may be anything, NaN included.
+ * own, already written.  A query that sees no token, or none that scores more than -inf, gets zeros.  What lies
+ * behind a row's length, and what a query does not see, may be anything, NaN included.
  *
  *   q, out  [n_seq n_query] tokens of [n_head][head_dim] of the cache's type, q_stride and out_stride
  *           elements apart (multiples of 8, 16-byte aligned); query head h reads key/value head h / (n_head / n_kv_head)

@@ -77,6 +77,31 @@ def test_several_tiles_of_own_queries(dim, heads, kv, nq):
     verify(s, attend(s))
 
 
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(6, 6, 64, F16), (8, 2, 64, BF16), (5, 1, 128, F16)])
+@pytest.mark.parametrize("nq,shared,lens", [(448, 0, [448, 300, 449, 600]), (130, 200, [329, 330, 331, 700, 513]), (1000, 0, [1000])])
+def test_prompts(nq, shared, lens, heads, kv, dim, dtype):
+    """A whole prompt's queries at once, one of them longer than its row; all queries of a row against 64 bits together."""
+    s = by_parts(make([len(lens)], [shared], lens, nq=nq, heads=heads, kv=kv, dim=dim, dtype=dtype, page=24))
+    out, c, rows, table = attend(s), s["cache"], s["rows"].tolist(), s["cache"].table.tolist()
+    u, scale = torch.finfo(dtype).eps / 2, dim ** -0.5
+    t0 = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    for i, n in enumerate(lens):
+        pages = table[rows[i]][:-(-n // 24)]
+        k, v = (c.pool[w, pages].transpose(0, 1).reshape(kv, -1, dim)[:, :n].double().repeat_interleave(heads // kv, 0) for w in (0, 1))
+        x = s["q"][i].double().transpose(0, 1)
+        see = n - nq + torch.arange(nq, device="cuda")[:, None] >= torch.arange(n, device="cuda")
+        sc = (scale * x @ k.transpose(1, 2)).masked_fill(~see, float("-inf"))
+        S = (scale * x.abs() @ k.abs().transpose(1, 2)).amax(2, keepdim=True)
+        p = torch.nan_to_num(torch.softmax(sc, 2))
+        o, A = p @ v, p @ v.abs()
+        e = (dim + 8) * 2 ** -24 * S + 8 * 2 ** -24 * (1 + S)
+        tol = A * (u + 2 * e + n * 2 ** -24) + n * t0 / 2 * v.abs().max() + o.abs() * u + t0
+        got = out[i].double().transpose(0, 1)
+        assert ((got - o).abs() <= tol).all(), i
+        assert not got[:, :max(0, nq - n)].any()
+    c.check()
+
+
 @pytest.mark.parametrize("path", PATHS)
 def test_rows_that_see_little_or_nothing(path):
     """No token, fewer tokens than queries, and groups that share nothing."""
@@ -244,3 +269,32 @@ def test_waits_that_run_out_are_reported(path):
     assert torch.isnan(out).all()
     assert torch.equal(attend(s), clean)
     s["cache"].check()
+
+
+def test_a_pool_beyond_32_bits():
+    """Planes of 4 GiB: new pages, copies, reads and moves at the far end of the last ones."""
+    from whisper4j_b200 import ops
+    n_pages, page = 1 << 17, 16
+    c = ops.PagedCache(2, 8, 128, n_pages, page, 4, 512, dtype=BF16)
+    c.ref.fill_(1)
+    c.ref[-40:] = 0  # the others are somebody else's
+    rows, start = torch.tensor([0, 1], dtype=torch.int32, device="cuda"), torch.tensor([0, 300, 323], dtype=torch.int32, device="cuda")
+    kv = torch.randn(2, 323, 8, 128, device="cuda").to(BF16)
+    c.extend(rows, start)
+    c.write(1, rows, start, kv[0], kv[1])
+    c.fork(torch.tensor([2], dtype=torch.int32, device="cuda"), rows[:1])
+    c.check()
+    assert c.table[:3, 0].tolist() == [n_pages - 40, n_pages - 21, n_pages - 40] and int(c.table[2, 18]) == n_pages - 19
+    for n in (3, 160):  # without and with scratch
+        order = [i % 3 for i in range(n)]
+        lens = [(300, 23, 300)[i] for i in order]
+        q = torch.randn(n, 1, 8, 128, device="cuda").to(BF16)
+        s = dict(cache=c, q=q, rows=torch.tensor(order, dtype=torch.int32, device="cuda"), lens=lens, max_shared=0, max_own=300,
+                 start=torch.arange(n + 1, dtype=torch.int32, device="cuda"), shared=torch.zeros(n, dtype=torch.int32, device="cuda"))
+        out = attend(s, layer=1)
+        verify(s, out, layer=1)
+    c.ref[5:9] = 0  # holes, far from the pages that close them
+    assert int(c.compact()) == n_pages - 40 + 22 - 4
+    assert sorted(set(c.table[:3].flatten().tolist()) & {5, 6, 7, 8}) == [5, 6, 7, 8]
+    assert torch.equal(attend(s, layer=1), out)
+    c.check()
