@@ -336,3 +336,32 @@ def test_outputs_over_the_inputs(m, k, ln, epilogue):
             assert ((out - base - (want - x)).abs() <= 4 * E * (out.abs() + want.abs() + x.abs() + base.abs())).all()  # four sums
         else:
             assert torch.equal(layer(wide[:, :k], ln=norm, epilogue=epilogue, out=wide[:, k // 2:k // 2 + k]), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.int32, torch.float8_e4m3fn])
+def test_types_of_outputs_are_refused_as_arguments(dtype):
+    from whisper4j_b200 import ops
+    layer = ops.Int8Linear.from_float(torch.randn(30, 40, device="cuda"))
+    for m in (1, 40):
+        with pytest.raises(ValueError, match="out"):
+            layer(torch.randn(m, 40, device="cuda"), out_dtype=dtype)
+        with pytest.raises(ValueError, match="out"):
+            layer(torch.randn(m, 40, device="cuda"), out=torch.empty(m, 30, device="cuda").to(dtype))
+
+
+@pytest.mark.parametrize("ldy", [(1 << 15) + 8, (1 << 15) + 9])  # whole boxes of outputs, and single ones
+def test_outputs_and_rows_beyond_32_bits(ldy):
+    from whisper4j_b200 import ops
+    m, n, k = (1 << 17) + 3, (1 << 15) + 8, 48
+    layer = ops.Int8Linear.from_float(torch.randn(n, k, device="cuda"), torch.randn(n, device="cuda"))
+    x = torch.randn(m, k, device="cuda")
+    y = torch.empty(m, ldy, device="cuda", dtype=torch.float16)[:, :n]
+    layer(x, out=y)
+    for a in (0, (1 << 16) - 40, m - 80):
+        part = layer(x[a:a + 80], out_dtype=torch.float16).double()
+        assert ((y[a:a + 80].double() - part).abs() <= 2 * torch.finfo(torch.float16).eps * part.abs() + 2 ** -24).all()
+    del y
+    wide = torch.randn(80, 1040, device="cuda", dtype=torch.float16).repeat(1 << 15, 1)
+    q, s = ops.quantize_rows(wide)
+    want = ops.quantize_rows(wide[:80].clone())
+    assert torch.equal(q[-80:], want[0]) and torch.equal(s[-80:], want[1]) and torch.equal(q[80 << 14:][:80], want[0])

@@ -317,6 +317,7 @@ class Int8Linear:
             _no_gradient("x or out")
         if out is None:
             _need(code != 2, "a residual needs the tensor that it is added to: out")
+            _need(out_dtype is None or out_dtype in _TYPES, "out_dtype must be float32, float16 or bfloat16")
             out = torch.empty(m, self.n, dtype=out_dtype or x.dtype, device=x.device)
             ldy = self.n
         else:
