@@ -44,7 +44,9 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Two numbers rounded to the cache's type (half a step of it: 2^-11 or 2^-8 relative), `lo` in the low half.
+// Two numbers rounded to the cache's type (half a step of it: 2^-11 or 2^-8 relative), `lo` in the low half: outputs, and the
+// softmax's weights, because the tensor cores take both operands of P V in one 16-bit type.  (In place of 32-bit weights that
+// takes the error of the measured cases from 2.1e-4 to 2.6e-4 .. 2.9e-4 in fp16, 1.7e-3 to 2.3e-3 in bf16.)
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -101,7 +103,7 @@ __device__ __forceinline__ bool wait_phase(uint64_t *bar, unsigned parity, int *
 // as TMA boxes (128-byte swizzle, read back by ldmatrix), so that a stage is in flight while another is worked on
 // without holding registers, and no warp waits for another.  Bound by HBM and, where rows are short, by the look-ups
 // that each begins with: 256 rows x 20 heads of 64, 257 tokens each on average, 61 us, 5.5 TB/s (112 us with fragments
-// loaded straight into registers); 64 x 5 rows of 111 tokens behind 227 shared ones 55 us, 4.6 TB/s.
+// loaded straight into registers); 64 x 5 rows of 111 tokens behind 227 shared ones 56 us, 4.5 TB/s.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     uint32_t r;

@@ -261,7 +261,8 @@ __device__ __forceinline__ float rcp(float x) {
     return y;
 }
 // GELU of two numbers in its tanh form, as v / (1 + 2^t) with t = -2 log2(e) u: no cancellation, and 0 where 2^t is beyond
-// 32 bits (NaN for -inf, as the formula's -inf x 0).
+// 32 bits (NaN for -inf, as the formula's -inf x 0).  The XU pipe is 46 % busy with them in the pair product; one reciprocal
+// for two numbers needs the exponent limited and a select to 0 behind that limit: 106 us instead of 93 for 12000 rows.
 __device__ __forceinline__ uint64_t gelu2(uint64_t v) {
     const uint64_t t = mul2(v, fma2(mul2(v, v), both(-0.1029432397f), both(-2.3022081985f)));
     const uint64_t d = add2(pack(ex2(lo(t)), ex2(hi(t))), both(1.f));

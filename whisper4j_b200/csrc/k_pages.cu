@@ -836,7 +836,8 @@ int small_threads(const PagesArgs &p, int n) {
 
 // A fork of more rows: the same by a cluster, whose blocks all plan for all rows and pages and share the tables'
 // entries out.  One block's time is its instructions (4 layers of large-v3-turbo, with the move: 5 rows 8.1 us on one, 8.7
-// on eight, 40 rows 12.0 and 10.0, 320 rows 19.4 and 14.7; 640 rows 23.4 where k_pages_fork took 37.4).
+// on eight, 40 rows 12.0 and 10.0, 320 rows 19.4 and 14.7; 640 rows 23.4 where k_pages_fork took 37.4;
+// the look at who holds the pages has since added 0.1 to 0.5 us, to k_pages_fork 3).
 constexpr int kForkBlocks = 8, kForkSteps = 6;
 int fork_threads(const PagesArgs &p, int n, int &blocks) {
     const long long steps = (long long)n * ((p.width + 31) / 32), by_pages = (p.n_pages + 32 * kRefs - 1) / (32 * kRefs);
